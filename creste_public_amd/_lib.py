@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libcreste_hip.so")
 
 ABI_VERSION = 12         # creste_abi_version() of the library this binding was written against
 ACT_NONE, ACT_RELU, ACT_SWISH = 0, 1, 2
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
 PREC_F32, PREC_BF16, PREC_BF16X3, PREC_BF16X6, PREC_F16X3 = 0, 1, 2, 3, 4
 
 
@@ -161,6 +162,18 @@ SIGNATURES = {
     "creste_trajectory_scores_f32": (_i, [_vp, _i, _i, _f, _i, _i, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp]),
     "creste_trajectory_scores_grouped_f32": (_i, [_vp, _i, _i, _f, _i, _i, _vp, _vp, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
     "creste_irl_visitation_mix_f32": (_i, [_vp, _vp, _vp, _vp, _vp, _f, _i, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "creste_linear_ce_workspace_bytes": (_i64, [_i64, _i64, _i, _i, _i]),
+    "creste_linear_ce_forward": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i, _i, _i64, _f, _i, _vp, _vp, _vp, _vp, _vp, _i64,
+                                      _vp]),
+    "creste_linear_ce_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i, _i, _i64, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp,
+                                       _i64, _vp]),
+    "creste_dropout": (_i, [_vp, _vp, _vp, _i64, _i, C.c_double, _i64, _i64, _vp, _vp]),
+    "creste_gated_recurrence_chunk_steps": (_i, []),
+    "creste_gated_recurrence_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "creste_gated_recurrence_forward": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp,
+                                             _i64, _vp]),
+    "creste_gated_recurrence_backward": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i,
+                                              _vp, _vp, _vp, _vp, _i64, _vp]),
     "creste_hip_model_load": (_i, [C.c_char_p, _i, C.POINTER(_vp)]),
     "creste_hip_model_free": (_i, [_vp]),
     "creste_hip_model_info": (C.c_char_p, [_vp]),

@@ -5,7 +5,9 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
+from torch.autograd.function import once_differentiable
+
+from . import _lib, ops
 from .ops import HipLibraryError, _stream
 from .train_ops import as_act
 
@@ -162,3 +164,41 @@ class SmoothL1Fn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gl):
         return None, ctx.g * gl, None, None, None, None, None, None
+
+
+class LinearCEFn(torch.autograd.Function):
+    """softmax cross entropy of x w^T / temperature against class labels, without the logits (csrc/linear_ce.hip); the backward
+    forms them again in pieces of the classes.  -> (loss, nll [N])"""
+
+    @staticmethod
+    def forward(ctx, x, weight, labels, ignore_index, temperature, reduction):
+        loss, nll, lse2, stat = ops.linear_ce(x, weight, labels, ignore_index, temperature, reduction)
+        ctx.save_for_backward(x, weight, labels, lse2, stat)
+        ctx.args = (ignore_index, temperature, reduction)
+        ctx.mark_non_differentiable(nll)
+        return loss, nll
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gl, _):
+        x, weight, labels, lse2, stat = ctx.saved_tensors
+        gx, gw = ops.linear_ce_bwd(x, weight, labels, lse2, stat, gl, *ctx.args, need_x=ctx.needs_input_grad[0],
+                                   need_w=ctx.needs_input_grad[1])
+        return gx, gw, None, None, None, None
+
+
+def linear_cross_entropy(x, weight, labels, ignore_index: int = -100, temperature: float = 1.0, reduction: str = "mean"):
+    """Cross entropy of the linear classifier `weight` [V,D] on features x [...,D] (fp32 / bf16 / fp16, one type for both) against
+    labels [...] int64, over any number of classes and without ever holding the N x V logits:
+        z = x weight^T / temperature;  nll = logsumexp(z) - z[label], 0 where label == ignore_index
+    -> (loss, nll): loss = mean of nll over the rows that count (0 when none does) or their sum, a differentiable fp32 scalar;
+    nll [...] fp32, not differentiable.  Features are expected to be finite.  A label that names neither a class nor
+    ignore_index makes the loss and its gradients NaN.  fp32 features are multiplied with 22 significand bits."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise HipLibraryError("linear_cross_entropy: x [...,D] expected")
+    lead = tuple(x.shape[:-1])
+    if not isinstance(labels, torch.Tensor) or tuple(labels.shape) != lead:
+        raise HipLibraryError(f"linear_cross_entropy: labels must have the shape {lead} of the features' rows")
+    loss, nll = LinearCEFn.apply(x.reshape(-1, x.shape[-1]) if x.numel() else x.reshape(0, x.shape[-1]), weight, labels.reshape(-1),
+                                 ignore_index, temperature, reduction)
+    return loss, nll.reshape(lead)

@@ -1457,3 +1457,224 @@ def expected_svf(policy, expert_xy, fov_u8, T, ds, temperature, sharpen=True, ze
                                            sharp.data_ptr(), svf.data_ptr(), states.data_ptr(),
                                            grid.data_ptr(), _stream()), "expected_svf")
     return svf, states, grid
+
+
+# ---- operators of a temporal classification head: features of frames -> gated linear recurrence -> dropout -> cross entropy over a
+# large set of classes.  Any of fp32 / bf16 / fp16; the autograd forms are train_ops.gated_recurrence / train_ops.dropout /
+# loss_ops.linear_cross_entropy.
+_DTYPE_CODE = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+
+
+def _features(t, name: str, ndim=None, like=None) -> int:
+    """-> dtype code of a feature tensor; raises unless it is a fp32 / bf16 / fp16 GPU tensor (of `ndim` dimensions; of the type
+    and on the device of `like`)"""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise HipLibraryError(f"{name}: expected a CUDA/HIP tensor (the HIP path has no CPU fallback)")
+    if t.dtype not in _DTYPE_CODE:
+        raise HipLibraryError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    if ndim is not None and t.dim() != ndim:
+        raise HipLibraryError(f"{name}: expected {ndim} dimensions, got shape {tuple(t.shape)}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise HipLibraryError(f"{name}: {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+    return _DTYPE_CODE[t.dtype]
+
+
+def _plain(t, dtype, shape, device, name: str) -> torch.Tensor:
+    """a contiguous tensor of this type, shape and device -- or an error (values are copied if only the strides differ)"""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device:
+        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise HipLibraryError(f"{name}: expected {dtype} {tuple(shape)} on {device}, got {got}")
+    return t.contiguous()
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """last dimension contiguous, no negative or overlapping-write concerns (the tensor is only read); copied otherwise"""
+    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _int64(v, name: str) -> int:
+    """a 64-bit pattern as the signed value ctypes takes"""
+    v = int(v)
+    if not -(1 << 63) <= v < (1 << 64):
+        raise HipLibraryError(f"{name}: {v} does not fit 64 bits")
+    return v - (1 << 64) if v >= (1 << 63) else v
+
+
+def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """y_i = keep_i ? x_i / (1 - p) : 0 (+ residual_i) -> a new contiguous tensor.  keep_i depends on (seed, offset, i) alone, i = the
+    element's index in row-major order of x's shape, whatever its strides (a non-contiguous x is copied first): one word of
+    Philox4x32-10 per element, compared with round(p 2^32).  Calls that shall draw independently take different offsets (or seeds).
+    `seed`: an int, or a CUDA int64 tensor (seed, offset) read when the kernel runs, so that a captured call can draw anew
+    on each replay (its second element is added to `offset`)."""
+    code = _features(x, "dropout: x")
+    if not 0.0 <= float(p) <= 1.0:
+        raise HipLibraryError(f"dropout: p = {p} outside [0, 1]")
+    state = None
+    if isinstance(seed, torch.Tensor):
+        state, seed = _plain(seed, torch.int64, (2,), x.device, "dropout: seed tensor"), 0
+    x_ = x.detach().contiguous()
+    r_ = None
+    if residual is not None:
+        if tuple(residual.shape) != tuple(x.shape):
+            raise HipLibraryError(f"dropout: residual {tuple(residual.shape)} beside x {tuple(x.shape)}")
+        _features(residual, "dropout: residual", like=x)
+        r_ = residual.detach().contiguous()
+    seed, offset = _int64(seed, "dropout: seed"), _int64(offset, "dropout: offset")
+    y = torch.empty_like(x_, memory_format=torch.contiguous_format)
+    if x_.numel():
+        with _on(x.device):
+            _lib.check(_lib.load().creste_dropout(x_.data_ptr(), r_.data_ptr() if r_ is not None else None, y.data_ptr(), x_.numel(),
+                                                  code, float(p), seed, offset, state.data_ptr() if state is not None else None,
+                                                  _stream()), "dropout")
+    return y
+
+
+class _on:
+    """make `device` the current one for a call (no work when it already is)"""
+
+    def __init__(self, device):
+        self.dev = device.index if device.index is not None else torch.cuda.current_device()
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.dev:
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *exc):
+        if self.prev != self.dev:
+            torch.cuda.set_device(self.prev)
+
+
+def _recurrence_args(gate, x, h0, lengths):
+    code = _features(gate, "gated_recurrence: gate", 3)
+    _features(x, "gated_recurrence: x", 3, like=gate)
+    if tuple(x.shape) != tuple(gate.shape):
+        raise HipLibraryError(f"gated_recurrence: gate {tuple(gate.shape)} beside x {tuple(x.shape)}")
+    B, T, Cc = gate.shape
+    if h0 is not None:
+        h0 = _plain(h0.detach() if isinstance(h0, torch.Tensor) else h0, torch.float32, (B, Cc), gate.device, "gated_recurrence: h0")
+    if lengths is not None:
+        lengths = _plain(lengths, torch.int64, (B,), gate.device, "gated_recurrence: lengths")
+    return code, _rows(gate.detach()), _rows(x.detach()), h0, lengths
+
+
+def gated_recurrence(gate: torch.Tensor, x: torch.Tensor, h0: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                     save: bool = False):
+    """h_t = sigmoid(gate_t) h_(t-1) + (1 - sigmoid(gate_t)) x_t for [B,T,C] sequences -> (h [B,T,C], h_last [B,C] fp32[, starts]).
+    h0 [B,C] fp32 (zeros if None) is the state in front of the first step and h_last the one behind a sequence's last step: a stream
+    is served step by step by handing h_last back as h0.  lengths [B] int64 (clamped to [0, T]): h is 0 behind a sequence's end and the
+    values there are not used.  The state is fp32 throughout.  gate / x may have any batch and time strides (time-major buffers); a
+    last dimension that is not contiguous is copied.  save=True: also the states gated_recurrence_bwd needs."""
+    code, g_, x_, h0, lengths = _recurrence_args(gate, x, h0, lengths)
+    B, T, Cc = g_.shape
+    dev = g_.device
+    h = torch.empty((B, T, Cc), dtype=g_.dtype, device=dev)
+    lib = _lib.load()
+    if h.numel() == 0:
+        last = h0.clone() if h0 is not None else torch.zeros((B, Cc), dtype=torch.float32, device=dev)
+        return (h, last, torch.empty(0, dtype=torch.float32, device=dev)) if save else (h, last)
+    with _on(dev):
+        last = torch.empty((B, Cc), dtype=torch.float32, device=dev)
+        starts = None
+        if save:
+            starts = torch.empty((-(-T // lib.creste_gated_recurrence_chunk_steps()), B, Cc), dtype=torch.float32, device=dev)
+        nb = lib.creste_gated_recurrence_workspace_bytes(B, T, Cc)
+        work = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
+        _lib.check(lib.creste_gated_recurrence_forward(
+            g_.data_ptr(), g_.stride(0), g_.stride(1), x_.data_ptr(), x_.stride(0), x_.stride(1),
+            h0.data_ptr() if h0 is not None else None, lengths.data_ptr() if lengths is not None else None, B, T, Cc, code,
+            h.data_ptr(), last.data_ptr(), starts.data_ptr() if save else None, work.data_ptr(), nb, _stream()),
+            "gated_recurrence_forward")
+    return (h, last, starts) if save else (h, last)
+
+
+def gated_recurrence_bwd(gate, x, lengths, starts, gh, gh_last=None):
+    """cotangents gh [B,T,C] (the features' type) and gh_last [B,C] fp32 (or None) -> (ggate, gx [B,T,C], gh0 [B,C] fp32)"""
+    code, g_, x_, _, lengths = _recurrence_args(gate, x, None, lengths)
+    B, T, Cc = g_.shape
+    dev = g_.device
+    _features(gh, "gated_recurrence: gh", 3, like=gate)
+    if tuple(gh.shape) != (B, T, Cc):
+        raise HipLibraryError(f"gated_recurrence: gh {tuple(gh.shape)} beside gate {(B, T, Cc)}")
+    if gh_last is not None:
+        gh_last = _plain(gh_last.detach(), torch.float32, (B, Cc), dev, "gated_recurrence: gh_last")
+    gg, gx = torch.empty((B, T, Cc), dtype=g_.dtype, device=dev), torch.empty((B, T, Cc), dtype=g_.dtype, device=dev)
+    if gg.numel() == 0:
+        return gg, gx, gh_last.clone() if gh_last is not None else torch.zeros((B, Cc), dtype=torch.float32, device=dev)
+    d_ = _rows(gh.detach())
+    lib = _lib.load()
+    starts = _plain(starts, torch.float32, (-(-T // lib.creste_gated_recurrence_chunk_steps()), B, Cc), dev, "gated_recurrence: starts")
+    with _on(dev):
+        gh0 = torch.empty((B, Cc), dtype=torch.float32, device=dev)
+        nb = lib.creste_gated_recurrence_workspace_bytes(B, T, Cc)
+        work = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
+        _lib.check(lib.creste_gated_recurrence_backward(
+            g_.data_ptr(), g_.stride(0), g_.stride(1), x_.data_ptr(), x_.stride(0), x_.stride(1), d_.data_ptr(), d_.stride(0),
+            d_.stride(1), gh_last.data_ptr() if gh_last is not None else None, lengths.data_ptr() if lengths is not None else None,
+            starts.data_ptr(), B, T, Cc, code, gg.data_ptr(), gx.data_ptr(), gh0.data_ptr(), work.data_ptr(), nb, _stream()),
+            "gated_recurrence_backward")
+    return gg, gx, gh0
+
+
+def _linear_ce_args(x, w, labels, temperature, reduction):
+    code = _features(x, "linear_cross_entropy: x", 2)
+    _features(w, "linear_cross_entropy: weight", 2, like=x)
+    if w.shape[1] != x.shape[1] or w.shape[0] < 1 or w.shape[1] < 1:
+        raise HipLibraryError(f"linear_cross_entropy: x {tuple(x.shape)} beside weight {tuple(w.shape)}")
+    labels = _plain(labels, torch.int64, (x.shape[0],), x.device, "linear_cross_entropy: labels")
+    if reduction not in ("mean", "sum"):
+        raise HipLibraryError(f"linear_cross_entropy: reduction {reduction!r} (mean or sum)")
+    if not 0.0 < float(temperature) < float("inf"):
+        raise HipLibraryError(f"linear_cross_entropy: temperature {temperature}")
+    return code, _rows(x.detach()), _rows(w.detach()), labels
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def linear_ce(x, w, labels, ignore_index: int = -100, temperature: float = 1.0, reduction: str = "mean"):
+    """forward of loss_ops.linear_cross_entropy -> (loss [], nll [N], lse2 [N], stat [2]), fp32"""
+    code, x_, w_, labels = _linear_ce_args(x, w, labels, temperature, reduction)
+    N, D = x_.shape
+    V, dev = w_.shape[0], x_.device
+    loss, stat = torch.empty((), dtype=torch.float32, device=dev), torch.empty(2, dtype=torch.float32, device=dev)
+    nll, lse2 = torch.empty(N, dtype=torch.float32, device=dev), torch.empty(N, dtype=torch.float32, device=dev)
+    if N == 0:
+        return loss.zero_(), nll, lse2, stat.zero_()
+    lib = _lib.load()
+    with _on(dev):
+        nb = lib.creste_linear_ce_workspace_bytes(N, V, D, code, 0)
+        work = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
+        _lib.check(lib.creste_linear_ce_forward(x_.data_ptr(), _row_stride(x_), w_.data_ptr(), _row_stride(w_), labels.data_ptr(), N, V, D,
+                                                code, int(ignore_index), float(temperature), int(reduction == "mean"),
+                                                loss.data_ptr(), nll.data_ptr(), lse2.data_ptr(), stat.data_ptr(),
+                                                work.data_ptr(), nb, _stream()), "linear_ce_forward")
+    return loss, nll, lse2, stat
+
+
+def linear_ce_bwd(x, w, labels, lse2, stat, g_loss, ignore_index: int = -100, temperature: float = 1.0, reduction: str = "mean",
+                  need_x: bool = True, need_w: bool = True):
+    """gradient of linear_ce for the cotangent g_loss (one fp32 element) -> (gx, gw); None for what is not needed"""
+    code, x_, w_, labels = _linear_ce_args(x, w, labels, temperature, reduction)
+    N, D = x_.shape
+    V, dev = w_.shape[0], x_.device
+    gx = torch.empty((N, D), dtype=x_.dtype, device=dev) if need_x else None
+    if N == 0:
+        return gx, torch.zeros((V, D), dtype=x_.dtype, device=dev) if need_w else None
+    gw = torch.empty((V, D), dtype=x_.dtype, device=dev) if need_w else None
+    if not (need_x or need_w):
+        return gx, gw
+    lse2 = _plain(lse2, torch.float32, (N,), dev, "linear_cross_entropy: lse2")
+    stat = _plain(stat, torch.float32, (2,), dev, "linear_cross_entropy: stat")
+    g_loss = _plain(g_loss.reshape(1), torch.float32, (1,), dev, "linear_cross_entropy: cotangent")
+    lib = _lib.load()
+    with _on(dev):
+        nb = lib.creste_linear_ce_workspace_bytes(N, V, D, code, 1)
+        work = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
+        _lib.check(lib.creste_linear_ce_backward(x_.data_ptr(), _row_stride(x_), w_.data_ptr(), _row_stride(w_), labels.data_ptr(), N, V,
+                                                 D, code, int(ignore_index), float(temperature), int(reduction == "mean"),
+                                                 lse2.data_ptr(), stat.data_ptr(), g_loss.data_ptr(),
+                                                 gx.data_ptr() if need_x else None, gw.data_ptr() if need_w else None,
+                                                 work.data_ptr(), nb, _stream()), "linear_ce_backward")
+    return gx, gw

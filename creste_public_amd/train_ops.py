@@ -22,6 +22,7 @@ import ctypes as C
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 from .ops import Act, HipLibraryError, _stream
@@ -605,3 +606,61 @@ def reward_forward_train(net, x: torch.Tensor) -> torch.Tensor:
         eng = net._train_engine = RewardTrainEngine(net)
     eng.use_graphs = bool(getattr(net, "train_graphs", False))
     return RewardFn.apply(eng, x, *eng.params())
+
+
+class DropoutFn(torch.autograd.Function):
+    """ops.dropout under autograd: no mask is kept, the backward draws the same words again (a seed TENSOR must therefore still hold
+    its values when the backward runs; autograd's version check raises if it was written in between)."""
+
+    @staticmethod
+    def forward(ctx, x, p, seed, offset, residual):
+        ctx.args = (p, None if isinstance(seed, torch.Tensor) else seed, offset)
+        if isinstance(seed, torch.Tensor):
+            ctx.save_for_backward(seed)
+        return ops.dropout(x, p, seed, offset, residual)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        p, seed, offset = ctx.args
+        if seed is None:
+            seed, = ctx.saved_tensors
+        gx = ops.dropout(gy, p, seed, offset) if ctx.needs_input_grad[0] else None
+        return gx, None, None, None, gy if ctx.needs_input_grad[4] else None
+
+
+def dropout(x, p: float, seed, offset: int = 0, residual=None):
+    """y = x / (1 - p) where an element is kept, else 0 (+ residual); see ops.dropout for what decides.  Differentiable in x and
+    residual.  fp32 / bf16 / fp16, any shape."""
+    return DropoutFn.apply(x, p, seed, offset, residual)
+
+
+class GatedRecurrenceFn(torch.autograd.Function):
+    """ops.gated_recurrence under autograd; keeps gate, x and one fp32 state per chunk of steps, not h"""
+
+    @staticmethod
+    def forward(ctx, gate, x, h0, lengths):
+        ctx.set_materialize_grads(False)
+        if not any(ctx.needs_input_grad[:3]):
+            return ops.gated_recurrence(gate, x, h0, lengths)
+        h, last, starts = ops.gated_recurrence(gate, x, h0, lengths, save=True)
+        ctx.save_for_backward(gate, x, lengths, starts)
+        return h, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gh, gh_last):
+        if gh is None and gh_last is None:
+            return None, None, None, None
+        gate, x, lengths, starts = ctx.saved_tensors
+        if gh is None:
+            gh = torch.zeros((), dtype=gate.dtype, device=gate.device).expand(gate.shape)
+        gg, gx, gh0 = ops.gated_recurrence_bwd(gate, x, lengths, starts, gh, gh_last)
+        want = ctx.needs_input_grad
+        return gg if want[0] else None, gx if want[1] else None, gh0 if want[2] else None, None
+
+
+def gated_recurrence(gate, x, h0=None, lengths=None):
+    """h_t = f_t h_(t-1) + (1 - f_t) x_t, f = sigmoid(gate), over [B,T,C] sequences -> (h [B,T,C], h_last [B,C] fp32); arguments as
+    ops.gated_recurrence.  Differentiable in gate, x and h0, through both outputs."""
+    return GatedRecurrenceFn.apply(gate, x, h0, lengths)

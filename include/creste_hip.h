@@ -32,6 +32,10 @@ extern "C" {
 #define CRESTE_ERR_HIP (-2)
 #define CRESTE_ERR_NOCONV (-3) /* value iteration hit max_sweeps */
 
+#define CRESTE_DT_F32 0 /* element types of the sequence / classification operators */
+#define CRESTE_DT_BF16 1
+#define CRESTE_DT_F16 2
+
 #define CRESTE_ACT_NONE 0
 #define CRESTE_ACT_RELU 1
 #define CRESTE_ACT_SWISH 2 /* x * sigmoid(x) (efficientnet_pytorch Swish) */
@@ -691,6 +695,48 @@ int creste_trajectory_scores_grouped_f32(const float* xy, int N, int T, float ma
 int creste_irl_visitation_mix_f32(const float* exp_svf_raw, const uint8_t* fov, const float* visit_expert,
                                   const float* visit_cf, const int* cf_ptr, float alpha, int B, int64_t HW, float* svf,
                                   float* exp_svf, float* cf_total, float* policy_svf, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Operators of a temporal classification head (no reference counterpart).  dtype = CRESTE_DT_*.
+ *
+ * Softmax cross entropy over V classes straight from the features (csrc/linear_ce.hip): z = x w^T / temperature, x [N][ldx],
+ * w [V][ldw] (strides in elements, D of them used), labels [N] int64; a row whose label is ignore_index does not count, one whose
+ * label names no class makes loss and gradients NaN.  No N x V buffer.
+ *   forward : loss [1] (mean over the counted rows, 0 if there are none, or sum), nll [N] (0 where ignored), lse2 [N] (log-sum-exp
+ *             in log2 units) and stat [2] = {sum nll, count} for the backward.
+ *   backward: gx [N][D], gw [V][D] (contiguous, the features' type; either may be NULL) for the cotangent g_loss [1].
+ * work: workspace_bytes(..., train = 0) for the forward, train = 1 for the backward; -1 = sizes out of range. */
+int64_t creste_linear_ce_workspace_bytes(int64_t N, int64_t V, int D, int dtype, int train);
+int creste_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* labels, int64_t N, int64_t V,
+                             int D, int dtype, int64_t ignore_index, float temperature, int mean, float* loss, float* nll,
+                             float* lse2, float* stat, void* work, int64_t work_bytes, void* stream);
+int creste_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* labels, int64_t N, int64_t V,
+                              int D, int dtype, int64_t ignore_index, float temperature, int mean, const float* lse2,
+                              const float* stat, const float* g_loss, void* gx, void* gw, void* work, int64_t work_bytes,
+                              void* stream);
+
+/* Dropout (csrc/dropout.hip): y_i = keep_i ? x_i / (1 - p) : 0 (+ residual_i), 0 <= p <= 1, n elements.  keep_i = word_i >=
+ * round(p 2^32), word_i = word i mod 4 of Philox4x32-10 with counter (i div 4, offset) and key seed, 64 bits each.  The backward is
+ * the same call on the cotangent.  state (may be NULL): device int64[2], seed = state[0] and offset += state[1] instead of the
+ * arguments, so that a captured call draws anew on every replay.  y may be x. */
+int creste_dropout(const void* x, const void* residual, void* y, int64_t n, int dtype, double p, int64_t seed, int64_t offset,
+                   const int64_t* state, void* stream);
+
+/* Gated linear recurrence over time (csrc/recurrence.hip), f = sigmoid(gate): h_t = f_t h_(t-1) + (1 - f_t) x_t per sequence and
+ * channel, state in fp32.  gate / x / gh: element (b, t, c) at b * sb + t * st + c; h / ggate / gx: contiguous [B][T][C]; h0 / h_last /
+ * gh_last / gh0: [B][C] fp32 (h0 NULL: zeros; gh_last NULL: zeros; gh0 NULL: not wanted).  lengths [B] int64 (NULL: all T):
+ * steps behind a sequence's length are 0 in h and the gradients and leave the state alone.
+ *   starts: state before every chunk_steps() steps, [chunks][B * C] fp32, chunks = ceil(T / chunk_steps()); forward writes it when
+ *           not NULL, backward reads it. */
+int creste_gated_recurrence_chunk_steps(void);
+int64_t creste_gated_recurrence_workspace_bytes(int64_t B, int64_t T, int64_t C);
+int creste_gated_recurrence_forward(const void* gate, int64_t gate_sb, int64_t gate_st, const void* x, int64_t x_sb, int64_t x_st,
+                                    const float* h0, const int64_t* lengths, int64_t B, int64_t T, int64_t C, int dtype, void* h,
+                                    float* h_last, float* starts, void* work, int64_t work_bytes, void* stream);
+int creste_gated_recurrence_backward(const void* gate, int64_t gate_sb, int64_t gate_st, const void* x, int64_t x_sb, int64_t x_st,
+                                     const void* gh, int64_t gh_sb, int64_t gh_st, const float* gh_last, const int64_t* lengths,
+                                     const float* starts, int64_t B, int64_t T, int64_t C, int dtype, void* ggate, void* gx,
+                                     float* gh0, void* work, int64_t work_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Python-free deployment entry (csrc/plan_runtime.cpp).  reference scripts/runtime/compile.py:160-210 traces
