@@ -343,6 +343,102 @@ __global__ __launch_bounds__(512, 2) void ce_gemm_kernel(CeArgs p) {
   }
 }
 
+// ------------------------------------------------------------------------------------------------------- few rows
+// LOSS for at most 32 rows: bound by reading w once, so no LDS and no copy of the operands -- a wave streams 64 classes from
+// memory straight into the matrix instructions, one group of loads (128 bytes of each class row) ahead.  fp32 goes through
+// the fp32 matrix instruction (32 x 32 x 2, 157 TF: 32 rows need 16 products a loaded element, well below it).  The lane
+// halves take alternate 16-byte pieces of the contraction in both operands, which for fp32 makes a 16-byte load feed four instructions.
+template <int DT>
+__global__ __launch_bounds__(256) void ce_few_kernel(CeArgs p, int D) {
+  constexpr int EB = DT == CRESTE_DT_F32 ? 4 : 2, STEP = 32 / EB;      // elements both halves take per load
+  typedef int iv4 __attribute__((ext_vector_type(4)));
+  __shared__ float2 sh[4][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, lh = lane >> 5;
+  const int m0 = blockIdx.x * kCeTile + wave * 64;
+  const int row = li < p.n ? li : p.n - 1;
+  const char* xr = p.b + row * p.ldb + lh * 16;
+  const char* wr[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t c = m0 + i * 32 + li;
+    wr[i] = p.a + (c < p.m ? c : p.m - 1) * p.lda + lh * 16;
+  }
+  cef16 acc[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+  const int steps = D / STEP;
+  iv4 xa[2][4], wa[2][2][4];
+  auto load = [&](int s, int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t o = (int64_t)(s + q < steps ? s + q : steps - 1) * 32;
+      xa[buf][q] = *reinterpret_cast<const iv4*>(xr + o);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) wa[buf][i][q] = *reinterpret_cast<const iv4*>(wr[i] + o);
+    }
+  };
+  auto mul = [&](int s, int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (s + q >= steps) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (DT == CRESTE_DT_F32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(cef4, wa[buf][i][q])[e], __builtin_bit_cast(cef4, xa[buf][q])[e],
+                                                          acc[i], 0, 0, 0);
+        } else {
+          acc[i] = ce_mfma<DT>(__builtin_bit_cast(ces8, wa[buf][i][q]), __builtin_bit_cast(ces8, xa[buf][q]), acc[i]);
+        }
+      }
+    }
+  };
+  load(0, 0);
+  for (int s = 0; s < steps; s += 8) {
+    load(s + 4, 1);
+    mul(s, 0);
+    load(s + 8, 0);
+    mul(s + 4, 1);
+  }
+  const float c2 = p.inv_tau * kCeLog2e;
+  const int64_t y = li < p.n ? p.labels[li] : -1;
+  const int64_t yr = y - m0;
+  const int lab = y >= 0 && y < p.classes && yr >= 0 && yr < 64 ? (int)yr : -1;
+  float mx = -INFINITY, sum = 0.f, z = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int cl = i * 32 + (r & 3) + 8 * (r >> 2) + 4 * lh;
+      if (m0 + cl >= p.m) acc[i][r] = -INFINITY;
+      z = cl == lab ? acc[i][r] : z;
+      mx = fmaxf(mx, acc[i][r]);
+    }
+  mx = fmaxf(mx * c2, -3.0e38f);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][r], c2, -mx));
+  const float mo = __shfl_xor(mx, 32, 64), so = __shfl_xor(sum, 32, 64);
+  float mm = fmaxf(mx, mo);
+  sum = sum * __builtin_amdgcn_exp2f(mx - mm) + so * __builtin_amdgcn_exp2f(mo - mm);
+  if (lh == 0) sh[wave][li] = make_float2(mm, sum);
+  if (lab >= 0 && ((lab >> 2) & 1) == lh) p.zlab[li] = z * c2;
+  __syncthreads();
+  if (threadIdx.x < 32 && (int)threadIdx.x < p.n) {
+    for (int j = 1; j < 4; ++j) {
+      const float2 v = sh[j][li];
+      const float m = fmaxf(mm, v.x);
+      sum = sum * __builtin_amdgcn_exp2f(mm - m) + v.y * __builtin_amdgcn_exp2f(v.x - m);
+      mm = m;
+    }
+    p.part[(int64_t)blockIdx.x * p.n + li] = make_float2(mm, sum);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------- small kernels
 __global__ void ce_zero_kernel(float* p, int n) {
   if ((int)threadIdx.x < n) p[threadIdx.x] = 0.f;
@@ -389,15 +485,18 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const T* __restrict__ x, i
   }
 }
 
-// per row: join the class tiles' (max, sum).  64 rows x 16 slices of the tiles per block; per block the sums of nll and count
+// per row: join the class tiles' (max, sum).  64 rows x 16 slices of the tiles per block; per block the sums of nll and count, or
+// the loss itself when there is one block
 __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ part, int tiles, int n, const float* __restrict__ zlab,
                                                        const int64_t* __restrict__ labels, int64_t ignore, int classes,
-                                                       float* __restrict__ nll, float* __restrict__ lse2, float2* __restrict__ bsum) {
+                                                       float* __restrict__ nll, float* __restrict__ lse2, float2* __restrict__ bsum,
+                                                       int mean, float* __restrict__ loss, float* __restrict__ stat) {
   __shared__ float2 sh[16][64];
   const int li = threadIdx.x & 63, sl = threadIdx.x >> 6;
   const int row = blockIdx.x * 64 + li;
   float mx = -3.0e38f, sum = 0.f;
   if (row < n)
+#pragma unroll 4
     for (int t = sl; t < tiles; t += 16) {
       const float2 v = part[(int64_t)t * n + row];
       const float m = fmaxf(mx, v.x);
@@ -430,7 +529,14 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
     l += __shfl_xor(l, o, 64);
     c += __shfl_xor(c, o, 64);
   }
-  if (li == 0) bsum[blockIdx.x] = make_float2(l, c);
+  if (li) return;
+  if (gridDim.x > 1) {
+    bsum[blockIdx.x] = make_float2(l, c);
+  } else {
+    stat[0] = l;
+    stat[1] = c;
+    *loss = mean ? l / fmaxf(c, 1.f) : l;
+  }
 }
 
 // loss from the blocks' sums (fixed order), stat = {sum nll, count}
@@ -499,6 +605,14 @@ constexpr int64_t kCePieceBytes = 512ll << 20;     // bound on G
 
 bool ce_direct(const void* x, int64_t ld, int D, int dtype) {
   return dtype != CRESTE_DT_F32 && D % 64 == 0 && ld % 8 == 0 && ((uintptr_t)x & 15) == 0;
+}
+
+constexpr int kCeFewRows = 32;
+
+// rows that the few-rows kernel can read in place: whole 32-byte steps on 16-byte boundaries
+bool ce_few(const void* x, int64_t ld, int D, int dtype) {
+  const int es = dtype == CRESTE_DT_F32 ? 4 : 2;
+  return D * es % 32 == 0 && ld * es % 16 == 0 && ((uintptr_t)x & 15) == 0;
 }
 
 CePlan ce_plan(int64_t N, int64_t V, int D, int dtype, bool packx, bool packw, bool train) {
@@ -643,14 +757,17 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
                                         void* stream) {
   const int bad = ce_check(x, ldx, w, ldw, labels, N, V, D, dtype, temperature);
   if (bad) return bad;
-  const CePlan q = ce_plan(N, V, D, dtype, !ce_direct(x, ldx, D, dtype), !ce_direct(w, ldw, D, dtype), false);
+  const bool few = N <= kCeFewRows && ce_few(x, ldx, D, dtype) && ce_few(w, ldw, D, dtype);
+  const CePlan q = ce_plan(N, V, D, dtype, !few && !ce_direct(x, ldx, D, dtype), !few && !ce_direct(w, ldw, D, dtype), false);
   CRESTE_REQUIRE(loss && nll && lse2 && stat && work && work_bytes >= q.total, "linear_ce_forward: outputs / workspace (%lld of %lld bytes)",
                  (long long)work_bytes, (long long)q.total);
   hipStream_t s = (hipStream_t)stream;
   char* wk = (char*)work;
-  CeOperand X, W;
-  const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, dtype, wk, &X, &W, s);
-  if (rc) return rc;
+  CeOperand X{(const char*)x, ldx * q.es, 0}, W{(const char*)w, ldw * q.es, 0};
+  if (!few) {
+    const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, dtype, wk, &X, &W, s);
+    if (rc) return rc;
+  }
   CeArgs a{};
   a.a = W.p; a.lda = W.ld; a.pa = W.piece; a.ra = V;
   a.b = X.p; a.ldb = X.ld; a.pb = X.piece; a.rb = N;
@@ -662,11 +779,19 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
   a.amax = q.P == 2 ? (const float*)(wk + q.amax) : nullptr;
   a.part = (float2*)(wk + q.part); a.zlab = (float*)(wk + q.zlab);
   CRESTE_REQUIRE((int64_t)a.mt * a.nt < (1ll << 31), "linear_ce: too many tiles");
-  const int rg = ce_dispatch<CE_LOSS>(q, a, a.mt * a.nt, s);
-  if (rg) return rg;
+  if (few) {
+    if (dtype == CRESTE_DT_F32) ce_few_kernel<CRESTE_DT_F32><<<q.tiles, 256, 0, s>>>(a, D);
+    else if (dtype == CRESTE_DT_BF16) ce_few_kernel<CRESTE_DT_BF16><<<q.tiles, 256, 0, s>>>(a, D);
+    else ce_few_kernel<CRESTE_DT_F16><<<q.tiles, 256, 0, s>>>(a, D);
+    CRESTE_CHECK_LAUNCH("linear_ce few rows");
+  } else {
+    const int rg = ce_dispatch<CE_LOSS>(q, a, a.mt * a.nt, s);
+    if (rg) return rg;
+  }
   const int nb = cdiv(N, 64);
-  ce_join_kernel<<<nb, 1024, 0, s>>>(a.part, q.tiles, (int)N, a.zlab, labels, ignore_index, (int)V, nll, lse2, (float2*)(wk + q.bsum));
-  ce_final_kernel<<<1, 256, 0, s>>>((const float2*)(wk + q.bsum), nb, mean, loss, stat);
+  ce_join_kernel<<<nb, 1024, 0, s>>>(a.part, q.tiles, (int)N, a.zlab, labels, ignore_index, (int)V, nll, lse2, (float2*)(wk + q.bsum),
+                                       mean, loss, stat);
+  if (nb > 1) ce_final_kernel<<<1, 256, 0, s>>>((const float2*)(wk + q.bsum), nb, mean, loss, stat);
   CRESTE_CHECK_LAUNCH("linear_ce join");
   return CRESTE_OK;
 }

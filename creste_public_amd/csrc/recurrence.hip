@@ -3,11 +3,14 @@
 // and its reverse:  e_t = f_t (dh_t + e_(t+1))  with e_T = dh_last;  delta_t = dh_t + e_(t+1);  dx_t = u_t delta_t;
 //   dgate_t = delta_t (h_(t-1) - x_t) f_t u_t;  dh0 = e_0.
 // Both are first-order linear maps of the carried value, so a run of steps is one pair (A, B): out = A in + B.
-// Layout.  Lanes = channels (VEC neighbours each, (b, c) flattened), waves of a workgroup = consecutive runs of LR steps held in
-// registers, joined through LDS: a workgroup takes a chunk of 8 * LR steps with one pass over its data, and walks its segment of the
-// time axis chunk by chunk, carrying the state.  With enough (b, c) columns one segment covers all of T and everything is read once.
-// With few, the time axis is split into segments: a first launch leaves each segment's (A, B) (forward: gate and x read twice;
-// backward: gate and dh), the second joins the segments in front of its own.
+// Layout.  Lanes = channels (VEC neighbours each, (b, c) flattened), the 8 waves of a workgroup = consecutive runs of LR steps held in
+// registers and joined through LDS: a workgroup takes one chunk of 8 * LR steps of 64 * VEC columns with ONE pass over its data.
+// Chunks of one column group meet by look-back: a workgroup publishes its chunk's (A, B), fetches those of the chunks in front of
+// it in its window of 16 and the value carried into the window (published by the window in front), the 8 waves two each at once.
+// Always the same pairs in the same order, whoever is ready first: results do not depend on timing.
+// Work is handed out by a ticket, so a chunk only ever waits for chunks that started earlier: every wait ends.  Each published word
+// is 8 bytes written at once, valid when not zero -- (-A, B): A >= 0, so the sign bit marks it -- hence no fences.  (The spin is
+// bounded all the same: past the bound the columns become NaN.)
 // The backward recomputes h inside a chunk from the chunk's starting state, which the forward saves (4 bytes per 8 * LR steps).
 // Steps behind a sequence's length have f = 1, u = 0, dh = 0: states and cotangents pass through unchanged.
 // Bound: HBM (forward 3 elements, backward 5 per step and channel), a single step: launch latency.
@@ -23,15 +26,27 @@ struct RecArgs {
   const float *h0, *gh_last;
   const int64_t* lengths;
   int64_t T, C, BC;
-  int chunks, seg_chunks, segs;
+  int chunks, groups;
   void *h, *ggate, *gx;
   float *h_last, *starts, *gh0;
-  float2* agg;                                  // [segs][BC] (A, B) of a segment
+  unsigned* ticket;                             // zeroed, as the words below
+  uint64_t *pair, *known;                       // [chunks][BC] (-A, B) of a chunk; (carried value behind it, 1)
 };
 
-// f = sigmoid(g), u = 1 - f, both to full relative accuracy
+constexpr int kRecSpin = 1 << 22, kRecWindow = 16;
+
+__device__ __forceinline__ uint64_t rec_word(unsigned lo, float hi) { return (uint64_t)__float_as_uint(hi) << 32 | lo; }
+__device__ __forceinline__ uint64_t rec_get(const uint64_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void rec_put(uint64_t* p, uint64_t v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// f = sigmoid(g), u = 1 - f, both to a few 2^-24 relative (hardware exponential and reciprocal: a full division would cost as much
+// as the rest of a step)
 __device__ __forceinline__ void rec_gate(float g, float& f, float& u) {
-  const float e = __expf(-fabsf(g)), r = 1.f / (1.f + e), s = e * r;
+  const float e = __builtin_amdgcn_exp2f(-1.44269504088896341f * fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
   f = g >= 0.f ? r : s;
   u = g >= 0.f ? s : r;
 }
@@ -44,8 +59,8 @@ template <int VEC>
 struct RecCol {
   int64_t col, b, c, len;
   bool on;
-  __device__ __forceinline__ RecCol(const RecArgs& p) {
-    col = ((int64_t)blockIdx.x * 64 + threadIdx.x) * VEC;
+  __device__ __forceinline__ RecCol(const RecArgs& p, int group) {
+    col = ((int64_t)group * 64 + threadIdx.x) * VEC;
     on = col < p.BC;
     if (!on) col = p.BC - VEC;                  // a copy of the last column; it stores nothing
     b = col / p.C;
@@ -58,264 +73,351 @@ struct RecCol {
   }
 };
 
-// AGG: leave the segment's (A, B) only
-template <typename T, int VEC, int LR, bool AGG>
-__global__ __launch_bounds__(512) void rec_forward_kernel(RecArgs p) {
-  typedef typename RecVec<T, VEC>::type vec;
-  __shared__ float2 sh[kRecWaves][64 * VEC];
-  const RecCol<VEC> k(p);
-  const int w = threadIdx.y, nw = blockDim.y, seg = blockIdx.y;
-  const T* gp = (const T*)p.gate + k.b * p.g_sb + k.c;
-  const T* xp = (const T*)p.x + k.b * p.x_sb + k.c;
-  float s[VEC], sa[VEC];                        // carried state; AGG: carried (A, B)
+// steps of the run t0 .. t0 + LR - 1 in front of `len`
+template <int LR>
+__device__ __forceinline__ int rec_live(int64_t t0, int64_t len) {
+  const int64_t n = len - t0;
+  return n < 0 ? 0 : n > LR ? LR : (int)n;
+}
+
+// which (column group, chunk in the order of the recurrence) this workgroup takes
+__device__ __forceinline__ void rec_ticket(const RecArgs& p, int& group, int& turn) {
+  if (p.chunks == 1) {
+    group = blockIdx.x;
+    turn = 0;
+    return;
+  }
+  __shared__ unsigned t;
+  if (threadIdx.x == 0 && threadIdx.y == 0) t = atomicAdd(p.ticket, 1u);
+  __syncthreads();
+  group = __builtin_amdgcn_readfirstlane((int)(t % (unsigned)p.groups));
+  turn = __builtin_amdgcn_readfirstlane((int)(t / (unsigned)p.groups));
+}
+
+// s (on entry the value in front of the first chunk) <- the value carried into this chunk.  (A, B): this chunk's pair.  turn = the
+// chunk's place in the order of the recurrence, step = +1 / -1 that order in chunks.  All threads of the workgroup call and get the result
+template <int VEC>
+__device__ __forceinline__ void rec_lookback(const RecArgs& p, const RecCol<VEC>& k, int ch, int turn, int step, const float (&A)[VEC],
+                                             const float (&B)[VEC], float (&s)[VEC]) {
+  __shared__ float2 sh[kRecWindow][64 * VEC];
+  __shared__ float carried[64 * VEC];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.y), at_w = turn % kRecWindow, base = turn - at_w;
+  const bool last = at_w == kRecWindow - 1;
+  if (w == 0 && k.on && !last)                  // (nobody asks for the pair of a window's last chunk)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      rec_put(p.pair + (int64_t)ch * p.BC + k.col + e, rec_word(__float_as_uint(A[e]) | 0x80000000u, B[e]));
+  // wave w fetches the pairs number w and w + 8 of the window, the last wave the value carried into the window
+  const uint64_t* src[3] = {nullptr, nullptr, nullptr};
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+    if (w + kRecWaves * q < at_w) src[q] = p.pair + (int64_t)(ch - step * (at_w - w - kRecWaves * q)) * p.BC + k.col;
+  if (w == kRecWaves - 1 && base > 0) src[2] = p.known + (int64_t)(ch - step * (at_w + 1)) * p.BC + k.col;
+  uint64_t v[3][VEC];
+  for (int spin = 0;; ++spin) {
+    bool all = true;
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[q][e] = src[q] ? rec_get(src[q] + e) : 1;
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) all &= v[q][e] != 0;
+    if (__all(all)) break;
+    if (spin == kRecSpin) {
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[q][e] = rec_word(0x7fc00000u, __builtin_nanf(""));
+      break;
+    }
+    __builtin_amdgcn_s_sleep(1);
+  }
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
-    s[e] = !AGG && p.h0 ? p.h0[k.col + e] : 0.f;
-    sa[e] = 1.f;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (src[q])
+        sh[w + kRecWaves * q][threadIdx.x * VEC + e] =
+            make_float2(__uint_as_float((unsigned)v[q][e] & 0x7fffffffu), __uint_as_float((unsigned)(v[q][e] >> 32)));
+    if (src[2]) carried[threadIdx.x * VEC + e] = __uint_as_float((unsigned)(v[2][e] >> 32));
   }
-  if constexpr (!AGG)
-    for (int j = 0; j < seg; ++j)
+  __syncthreads();
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float2 v = p.agg[(int64_t)j * p.BC + k.col + e];
-        s[e] = fmaf(v.x, s[e], v.y);
-      }
-  const int c0 = seg * p.seg_chunks, c1 = min(p.chunks, c0 + p.seg_chunks);
-  for (int ch = c0; ch < c1; ++ch) {
-    const int64_t t0 = ((int64_t)ch * nw + w) * LR;
-    vec gv[LR], xv[LR];
-#pragma unroll
-    for (int i = 0; i < LR; ++i) {
-      const int64_t t = t0 + i < p.T ? t0 + i : p.T - 1;
-      gv[i] = *reinterpret_cast<const vec*>(gp + t * p.g_st);
-      xv[i] = *reinterpret_cast<const vec*>(xp + t * p.x_st);
+  for (int e = 0; e < VEC; ++e) {
+    if (base > 0) s[e] = carried[threadIdx.x * VEC + e];
+    for (int j = 0; j < at_w; ++j) {
+      const float2 q = sh[j][threadIdx.x * VEC + e];
+      s[e] = fmaf(q.x, s[e], q.y);
     }
-    float f[LR][VEC], b[LR][VEC], A[VEC], B[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) { A[e] = 1.f; B[e] = 0.f; }
-#pragma unroll
-    for (int i = 0; i < LR; ++i) {
-      const bool live = t0 + i < k.len;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float u;
-        rec_gate((float)gv[i][e], f[i][e], u);
-        f[i][e] = live ? f[i][e] : 1.f;
-        b[i][e] = live ? u * (float)xv[i][e] : 0.f;
-        A[e] *= f[i][e];
-        B[e] = fmaf(f[i][e], B[e], b[i][e]);
-      }
-    }
-    if (nw > 1) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) sh[w][threadIdx.x * VEC + e] = make_float2(A[e], B[e]);
-      __syncthreads();
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if constexpr (!AGG)
-        if (w == 0 && p.starts && k.on) p.starts[(int64_t)ch * p.BC + k.col + e] = s[e];
-      float mine = s[e];                        // state in front of this wave's run
-      for (int j = 0; j < nw; ++j) {
-        const float2 v = nw > 1 ? sh[j][threadIdx.x * VEC + e] : make_float2(A[e], B[e]);
-        if (j == w) mine = s[e];
-        s[e] = fmaf(v.x, s[e], v.y);
-        if constexpr (AGG) sa[e] *= v.x;
-      }
-      if constexpr (!AGG) {
-#pragma unroll
-        for (int i = 0; i < LR; ++i) {
-          mine = fmaf(f[i][e], mine, b[i][e]);
-          b[i][e] = mine;
-        }
-      }
-    }
-    if constexpr (!AGG) {
-      T* hp = (T*)p.h + (k.b * p.T) * p.C + k.c;
-#pragma unroll
-      for (int i = 0; i < LR; ++i) {
-        vec o;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] = (T)(t0 + i < k.len ? b[i][e] : 0.f);
-        if (k.on && t0 + i < p.T) *reinterpret_cast<vec*>(hp + (t0 + i) * p.C) = o;
-      }
-    }
-    if (nw > 1) __syncthreads();
-  }
-  if (w == 0 && k.on) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if constexpr (AGG) p.agg[(int64_t)seg * p.BC + k.col + e] = make_float2(sa[e], s[e]);
-      else if (seg == p.segs - 1) p.h_last[k.col + e] = s[e];
-    }
+    if (last && w == 0 && k.on) rec_put(p.known + (int64_t)ch * p.BC + k.col + e, rec_word(1u, fmaf(A[e], s[e], B[e])));
   }
 }
 
-template <typename T, int VEC, int LR, bool AGG>
-__global__ __launch_bounds__(512) void rec_backward_kernel(RecArgs p) {
+template <typename T, int VEC, int LR>
+__global__ __launch_bounds__(512, 4) void rec_forward_kernel(RecArgs p) {
   typedef typename RecVec<T, VEC>::type vec;
-  __shared__ float2 sh[kRecWaves][64 * VEC], fw[AGG ? 1 : kRecWaves][64 * VEC];
-  const RecCol<VEC> k(p);
-  const int w = threadIdx.y, nw = blockDim.y, seg = blockIdx.y;
-  const T* gp = (const T*)p.gate + k.b * p.g_sb + k.c;
-  const T* xp = (const T*)p.x + k.b * p.x_sb + k.c;
-  const T* dp = (const T*)p.gh + k.b * p.h_sb + k.c;
-  float s[VEC], sa[VEC];                        // e carried from the later steps
+  __shared__ float2 sh[kRecWaves][64 * VEC];
+  int group, ch;
+  rec_ticket(p, group, ch);
+  const RecCol<VEC> k(p, group);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.y), nw = blockDim.y;
+  const int64_t t0 = ((int64_t)ch * nw + w) * LR;
+  const T *gp = (const T*)p.gate + k.b * p.g_sb + k.c, *xp = (const T*)p.x + k.b * p.x_sb + k.c;
+  vec gv[LR], xv[LR];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    s[e] = !AGG && p.gh_last ? p.gh_last[k.col + e] : 0.f;
-    sa[e] = 1.f;
+  for (int i = 0; i < LR; ++i) {
+    const int64_t t = t0 + i < p.T ? t0 + i : p.T - 1;
+    gv[i] = *reinterpret_cast<const vec*>(gp + t * p.g_st);
+    xv[i] = *reinterpret_cast<const vec*>(xp + t * p.x_st);
   }
-  if constexpr (!AGG)
-    for (int j = p.segs - 1; j > seg; --j)
+  float s[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float2 v = p.agg[(int64_t)j * p.BC + k.col + e];
-        s[e] = fmaf(v.x, s[e], v.y);
-      }
-  const int c0 = seg * p.seg_chunks, c1 = min(p.chunks, c0 + p.seg_chunks);
-  for (int ch = c1 - 1; ch >= c0; --ch) {
-    const int64_t t0 = ((int64_t)ch * nw + w) * LR;
-    vec gv[LR], xv[LR], dv[LR];
-    float st[VEC];
+  for (int e = 0; e < VEC; ++e) s[e] = p.h0 ? p.h0[k.col + e] : 0.f;
+  const int live = rec_live<LR>(t0, k.len);     // steps of this run in front of the sequence's end
+  const bool whole = __all(live == LR);
+  float f[LR][VEC], b[LR][VEC], A[VEC], B[VEC];
 #pragma unroll
-    for (int i = 0; i < LR; ++i) {
-      const int64_t t = t0 + i < p.T ? t0 + i : p.T - 1;
-      gv[i] = *reinterpret_cast<const vec*>(gp + t * p.g_st);
-      if constexpr (!AGG) xv[i] = *reinterpret_cast<const vec*>(xp + t * p.x_st);
-      dv[i] = *reinterpret_cast<const vec*>(dp + t * p.h_st);
+  for (int i = 0; i < LR; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float u;
+      rec_gate((float)gv[i][e], f[i][e], u);
+      b[i][e] = u * (float)xv[i][e];
     }
-    if constexpr (!AGG)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) st[e] = p.starts[(int64_t)ch * p.BC + k.col + e];
-    float f[LR][VEC], u[LR][VEC];
+  if (!whole)
 #pragma unroll
     for (int i = 0; i < LR; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        rec_gate((float)gv[i][e], f[i][e], u[i][e]);
-        if (t0 + i >= k.len) { f[i][e] = 1.f; u[i][e] = 0.f; }
+        f[i][e] = i < live ? f[i][e] : 1.f;
+        b[i][e] = i < live ? b[i][e] : 0.f;
       }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      float A = 1.f, B = 0.f;
+  for (int e = 0; e < VEC; ++e) {
+    A[e] = 1.f;
+    B[e] = 0.f;
 #pragma unroll
-      for (int i = LR - 1; i >= 0; --i) {
-        const float d = t0 + i < k.len ? (float)dv[i][e] : 0.f;
-        B = f[i][e] * (d + B);
-        A *= f[i][e];
-      }
-      sh[w][threadIdx.x * VEC + e] = make_float2(A, B);
-      if constexpr (!AGG) {
-        float H = 0.f;                          // the forward pair of the run: (A, H)
-#pragma unroll
-        for (int i = 0; i < LR; ++i) H = fmaf(f[i][e], H, u[i][e] != 0.f ? u[i][e] * (float)xv[i][e] : 0.f);
-        fw[w][threadIdx.x * VEC + e] = make_float2(A, H);
-      }
+    for (int i = 0; i < LR; ++i) {
+      A[e] *= f[i][e];
+      B[e] = fmaf(f[i][e], B[e], b[i][e]);
     }
-    if (nw > 1) __syncthreads();
-    float mine[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      for (int j = nw - 1; j >= 0; --j) {
-        const float2 v = sh[j][threadIdx.x * VEC + e];
-        if (j == w) mine[e] = s[e];
-        s[e] = fmaf(v.x, s[e], v.y);
-        if constexpr (AGG) sa[e] *= v.x;
-      }
-      if constexpr (!AGG)
-        for (int j = 0; j < w; ++j) {
-          const float2 v = fw[j][threadIdx.x * VEC + e];
-          st[e] = fmaf(v.x, st[e], v.y);
-        }
-    }
-    if constexpr (!AGG) {
-      float hp[LR][VEC];                        // h_(t-1)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e)
-#pragma unroll
-        for (int i = 0; i < LR; ++i) {
-          hp[i][e] = st[e];
-          st[e] = fmaf(f[i][e], st[e], u[i][e] != 0.f ? u[i][e] * (float)xv[i][e] : 0.f);
-        }
-      T* ggp = (T*)p.ggate + (k.b * p.T) * p.C + k.c;
-      T* gxp = (T*)p.gx + (k.b * p.T) * p.C + k.c;
-#pragma unroll
-      for (int i = LR - 1; i >= 0; --i) {
-        vec og, ox;
-        const bool live = t0 + i < k.len;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float d = (live ? (float)dv[i][e] : 0.f) + mine[e];
-          og[e] = (T)(live ? d * (hp[i][e] - (float)xv[i][e]) * (f[i][e] * u[i][e]) : 0.f);
-          ox[e] = (T)(live ? d * u[i][e] : 0.f);
-          mine[e] = f[i][e] * d;
-        }
-        if (k.on && t0 + i < p.T) {
-          *reinterpret_cast<vec*>(ggp + (t0 + i) * p.C) = og;
-          *reinterpret_cast<vec*>(gxp + (t0 + i) * p.C) = ox;
-        }
-      }
-    }
-    if (nw > 1) __syncthreads();
   }
+  float wa[VEC], wb[VEC];                       // pair of the runs in front of this wave's
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) { wa[e] = 1.f; wb[e] = 0.f; }
+  if (nw > 1) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sh[w][threadIdx.x * VEC + e] = make_float2(A[e], B[e]);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float ca = 1.f, cb = 0.f;
+      for (int j = 0; j < nw; ++j) {
+        const float2 v = sh[j][threadIdx.x * VEC + e];
+        if (j == w) { wa[e] = ca; wb[e] = cb; }
+        cb = fmaf(v.x, cb, v.y);
+        ca *= v.x;
+      }
+      A[e] = ca;
+      B[e] = cb;
+    }
+  }
+  if constexpr (LR > 1)
+    if (p.chunks > 1) rec_lookback<VEC>(p, k, ch, ch, 1, A, B, s);
   if (w == 0 && k.on) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      if constexpr (AGG) p.agg[(int64_t)seg * p.BC + k.col + e] = make_float2(sa[e], s[e]);
-      else if (seg == 0 && p.gh0) p.gh0[k.col + e] = s[e];
+      if (p.starts) p.starts[(int64_t)ch * p.BC + k.col + e] = s[e];
+      if (ch == p.chunks - 1) p.h_last[k.col + e] = fmaf(A[e], s[e], B[e]);
     }
   }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) s[e] = fmaf(wa[e], s[e], wb[e]);
+  T* hp = (T*)p.h + (k.b * p.T) * p.C + k.c;
+#pragma unroll
+  for (int i = 0; i < LR; ++i) {
+    vec o;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      s[e] = fmaf(f[i][e], s[e], b[i][e]);
+      o[e] = (T)(i < live ? s[e] : 0.f);
+    }
+    if (k.on && t0 + i < p.T) *reinterpret_cast<vec*>(hp + (t0 + i) * p.C) = o;
+  }
+}
+
+template <typename T, int VEC, int LR>
+__global__ __launch_bounds__(512, 4) void rec_backward_kernel(RecArgs p) {
+  typedef typename RecVec<T, VEC>::type vec;
+  __shared__ float2 sh[kRecWaves][64 * VEC], fw[kRecWaves][64 * VEC];
+  int group, turn;
+  rec_ticket(p, group, turn);
+  const int ch = p.chunks - 1 - turn;
+  const RecCol<VEC> k(p, group);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.y), nw = blockDim.y;
+  const int64_t t0 = ((int64_t)ch * nw + w) * LR;
+  const T *gp = (const T*)p.gate + k.b * p.g_sb + k.c, *xp = (const T*)p.x + k.b * p.x_sb + k.c;
+  const T* dp = (const T*)p.gh + k.b * p.h_sb + k.c;
+  vec gv[LR], xv[LR], dv[LR];
+#pragma unroll
+  for (int i = 0; i < LR; ++i) {
+    const int64_t t = t0 + i < p.T ? t0 + i : p.T - 1;
+    gv[i] = *reinterpret_cast<const vec*>(gp + t * p.g_st);
+    dv[i] = *reinterpret_cast<const vec*>(dp + t * p.h_st);
+    xv[i] = *reinterpret_cast<const vec*>(xp + t * p.x_st);
+  }
+  float st[VEC], s[VEC];                        // h in front of the chunk; e behind it
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    st[e] = p.starts[(int64_t)ch * p.BC + k.col + e];
+    s[e] = p.gh_last ? p.gh_last[k.col + e] : 0.f;
+  }
+  const int live = rec_live<LR>(t0, k.len);
+  const bool whole = __all(live == LR);
+  float f[LR][VEC], u[LR][VEC], x[LR][VEC], d[LR][VEC], A[VEC], B[VEC], wa[VEC], wb[VEC];
+#pragma unroll
+  for (int i = 0; i < LR; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      rec_gate((float)gv[i][e], f[i][e], u[i][e]);
+      x[i][e] = (float)xv[i][e];
+      d[i][e] = (float)dv[i][e];
+    }
+  if (!whole)
+#pragma unroll
+    for (int i = 0; i < LR; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        f[i][e] = i < live ? f[i][e] : 1.f;
+        u[i][e] = i < live ? u[i][e] : 0.f;
+        x[i][e] = i < live ? x[i][e] : 0.f;
+        d[i][e] = i < live ? d[i][e] : 0.f;
+      }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    float a = 1.f, b = 0.f, h = 0.f;            // (a, b): e through the run, (a, h): the state
+#pragma unroll
+    for (int i = LR - 1; i >= 0; --i) {
+      b = f[i][e] * (d[i][e] + b);
+      a *= f[i][e];
+    }
+#pragma unroll
+    for (int i = 0; i < LR; ++i) h = fmaf(f[i][e], h, u[i][e] * x[i][e]);
+    A[e] = a; B[e] = b;
+    wa[e] = 1.f; wb[e] = 0.f;
+    if (nw > 1) {
+      sh[w][threadIdx.x * VEC + e] = make_float2(a, b);
+      fw[w][threadIdx.x * VEC + e] = make_float2(a, h);
+    }
+  }
+  if (nw > 1) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float ca = 1.f, cb = 0.f;
+      for (int j = nw - 1; j >= 0; --j) {
+        const float2 v = sh[j][threadIdx.x * VEC + e];
+        if (j == w) { wa[e] = ca; wb[e] = cb; }
+        cb = fmaf(v.x, cb, v.y);
+        ca *= v.x;
+      }
+      A[e] = ca;
+      B[e] = cb;
+      for (int j = 0; j < w; ++j) {
+        const float2 v = fw[j][threadIdx.x * VEC + e];
+        st[e] = fmaf(v.x, st[e], v.y);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {               // x <- (h_(t-1) - x_t) f_t u_t, all that dgate needs besides delta
+#pragma unroll
+    for (int i = 0; i < LR; ++i) {
+      const float h = st[e];
+      st[e] = fmaf(f[i][e], h, u[i][e] * x[i][e]);
+      x[i][e] = (h - x[i][e]) * (f[i][e] * u[i][e]);
+    }
+  }
+  if constexpr (LR > 1)
+    if (p.chunks > 1) rec_lookback<VEC>(p, k, ch, turn, -1, A, B, s);
+  if (w == 0 && k.on && ch == 0 && p.gh0)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) p.gh0[k.col + e] = fmaf(A[e], s[e], B[e]);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) s[e] = fmaf(wa[e], s[e], wb[e]);
+  T* ggp = (T*)p.ggate + (k.b * p.T) * p.C + k.c;
+  T* gxp = (T*)p.gx + (k.b * p.T) * p.C + k.c;
+#pragma unroll
+  for (int i = LR - 1; i >= 0; --i) {
+    vec og, ox;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {             // (behind the end: u = 0 and d = 0, so both are 0 and e passes)
+      const float delta = d[i][e] + s[e];
+      og[e] = (T)(i < live ? delta * x[i][e] : 0.f);
+      ox[e] = (T)(i < live ? delta * u[i][e] : 0.f);
+      s[e] = f[i][e] * delta;
+    }
+    if (k.on && t0 + i < p.T) {
+      *reinterpret_cast<vec*>(ggp + (t0 + i) * p.C) = og;
+      *reinterpret_cast<vec*>(gxp + (t0 + i) * p.C) = ox;
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void rec_zero_kernel(uint4* __restrict__ p, int64_t n) {
+  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) p[i] = make_uint4(0, 0, 0, 0);
 }
 
 namespace {
 
-// segments: one while the columns alone give >= 512 workgroups, else enough for ~1024, at most one per chunk and at most 64 (every
-// workgroup reads the pairs of the segments in front of it)
-int rec_segments(int64_t BC, int64_t chunks) {
-  const int64_t groups = (BC + 63) / 64;
-  if (groups >= 512 || chunks < 2) return 1;
-  int64_t s = 1024 / groups;
-  s = s > chunks ? chunks : s;
-  return (int)(s > 64 ? 64 : s < 1 ? 1 : s);
+int64_t rec_chunks(int64_t T) { return (T + kRecChunk - 1) / kRecChunk; }
+
+// the ticket (16 bytes) and the two arrays of published words, a multiple of 16 bytes in all
+int64_t rec_work(int64_t BC, int64_t T) {
+  const int64_t n = rec_chunks(T);
+  return n == 1 ? 16 : 16 + 16 * ((n * BC + 1) / 2 * 2);
 }
 
 template <typename T, int VEC, int LR>
-int rec_launch(RecArgs& p, bool bwd, hipStream_t s) {
+int rec_launch(RecArgs& p, bool bwd, char* work, hipStream_t s) {
   const int64_t groups = (p.BC / VEC + 63) / 64;
-  CRESTE_REQUIRE(groups < (1ll << 31), "gated_recurrence: too many columns");
   int64_t nw = (p.T + LR - 1) / LR;
   nw = nw > kRecWaves ? kRecWaves : nw;
-  p.chunks = (int)((p.T + nw * LR - 1) / (nw * LR));
-  int segs = LR == 1 ? 1 : rec_segments(p.BC, p.chunks);
-  p.seg_chunks = (p.chunks + segs - 1) / segs;
-  p.segs = (p.chunks + p.seg_chunks - 1) / p.seg_chunks;
-  const dim3 grid((unsigned)groups, p.segs), block(64, (unsigned)nw);
-  if (p.segs > 1) {
-    if (bwd) rec_backward_kernel<T, VEC, LR, true><<<grid, block, 0, s>>>(p);
-    else rec_forward_kernel<T, VEC, LR, true><<<grid, block, 0, s>>>(p);
-    CRESTE_CHECK_LAUNCH("gated_recurrence segments");
+  const int64_t chunks = (p.T + nw * LR - 1) / (nw * LR);
+  CRESTE_REQUIRE(groups * chunks < (1ll << 31), "gated_recurrence: too many columns and chunks of steps");
+  p.chunks = (int)chunks;
+  p.groups = (int)groups;
+  if (chunks > 1) {
+    const int64_t n = rec_work(p.BC, p.T) / 16, nb = (n + 255) / 256;
+    p.ticket = (unsigned*)work;
+    p.pair = (uint64_t*)(work + 16);
+    p.known = p.pair + chunks * p.BC;
+    rec_zero_kernel<<<(int)(nb > 2048 ? 2048 : nb), 256, 0, s>>>((uint4*)work, n);
+    CRESTE_CHECK_LAUNCH("gated_recurrence zero");
   }
-  if (bwd) rec_backward_kernel<T, VEC, LR, false><<<grid, block, 0, s>>>(p);
-  else rec_forward_kernel<T, VEC, LR, false><<<grid, block, 0, s>>>(p);
+  const dim3 grid((unsigned)(groups * chunks)), block(64, (unsigned)nw);
+  if (bwd) rec_backward_kernel<T, VEC, LR><<<grid, block, 0, s>>>(p);
+  else rec_forward_kernel<T, VEC, LR><<<grid, block, 0, s>>>(p);
   CRESTE_CHECK_LAUNCH("gated_recurrence");
   return CRESTE_OK;
 }
 
 template <typename T>
-int rec_typed(RecArgs& p, bool bwd, hipStream_t s) {
+int rec_typed(RecArgs& p, bool bwd, char* work, hipStream_t s) {
   // two channels per lane where every row starts on a boundary of two elements
   const uintptr_t ptrs = (uintptr_t)p.gate | (uintptr_t)p.x | (uintptr_t)p.gh | (uintptr_t)p.h | (uintptr_t)p.ggate | (uintptr_t)p.gx;
   const int64_t strides = p.C | p.g_sb | p.g_st | p.x_sb | p.x_st | p.h_sb | p.h_st;
   const bool two = (ptrs & (2 * sizeof(T) - 1)) == 0 && (strides & 1) == 0;
-  if (p.T == 1) return two ? rec_launch<T, 2, 1>(p, bwd, s) : rec_launch<T, 1, 1>(p, bwd, s);
-  return two ? rec_launch<T, 2, kRecRun>(p, bwd, s) : rec_launch<T, 1, kRecRun>(p, bwd, s);
+  if (p.T == 1) return two ? rec_launch<T, 2, 1>(p, bwd, work, s) : rec_launch<T, 1, 1>(p, bwd, work, s);
+  return two ? rec_launch<T, 2, kRecRun>(p, bwd, work, s) : rec_launch<T, 1, kRecRun>(p, bwd, work, s);
 }
 
-int rec_run(RecArgs& p, int dtype, bool bwd, hipStream_t s) {
-  if (dtype == CRESTE_DT_F32) return rec_typed<float>(p, bwd, s);
-  if (dtype == CRESTE_DT_BF16) return rec_typed<__bf16>(p, bwd, s);
-  if (dtype == CRESTE_DT_F16) return rec_typed<_Float16>(p, bwd, s);
+int rec_run(RecArgs& p, int dtype, bool bwd, char* work, hipStream_t s) {
+  if (dtype == CRESTE_DT_F32) return rec_typed<float>(p, bwd, work, s);
+  if (dtype == CRESTE_DT_BF16) return rec_typed<__bf16>(p, bwd, work, s);
+  if (dtype == CRESTE_DT_F16) return rec_typed<_Float16>(p, bwd, work, s);
   set_error("gated_recurrence: dtype %d", dtype);
   return CRESTE_ERR_ARG;
 }
@@ -335,7 +437,7 @@ extern "C" int creste_gated_recurrence_chunk_steps(void) { return kRecChunk; }
 
 extern "C" int64_t creste_gated_recurrence_workspace_bytes(int64_t B, int64_t T, int64_t C) {
   if (B <= 0 || T <= 0 || C <= 0 || B >= (1ll << 31) || C >= (1ll << 31) || B * C >= (1ll << 40) || T >= (1ll << 36)) return -1;
-  return rec_segments(B * C, (T + kRecChunk - 1) / kRecChunk) * B * C * (int64_t)sizeof(float2) + 16;
+  return rec_work(B * C, T);
 }
 
 extern "C" int creste_gated_recurrence_forward(const void* gate, int64_t gate_sb, int64_t gate_st, const void* x, int64_t x_sb,
@@ -344,15 +446,15 @@ extern "C" int creste_gated_recurrence_forward(const void* gate, int64_t gate_sb
                                                int64_t work_bytes, void* stream) {
   const int rc = rec_check(B, T, C);
   if (rc) return rc;
-  CRESTE_REQUIRE(gate && x && h && h_last && work && work_bytes >= creste_gated_recurrence_workspace_bytes(B, T, C),
+  CRESTE_REQUIRE(gate && x && h && h_last && work && ((uintptr_t)work & 15) == 0 && work_bytes >= creste_gated_recurrence_workspace_bytes(B, T, C),
                  "gated_recurrence_forward: null pointer or workspace of %lld bytes", (long long)work_bytes);
   RecArgs p{};
   p.gate = gate; p.g_sb = gate_sb; p.g_st = gate_st;
   p.x = x; p.x_sb = x_sb; p.x_st = x_st;
   p.h0 = h0; p.lengths = lengths;
   p.T = T; p.C = C; p.BC = B * C;
-  p.h = h; p.h_last = h_last; p.starts = starts; p.agg = (float2*)work;
-  return rec_run(p, dtype, false, (hipStream_t)stream);
+  p.h = h; p.h_last = h_last; p.starts = starts;
+  return rec_run(p, dtype, false, (char*)work, (hipStream_t)stream);
 }
 
 extern "C" int creste_gated_recurrence_backward(const void* gate, int64_t gate_sb, int64_t gate_st, const void* x, int64_t x_sb,
@@ -362,7 +464,7 @@ extern "C" int creste_gated_recurrence_backward(const void* gate, int64_t gate_s
                                                 int64_t work_bytes, void* stream) {
   const int rc = rec_check(B, T, C);
   if (rc) return rc;
-  CRESTE_REQUIRE(gate && x && gh && starts && ggate && gx && work &&
+  CRESTE_REQUIRE(gate && x && gh && starts && ggate && gx && work && ((uintptr_t)work & 15) == 0 &&
                      work_bytes >= creste_gated_recurrence_workspace_bytes(B, T, C),
                  "gated_recurrence_backward: null pointer or workspace of %lld bytes", (long long)work_bytes);
   RecArgs p{};
@@ -371,6 +473,6 @@ extern "C" int creste_gated_recurrence_backward(const void* gate, int64_t gate_s
   p.gh = gh; p.h_sb = gh_sb; p.h_st = gh_st;
   p.gh_last = gh_last; p.lengths = lengths; p.starts = const_cast<float*>(starts);
   p.T = T; p.C = C; p.BC = B * C;
-  p.ggate = ggate; p.gx = gx; p.gh0 = gh0; p.agg = (float2*)work;
-  return rec_run(p, dtype, true, (hipStream_t)stream);
+  p.ggate = ggate; p.gx = gx; p.gh0 = gh0;
+  return rec_run(p, dtype, true, (char*)work, (hipStream_t)stream);
 }

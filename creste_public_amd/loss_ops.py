@@ -5,11 +5,9 @@ from __future__ import annotations
 
 import torch
 
-from torch.autograd.function import once_differentiable
-
 from . import _lib, ops
 from .ops import HipLibraryError, _stream
-from .train_ops import as_act
+from .train_ops import as_act, once
 
 
 def _work(dev):
@@ -179,7 +177,7 @@ class LinearCEFn(torch.autograd.Function):
         return loss, nll
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, gl, _):
         x, weight, labels, lse2, stat = ctx.saved_tensors
         gx, gw = ops.linear_ce_bwd(x, weight, labels, lse2, stat, gl, *ctx.args, need_x=ctx.needs_input_grad[0],
@@ -196,9 +194,10 @@ def linear_cross_entropy(x, weight, labels, ignore_index: int = -100, temperatur
     ignore_index makes the loss and its gradients NaN.  fp32 features are multiplied with 22 significand bits."""
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise HipLibraryError("linear_cross_entropy: x [...,D] expected")
-    lead = tuple(x.shape[:-1])
-    if not isinstance(labels, torch.Tensor) or tuple(labels.shape) != lead:
-        raise HipLibraryError(f"linear_cross_entropy: labels must have the shape {lead} of the features' rows")
-    loss, nll = LinearCEFn.apply(x.reshape(-1, x.shape[-1]) if x.numel() else x.reshape(0, x.shape[-1]), weight, labels.reshape(-1),
-                                 ignore_index, temperature, reduction)
+    lead = x.shape[:-1]
+    if not isinstance(labels, torch.Tensor) or labels.shape != lead:
+        raise HipLibraryError(f"linear_cross_entropy: labels must have the shape {tuple(lead)} of the features' rows")
+    if x.dim() == 2:
+        return LinearCEFn.apply(x, weight, labels, ignore_index, temperature, reduction)
+    loss, nll = LinearCEFn.apply(x.reshape(labels.numel(), x.shape[-1]), weight, labels.reshape(-1), ignore_index, temperature, reduction)
     return loss, nll.reshape(lead)

@@ -1481,7 +1481,7 @@ def _features(t, name: str, ndim=None, like=None) -> int:
 
 def _plain(t, dtype, shape, device, name: str) -> torch.Tensor:
     """a contiguous tensor of this type, shape and device -- or an error (values are copied if only the strides differ)"""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device:
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape or t.device != device:
         got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
         raise HipLibraryError(f"{name}: expected {dtype} {tuple(shape)} on {device}, got {got}")
     return t.contiguous()
@@ -1500,6 +1500,25 @@ def _int64(v, name: str) -> int:
     return v - (1 << 64) if v >= (1 << 63) else v
 
 
+class _on:
+    """make `device` the current one for a call; `.stream` = its current stream"""
+    __slots__ = ("dev", "prev", "stream")
+
+    def __init__(self, device):
+        self.dev = device.index
+
+    def __enter__(self):
+        self.prev = torch._C._cuda_getDevice()
+        if self.prev != self.dev:
+            torch.cuda.set_device(self.dev)
+        self.stream = torch._C._cuda_getCurrentRawStream(self.dev)
+        return self
+
+    def __exit__(self, *exc):
+        if self.prev != self.dev:
+            torch.cuda.set_device(self.prev)
+
+
 def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Tensor | None = None) -> torch.Tensor:
     """y_i = keep_i ? x_i / (1 - p) : 0 (+ residual_i) -> a new contiguous tensor.  keep_i depends on (seed, offset, i) alone, i = the
     element's index in row-major order of x's shape, whatever its strides (a non-contiguous x is copied first): one word of
@@ -1515,40 +1534,24 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Te
     x_ = x.detach().contiguous()
     r_ = None
     if residual is not None:
-        if tuple(residual.shape) != tuple(x.shape):
+        if residual.shape != x.shape:
             raise HipLibraryError(f"dropout: residual {tuple(residual.shape)} beside x {tuple(x.shape)}")
         _features(residual, "dropout: residual", like=x)
         r_ = residual.detach().contiguous()
     seed, offset = _int64(seed, "dropout: seed"), _int64(offset, "dropout: offset")
-    y = torch.empty_like(x_, memory_format=torch.contiguous_format)
+    y = torch.empty_like(x_)
     if x_.numel():
-        with _on(x.device):
+        with _on(x.device) as on:
             _lib.check(_lib.load().creste_dropout(x_.data_ptr(), r_.data_ptr() if r_ is not None else None, y.data_ptr(), x_.numel(),
                                                   code, float(p), seed, offset, state.data_ptr() if state is not None else None,
-                                                  _stream()), "dropout")
+                                                  on.stream), "dropout")
     return y
-
-
-class _on:
-    """make `device` the current one for a call (no work when it already is)"""
-
-    def __init__(self, device):
-        self.dev = device.index if device.index is not None else torch.cuda.current_device()
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *exc):
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.prev)
 
 
 def _recurrence_args(gate, x, h0, lengths):
     code = _features(gate, "gated_recurrence: gate", 3)
     _features(x, "gated_recurrence: x", 3, like=gate)
-    if tuple(x.shape) != tuple(gate.shape):
+    if x.shape != gate.shape:
         raise HipLibraryError(f"gated_recurrence: gate {tuple(gate.shape)} beside x {tuple(x.shape)}")
     B, T, Cc = gate.shape
     if h0 is not None:
@@ -1573,7 +1576,7 @@ def gated_recurrence(gate: torch.Tensor, x: torch.Tensor, h0: torch.Tensor | Non
     if h.numel() == 0:
         last = h0.clone() if h0 is not None else torch.zeros((B, Cc), dtype=torch.float32, device=dev)
         return (h, last, torch.empty(0, dtype=torch.float32, device=dev)) if save else (h, last)
-    with _on(dev):
+    with _on(dev) as on:
         last = torch.empty((B, Cc), dtype=torch.float32, device=dev)
         starts = None
         if save:
@@ -1583,7 +1586,7 @@ def gated_recurrence(gate: torch.Tensor, x: torch.Tensor, h0: torch.Tensor | Non
         _lib.check(lib.creste_gated_recurrence_forward(
             g_.data_ptr(), g_.stride(0), g_.stride(1), x_.data_ptr(), x_.stride(0), x_.stride(1),
             h0.data_ptr() if h0 is not None else None, lengths.data_ptr() if lengths is not None else None, B, T, Cc, code,
-            h.data_ptr(), last.data_ptr(), starts.data_ptr() if save else None, work.data_ptr(), nb, _stream()),
+            h.data_ptr(), last.data_ptr(), starts.data_ptr() if save else None, work.data_ptr(), nb, on.stream),
             "gated_recurrence_forward")
     return (h, last, starts) if save else (h, last)
 
@@ -1604,14 +1607,14 @@ def gated_recurrence_bwd(gate, x, lengths, starts, gh, gh_last=None):
     d_ = _rows(gh.detach())
     lib = _lib.load()
     starts = _plain(starts, torch.float32, (-(-T // lib.creste_gated_recurrence_chunk_steps()), B, Cc), dev, "gated_recurrence: starts")
-    with _on(dev):
+    with _on(dev) as on:
         gh0 = torch.empty((B, Cc), dtype=torch.float32, device=dev)
         nb = lib.creste_gated_recurrence_workspace_bytes(B, T, Cc)
         work = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
         _lib.check(lib.creste_gated_recurrence_backward(
             g_.data_ptr(), g_.stride(0), g_.stride(1), x_.data_ptr(), x_.stride(0), x_.stride(1), d_.data_ptr(), d_.stride(0),
             d_.stride(1), gh_last.data_ptr() if gh_last is not None else None, lengths.data_ptr() if lengths is not None else None,
-            starts.data_ptr(), B, T, Cc, code, gg.data_ptr(), gx.data_ptr(), gh0.data_ptr(), work.data_ptr(), nb, _stream()),
+            starts.data_ptr(), B, T, Cc, code, gg.data_ptr(), gx.data_ptr(), gh0.data_ptr(), work.data_ptr(), nb, on.stream),
             "gated_recurrence_backward")
     return gg, gx, gh0
 
@@ -1643,13 +1646,13 @@ def linear_ce(x, w, labels, ignore_index: int = -100, temperature: float = 1.0, 
     if N == 0:
         return loss.zero_(), nll, lse2, stat.zero_()
     lib = _lib.load()
-    with _on(dev):
+    with _on(dev) as on:
         nb = lib.creste_linear_ce_workspace_bytes(N, V, D, code, 0)
         work = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
         _lib.check(lib.creste_linear_ce_forward(x_.data_ptr(), _row_stride(x_), w_.data_ptr(), _row_stride(w_), labels.data_ptr(), N, V, D,
                                                 code, int(ignore_index), float(temperature), int(reduction == "mean"),
                                                 loss.data_ptr(), nll.data_ptr(), lse2.data_ptr(), stat.data_ptr(),
-                                                work.data_ptr(), nb, _stream()), "linear_ce_forward")
+                                                work.data_ptr(), nb, on.stream), "linear_ce_forward")
     return loss, nll, lse2, stat
 
 
@@ -1669,12 +1672,12 @@ def linear_ce_bwd(x, w, labels, lse2, stat, g_loss, ignore_index: int = -100, te
     stat = _plain(stat, torch.float32, (2,), dev, "linear_cross_entropy: stat")
     g_loss = _plain(g_loss.reshape(1), torch.float32, (1,), dev, "linear_cross_entropy: cotangent")
     lib = _lib.load()
-    with _on(dev):
+    with _on(dev) as on:
         nb = lib.creste_linear_ce_workspace_bytes(N, V, D, code, 1)
         work = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
         _lib.check(lib.creste_linear_ce_backward(x_.data_ptr(), _row_stride(x_), w_.data_ptr(), _row_stride(w_), labels.data_ptr(), N, V,
                                                  D, code, int(ignore_index), float(temperature), int(reduction == "mean"),
                                                  lse2.data_ptr(), stat.data_ptr(), g_loss.data_ptr(),
                                                  gx.data_ptr() if need_x else None, gw.data_ptr() if need_w else None,
-                                                 work.data_ptr(), nb, _stream()), "linear_ce_backward")
+                                                 work.data_ptr(), nb, on.stream), "linear_ce_backward")
     return gx, gw

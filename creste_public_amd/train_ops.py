@@ -608,6 +608,12 @@ def reward_forward_train(net, x: torch.Tensor) -> torch.Tensor:
     return RewardFn.apply(eng, x, *eng.params())
 
 
+def once(fn):
+    """@once_differentiable whose bookkeeping is only paid when the backward itself is recorded (create_graph=True)"""
+    recorded = once_differentiable(fn)
+    return lambda ctx, *g: recorded(ctx, *g) if torch.is_grad_enabled() else fn(ctx, *g)
+
+
 class DropoutFn(torch.autograd.Function):
     """ops.dropout under autograd: no mask is kept, the backward draws the same words again (a seed TENSOR must therefore still hold
     its values when the backward runs; autograd's version check raises if it was written in between)."""
@@ -620,12 +626,12 @@ class DropoutFn(torch.autograd.Function):
         return ops.dropout(x, p, seed, offset, residual)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, gy):
+    def backward(ctx, gy):                     # linear in gy: the same operator, differentiable once more if asked for
         p, seed, offset = ctx.args
         if seed is None:
             seed, = ctx.saved_tensors
-        gx = ops.dropout(gy, p, seed, offset) if ctx.needs_input_grad[0] else None
+        drop = DropoutFn.apply if torch.is_grad_enabled() else ops.dropout
+        gx = drop(gy, p, seed, offset, None) if ctx.needs_input_grad[0] else None
         return gx, None, None, None, gy if ctx.needs_input_grad[4] else None
 
 
@@ -648,7 +654,7 @@ class GatedRecurrenceFn(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, gh, gh_last):
         if gh is None and gh_last is None:
             return None, None, None, None
