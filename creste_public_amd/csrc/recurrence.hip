@@ -8,17 +8,22 @@
 // Chunks of one column group meet by look-back: a workgroup publishes its chunk's (A, B), fetches those of the chunks in front of
 // it in its window of 16 and the value carried into the window (published by the window in front), the 8 waves two each at once.
 // Always the same pairs in the same order, whoever is ready first: results do not depend on timing.
-// Work is handed out by a ticket, so a chunk only ever waits for chunks that started earlier: every wait ends.  Each published word
+// Chunks are handed out by tickets, so one only ever waits for chunks that started earlier: every wait ends.  Each published word
 // is 8 bytes written at once, valid when not zero -- (-A, B): A >= 0, so the sign bit marks it -- hence no fences.  (The spin is
 // bounded all the same: past the bound the columns become NaN.)
-// The backward recomputes h inside a chunk from the chunk's starting state, which the forward saves (4 bytes per 8 * LR steps).
+// The backward recomputes h inside a chunk from the chunk's starting state, which the forward saves (4 bytes per 64 steps).
 // Steps behind a sequence's length have f = 1, u = 0, dh = 0: states and cotangents pass through unchanged.
-// Bound: HBM (forward 3 elements, backward 5 per step and channel), a single step: launch latency.
+// Bound: HBM (forward 3 elements, backward 5 per step and channel), a single step: launch latency.  Measured, 4 x 16384 x 1024
+// bf16: forward 100 us (4.0 TB/s), backward 183 us (3.7 TB/s; a large copy: 5.1); two passes over the data with a launch between
+// them took 176 and 280.  Flags that a single lane polls, or windows of windows to shorten the chain, were slower (more round trips).
 #include "common.h"
 
 namespace creste {
 
-constexpr int kRecRun = 8, kRecWaves = 8, kRecChunk = kRecRun * kRecWaves;
+// steps a wave holds: 16 in the forward (4 x 16384 x 1024 bf16: 100 us against 121 with 8: half as many workgroups to meet), 8 in the
+// backward, whose 16 would leave one workgroup per CU (191 us against 183)
+constexpr int kRecWaves = 8, kRecRunF = 16, kRecRunB = 8;
+constexpr int kRecChunkF = kRecRunF * kRecWaves, kRecChunkB = kRecRunB * kRecWaves;
 
 struct RecArgs {
   const void *gate, *x, *gh;
@@ -29,11 +34,11 @@ struct RecArgs {
   int chunks, groups;
   void *h, *ggate, *gx;
   float *h_last, *starts, *gh0;
-  unsigned* ticket;                             // zeroed, as the words below
-  uint64_t *pair, *known;                       // [chunks][BC] (-A, B) of a chunk; (carried value behind it, 1)
+  unsigned* ticket;                             // [groups][16]; zeroed, as the words below
+  uint64_t *pair, *known;                       // [chunks][BC] (-A, B) of a chunk; [chunks / 16][BC] (carried value behind a window, 1)
 };
 
-constexpr int kRecSpin = 1 << 22, kRecWindow = 16;
+constexpr int kRecSpin = 1 << 22, kRecWindow = 16, kRecTicket = 16;
 
 __device__ __forceinline__ uint64_t rec_word(unsigned lo, float hi) { return (uint64_t)__float_as_uint(hi) << 32 | lo; }
 __device__ __forceinline__ uint64_t rec_get(const uint64_t* p) {
@@ -80,24 +85,22 @@ __device__ __forceinline__ int rec_live(int64_t t0, int64_t len) {
   return n < 0 ? 0 : n > LR ? LR : (int)n;
 }
 
-// which (column group, chunk in the order of the recurrence) this workgroup takes
+// which (column group, chunk in the order of the recurrence) this workgroup takes.  One counter per group, a cache line each: chunks
+// wait within their group only
 __device__ __forceinline__ void rec_ticket(const RecArgs& p, int& group, int& turn) {
-  if (p.chunks == 1) {
-    group = blockIdx.x;
-    turn = 0;
-    return;
-  }
+  group = blockIdx.x % p.groups;
+  turn = 0;
+  if (p.chunks == 1) return;
   __shared__ unsigned t;
-  if (threadIdx.x == 0 && threadIdx.y == 0) t = atomicAdd(p.ticket, 1u);
+  if (threadIdx.x == 0 && threadIdx.y == 0) t = atomicAdd(p.ticket + (int64_t)group * kRecTicket, 1u);
   __syncthreads();
-  group = __builtin_amdgcn_readfirstlane((int)(t % (unsigned)p.groups));
-  turn = __builtin_amdgcn_readfirstlane((int)(t / (unsigned)p.groups));
+  turn = __builtin_amdgcn_readfirstlane((int)t);
 }
 
 // s (on entry the value in front of the first chunk) <- the value carried into this chunk.  (A, B): this chunk's pair.  turn = the
-// chunk's place in the order of the recurrence, step = +1 / -1 that order in chunks.  All threads of the workgroup call and get the result
+// chunk's place in the order of the recurrence.  All threads of the workgroup call and get the result
 template <int VEC>
-__device__ __forceinline__ void rec_lookback(const RecArgs& p, const RecCol<VEC>& k, int ch, int turn, int step, const float (&A)[VEC],
+__device__ __forceinline__ void rec_lookback(const RecArgs& p, const RecCol<VEC>& k, int turn, const float (&A)[VEC],
                                              const float (&B)[VEC], float (&s)[VEC]) {
   __shared__ float2 sh[kRecWindow][64 * VEC];
   __shared__ float carried[64 * VEC];
@@ -106,28 +109,31 @@ __device__ __forceinline__ void rec_lookback(const RecArgs& p, const RecCol<VEC>
   if (w == 0 && k.on && !last)                  // (nobody asks for the pair of a window's last chunk)
 #pragma unroll
     for (int e = 0; e < VEC; ++e)
-      rec_put(p.pair + (int64_t)ch * p.BC + k.col + e, rec_word(__float_as_uint(A[e]) | 0x80000000u, B[e]));
-  // wave w fetches the pairs number w and w + 8 of the window, the last wave the value carried into the window
-  const uint64_t* src[3] = {nullptr, nullptr, nullptr};
+      rec_put(p.pair + (int64_t)turn * p.BC + k.col + e, rec_word(__float_as_uint(A[e]) | 0x80000000u, B[e]));
+  // wave w fetches the pairs number w, w + 8, .. of the window, the last wave the value carried into the window
+  constexpr int PQ = kRecWindow / kRecWaves;
+  const uint64_t* src[PQ + 1];
 #pragma unroll
-  for (int q = 0; q < 2; ++q)
-    if (w + kRecWaves * q < at_w) src[q] = p.pair + (int64_t)(ch - step * (at_w - w - kRecWaves * q)) * p.BC + k.col;
-  if (w == kRecWaves - 1 && base > 0) src[2] = p.known + (int64_t)(ch - step * (at_w + 1)) * p.BC + k.col;
-  uint64_t v[3][VEC];
+  for (int q = 0; q <= PQ; ++q) src[q] = nullptr;
+#pragma unroll
+  for (int q = 0; q < PQ; ++q)
+    if (w + kRecWaves * q < at_w) src[q] = p.pair + (int64_t)(base + w + kRecWaves * q) * p.BC + k.col;
+  if (w == kRecWaves - 1 && base > 0) src[PQ] = p.known + (int64_t)(base / kRecWindow - 1) * p.BC + k.col;
+  uint64_t v[PQ + 1][VEC];
   for (int spin = 0;; ++spin) {
     bool all = true;
 #pragma unroll
-    for (int q = 0; q < 3; ++q)
+    for (int q = 0; q <= PQ; ++q)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[q][e] = src[q] ? rec_get(src[q] + e) : 1;
 #pragma unroll
-    for (int q = 0; q < 3; ++q)
+    for (int q = 0; q <= PQ; ++q)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) all &= v[q][e] != 0;
     if (__all(all)) break;
     if (spin == kRecSpin) {
 #pragma unroll
-      for (int q = 0; q < 3; ++q)
+      for (int q = 0; q <= PQ; ++q)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[q][e] = rec_word(0x7fc00000u, __builtin_nanf(""));
       break;
@@ -137,11 +143,11 @@ __device__ __forceinline__ void rec_lookback(const RecArgs& p, const RecCol<VEC>
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
+    for (int q = 0; q < PQ; ++q)
       if (src[q])
         sh[w + kRecWaves * q][threadIdx.x * VEC + e] =
             make_float2(__uint_as_float((unsigned)v[q][e] & 0x7fffffffu), __uint_as_float((unsigned)(v[q][e] >> 32)));
-    if (src[2]) carried[threadIdx.x * VEC + e] = __uint_as_float((unsigned)(v[2][e] >> 32));
+    if (src[PQ]) carried[threadIdx.x * VEC + e] = __uint_as_float((unsigned)(v[PQ][e] >> 32));
   }
   __syncthreads();
 #pragma unroll
@@ -151,7 +157,7 @@ __device__ __forceinline__ void rec_lookback(const RecArgs& p, const RecCol<VEC>
       const float2 q = sh[j][threadIdx.x * VEC + e];
       s[e] = fmaf(q.x, s[e], q.y);
     }
-    if (last && w == 0 && k.on) rec_put(p.known + (int64_t)ch * p.BC + k.col + e, rec_word(1u, fmaf(A[e], s[e], B[e])));
+    if (last && w == 0 && k.on) rec_put(p.known + (int64_t)(turn / kRecWindow) * p.BC + k.col + e, rec_word(1u, fmaf(A[e], s[e], B[e])));
   }
 }
 
@@ -225,16 +231,15 @@ __global__ __launch_bounds__(512, 4) void rec_forward_kernel(RecArgs p) {
     }
   }
   if constexpr (LR > 1)
-    if (p.chunks > 1) rec_lookback<VEC>(p, k, ch, ch, 1, A, B, s);
-  if (w == 0 && k.on) {
+    if (p.chunks > 1) rec_lookback<VEC>(p, k, ch, A, B, s);
+  if (w == 0 && k.on && ch == p.chunks - 1)
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if (p.starts) p.starts[(int64_t)ch * p.BC + k.col + e] = s[e];
-      if (ch == p.chunks - 1) p.h_last[k.col + e] = fmaf(A[e], s[e], B[e]);
-    }
-  }
+    for (int e = 0; e < VEC; ++e) p.h_last[k.col + e] = fmaf(A[e], s[e], B[e]);
 #pragma unroll
   for (int e = 0; e < VEC; ++e) s[e] = fmaf(wa[e], s[e], wb[e]);
+  if (p.starts && k.on && (LR == 1 || t0 % kRecChunkB == 0) && t0 < p.T)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) p.starts[t0 / kRecChunkB * p.BC + k.col + e] = s[e];
   T* hp = (T*)p.h + (k.b * p.T) * p.C + k.c;
 #pragma unroll
   for (int i = 0; i < LR; ++i) {
@@ -341,7 +346,7 @@ __global__ __launch_bounds__(512, 4) void rec_backward_kernel(RecArgs p) {
     }
   }
   if constexpr (LR > 1)
-    if (p.chunks > 1) rec_lookback<VEC>(p, k, ch, turn, -1, A, B, s);
+    if (p.chunks > 1) rec_lookback<VEC>(p, k, turn, A, B, s);
   if (w == 0 && k.on && ch == 0 && p.gh0)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) p.gh0[k.col + e] = fmaf(A[e], s[e], B[e]);
@@ -372,16 +377,19 @@ __global__ __launch_bounds__(256) void rec_zero_kernel(uint4* __restrict__ p, in
 
 namespace {
 
-int64_t rec_chunks(int64_t T) { return (T + kRecChunk - 1) / kRecChunk; }
+int64_t rec_chunks(int64_t T) { return (T + kRecChunkB - 1) / kRecChunkB; }     // the smaller of the two chunks
 
-// the ticket (16 bytes) and the two arrays of published words, a multiple of 16 bytes in all
+// The workspace, all zero at the start: a ticket line per column group (sized as if a lane took one column), the published pairs
+// and values; a multiple of 16 bytes in all
+int64_t rec_tickets(int64_t BC) { return (BC + 63) / 64 * kRecTicket * 4; }
 int64_t rec_work(int64_t BC, int64_t T) {
   const int64_t n = rec_chunks(T);
-  return n == 1 ? 16 : 16 + 16 * ((n * BC + 1) / 2 * 2);
+  return n == 1 ? 16 : rec_tickets(BC) + ((n + n / kRecWindow) * BC + 1) / 2 * 16;
 }
 
-template <typename T, int VEC, int LR>
+template <typename T, int VEC, int LF, int LB>
 int rec_launch(RecArgs& p, bool bwd, char* work, hipStream_t s) {
+  const int LR = bwd ? LB : LF;
   const int64_t groups = (p.BC / VEC + 63) / 64;
   int64_t nw = (p.T + LR - 1) / LR;
   nw = nw > kRecWaves ? kRecWaves : nw;
@@ -392,14 +400,14 @@ int rec_launch(RecArgs& p, bool bwd, char* work, hipStream_t s) {
   if (chunks > 1) {
     const int64_t n = rec_work(p.BC, p.T) / 16, nb = (n + 255) / 256;
     p.ticket = (unsigned*)work;
-    p.pair = (uint64_t*)(work + 16);
+    p.pair = (uint64_t*)(work + rec_tickets(p.BC));
     p.known = p.pair + chunks * p.BC;
     rec_zero_kernel<<<(int)(nb > 2048 ? 2048 : nb), 256, 0, s>>>((uint4*)work, n);
     CRESTE_CHECK_LAUNCH("gated_recurrence zero");
   }
   const dim3 grid((unsigned)(groups * chunks)), block(64, (unsigned)nw);
-  if (bwd) rec_backward_kernel<T, VEC, LR><<<grid, block, 0, s>>>(p);
-  else rec_forward_kernel<T, VEC, LR><<<grid, block, 0, s>>>(p);
+  if (bwd) rec_backward_kernel<T, VEC, LB><<<grid, block, 0, s>>>(p);
+  else rec_forward_kernel<T, VEC, LF><<<grid, block, 0, s>>>(p);
   CRESTE_CHECK_LAUNCH("gated_recurrence");
   return CRESTE_OK;
 }
@@ -410,8 +418,8 @@ int rec_typed(RecArgs& p, bool bwd, char* work, hipStream_t s) {
   const uintptr_t ptrs = (uintptr_t)p.gate | (uintptr_t)p.x | (uintptr_t)p.gh | (uintptr_t)p.h | (uintptr_t)p.ggate | (uintptr_t)p.gx;
   const int64_t strides = p.C | p.g_sb | p.g_st | p.x_sb | p.x_st | p.h_sb | p.h_st;
   const bool two = (ptrs & (2 * sizeof(T) - 1)) == 0 && (strides & 1) == 0;
-  if (p.T == 1) return two ? rec_launch<T, 2, 1>(p, bwd, work, s) : rec_launch<T, 1, 1>(p, bwd, work, s);
-  return two ? rec_launch<T, 2, kRecRun>(p, bwd, work, s) : rec_launch<T, 1, kRecRun>(p, bwd, work, s);
+  if (p.T == 1) return two ? rec_launch<T, 2, 1, 1>(p, bwd, work, s) : rec_launch<T, 1, 1, 1>(p, bwd, work, s);
+  return two ? rec_launch<T, 2, kRecRunF, kRecRunB>(p, bwd, work, s) : rec_launch<T, 1, kRecRunF, kRecRunB>(p, bwd, work, s);
 }
 
 int rec_run(RecArgs& p, int dtype, bool bwd, char* work, hipStream_t s) {
@@ -433,7 +441,7 @@ int rec_check(int64_t B, int64_t T, int64_t C) {
 
 using namespace creste;
 
-extern "C" int creste_gated_recurrence_chunk_steps(void) { return kRecChunk; }
+extern "C" int creste_gated_recurrence_chunk_steps(void) { return kRecChunkB; }
 
 extern "C" int64_t creste_gated_recurrence_workspace_bytes(int64_t B, int64_t T, int64_t C) {
   if (B <= 0 || T <= 0 || C <= 0 || B >= (1ll << 31) || C >= (1ll << 31) || B * C >= (1ll << 40) || T >= (1ll << 36)) return -1;
