@@ -23,7 +23,7 @@ namespace creste {
 // steps a wave holds: 16 in the forward (4 x 16384 x 1024 bf16: 100 us against 121 with 8: half as many workgroups to meet), 8 in the
 // backward, whose 16 would leave one workgroup per CU (191 us against 183)
 constexpr int kRecWaves = 8, kRecRunF = 16, kRecRunB = 8;
-constexpr int kRecChunkF = kRecRunF * kRecWaves, kRecChunkB = kRecRunB * kRecWaves;
+constexpr int kRecChunkB = kRecRunB * kRecWaves;                     // the backward's chunk: one saved state each
 
 struct RecArgs {
   const void *gate, *x, *gh;
@@ -382,9 +382,8 @@ int64_t rec_chunks(int64_t T) { return (T + kRecChunkB - 1) / kRecChunkB; }     
 // The workspace, all zero at the start: a ticket line per column group (sized as if a lane took one column), the published pairs
 // and values; a multiple of 16 bytes in all
 int64_t rec_tickets(int64_t BC) { return (BC + 63) / 64 * kRecTicket * 4; }
-int64_t rec_work(int64_t BC, int64_t T) {
-  const int64_t n = rec_chunks(T);
-  return n == 1 ? 16 : rec_tickets(BC) + ((n + n / kRecWindow) * BC + 1) / 2 * 16;
+int64_t rec_work(int64_t BC, int64_t chunks) {
+  return chunks == 1 ? 16 : rec_tickets(BC) + ((chunks + chunks / kRecWindow) * BC + 1) / 2 * 16;
 }
 
 template <typename T, int VEC, int LF, int LB>
@@ -398,7 +397,7 @@ int rec_launch(RecArgs& p, bool bwd, char* work, hipStream_t s) {
   p.chunks = (int)chunks;
   p.groups = (int)groups;
   if (chunks > 1) {
-    const int64_t n = rec_work(p.BC, p.T) / 16, nb = (n + 255) / 256;
+    const int64_t n = rec_work(p.BC, chunks) / 16, nb = (n + 255) / 256;
     p.ticket = (unsigned*)work;
     p.pair = (uint64_t*)(work + rec_tickets(p.BC));
     p.known = p.pair + chunks * p.BC;
@@ -445,7 +444,7 @@ extern "C" int creste_gated_recurrence_chunk_steps(void) { return kRecChunkB; }
 
 extern "C" int64_t creste_gated_recurrence_workspace_bytes(int64_t B, int64_t T, int64_t C) {
   if (B <= 0 || T <= 0 || C <= 0 || B >= (1ll << 31) || C >= (1ll << 31) || B * C >= (1ll << 40) || T >= (1ll << 36)) return -1;
-  return rec_work(B * C, T);
+  return rec_work(B * C, rec_chunks(T));
 }
 
 extern "C" int creste_gated_recurrence_forward(const void* gate, int64_t gate_sb, int64_t gate_st, const void* x, int64_t x_sb,

@@ -180,8 +180,8 @@ class LinearCEFn(torch.autograd.Function):
     @once
     def backward(ctx, gl, _):
         x, weight, labels, lse2, stat = ctx.saved_tensors
-        gx, gw = ops.linear_ce_bwd(x, weight, labels, lse2, stat, gl, *ctx.args, need_x=ctx.needs_input_grad[0],
-                                   need_w=ctx.needs_input_grad[1])
+        gx, gw = ops._linear_ce_bwd(ops._rows(x), ops._rows(weight), labels.contiguous(), lse2, stat, gl, *ctx.args,
+                                    ctx.needs_input_grad[0], ctx.needs_input_grad[1], ops._DTYPE_CODE[x.dtype])
         return gx, gw, None, None, None, None
 
 

@@ -1531,20 +1531,23 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Te
     state = None
     if isinstance(seed, torch.Tensor):
         state, seed = _plain(seed, torch.int64, (2,), x.device, "dropout: seed tensor"), 0
-    x_ = x.detach().contiguous()
     r_ = None
     if residual is not None:
         if residual.shape != x.shape:
             raise HipLibraryError(f"dropout: residual {tuple(residual.shape)} beside x {tuple(x.shape)}")
         _features(residual, "dropout: residual", like=x)
         r_ = residual.detach().contiguous()
-    seed, offset = _int64(seed, "dropout: seed"), _int64(offset, "dropout: offset")
-    y = torch.empty_like(x_)
-    if x_.numel():
+    return _dropout(x.detach().contiguous(), r_, float(p), _int64(seed, "dropout: seed"), _int64(offset, "dropout: offset"), state, code)
+
+
+def _dropout(x, residual, p, seed, offset, state, code):
+    """dropout of checked, contiguous tensors"""
+    y, n = torch.empty_like(x), x.numel()
+    if n:
         with _on(x.device) as on:
-            _lib.check(_lib.load().creste_dropout(x_.data_ptr(), r_.data_ptr() if r_ is not None else None, y.data_ptr(), x_.numel(),
-                                                  code, float(p), seed, offset, state.data_ptr() if state is not None else None,
-                                                  on.stream), "dropout")
+            _lib.check(_lib.load().creste_dropout(x.data_ptr(), residual.data_ptr() if residual is not None else None, y.data_ptr(), n,
+                                                  code, p, seed, offset, state.data_ptr() if state is not None else None, on.stream),
+                       "dropout")
     return y
 
 
@@ -1582,7 +1585,7 @@ def gated_recurrence(gate: torch.Tensor, x: torch.Tensor, h0: torch.Tensor | Non
         if save:
             starts = torch.empty((-(-T // lib.creste_gated_recurrence_chunk_steps()), B, Cc), dtype=torch.float32, device=dev)
         nb = lib.creste_gated_recurrence_workspace_bytes(B, T, Cc)
-        work = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
+        work = torch.empty(nb, dtype=torch.uint8, device=dev)
         _lib.check(lib.creste_gated_recurrence_forward(
             g_.data_ptr(), g_.stride(0), g_.stride(1), x_.data_ptr(), x_.stride(0), x_.stride(1),
             h0.data_ptr() if h0 is not None else None, lengths.data_ptr() if lengths is not None else None, B, T, Cc, code,
@@ -1601,19 +1604,27 @@ def gated_recurrence_bwd(gate, x, lengths, starts, gh, gh_last=None):
         raise HipLibraryError(f"gated_recurrence: gh {tuple(gh.shape)} beside gate {(B, T, Cc)}")
     if gh_last is not None:
         gh_last = _plain(gh_last.detach(), torch.float32, (B, Cc), dev, "gated_recurrence: gh_last")
-    gg, gx = torch.empty((B, T, Cc), dtype=g_.dtype, device=dev), torch.empty((B, T, Cc), dtype=g_.dtype, device=dev)
+    if T:
+        starts = _plain(starts, torch.float32, (-(-T // _lib.load().creste_gated_recurrence_chunk_steps()), B, Cc), dev,
+                        "gated_recurrence: starts")
+    return _recurrence_bwd(g_, x_, lengths, starts, _rows(gh.detach()), gh_last, code)
+
+
+def _recurrence_bwd(gate, x, lengths, starts, gh, gh_last, code):
+    """gated_recurrence_bwd of checked tensors (lengths / starts / gh_last contiguous)"""
+    B, T, Cc = gate.shape
+    gg = torch.empty((B, T, Cc), dtype=gate.dtype, device=gate.device)
+    gx = torch.empty_like(gg)
+    gh0 = torch.empty((B, Cc), dtype=torch.float32, device=gate.device)
     if gg.numel() == 0:
-        return gg, gx, gh_last.clone() if gh_last is not None else torch.zeros((B, Cc), dtype=torch.float32, device=dev)
-    d_ = _rows(gh.detach())
+        return gg, gx, gh0.copy_(gh_last) if gh_last is not None else gh0.zero_()
     lib = _lib.load()
-    starts = _plain(starts, torch.float32, (-(-T // lib.creste_gated_recurrence_chunk_steps()), B, Cc), dev, "gated_recurrence: starts")
-    with _on(dev) as on:
-        gh0 = torch.empty((B, Cc), dtype=torch.float32, device=dev)
+    with _on(gate.device) as on:
         nb = lib.creste_gated_recurrence_workspace_bytes(B, T, Cc)
-        work = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
+        work = torch.empty(nb, dtype=torch.uint8, device=gate.device)
         _lib.check(lib.creste_gated_recurrence_backward(
-            g_.data_ptr(), g_.stride(0), g_.stride(1), x_.data_ptr(), x_.stride(0), x_.stride(1), d_.data_ptr(), d_.stride(0),
-            d_.stride(1), gh_last.data_ptr() if gh_last is not None else None, lengths.data_ptr() if lengths is not None else None,
+            gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1), gh.data_ptr(), gh.stride(0),
+            gh.stride(1), gh_last.data_ptr() if gh_last is not None else None, lengths.data_ptr() if lengths is not None else None,
             starts.data_ptr(), B, T, Cc, code, gg.data_ptr(), gx.data_ptr(), gh0.data_ptr(), work.data_ptr(), nb, on.stream),
             "gated_recurrence_backward")
     return gg, gx, gh0
@@ -1648,7 +1659,7 @@ def linear_ce(x, w, labels, ignore_index: int = -100, temperature: float = 1.0, 
     lib = _lib.load()
     with _on(dev) as on:
         nb = lib.creste_linear_ce_workspace_bytes(N, V, D, code, 0)
-        work = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
+        work = torch.empty(nb, dtype=torch.uint8, device=dev)
         _lib.check(lib.creste_linear_ce_forward(x_.data_ptr(), _row_stride(x_), w_.data_ptr(), _row_stride(w_), labels.data_ptr(), N, V, D,
                                                 code, int(ignore_index), float(temperature), int(reduction == "mean"),
                                                 loss.data_ptr(), nll.data_ptr(), lse2.data_ptr(), stat.data_ptr(),
@@ -1662,21 +1673,26 @@ def linear_ce_bwd(x, w, labels, lse2, stat, g_loss, ignore_index: int = -100, te
     code, x_, w_, labels = _linear_ce_args(x, w, labels, temperature, reduction)
     N, D = x_.shape
     V, dev = w_.shape[0], x_.device
-    gx = torch.empty((N, D), dtype=x_.dtype, device=dev) if need_x else None
-    if N == 0:
-        return gx, torch.zeros((V, D), dtype=x_.dtype, device=dev) if need_w else None
-    gw = torch.empty((V, D), dtype=x_.dtype, device=dev) if need_w else None
-    if not (need_x or need_w):
-        return gx, gw
     lse2 = _plain(lse2, torch.float32, (N,), dev, "linear_cross_entropy: lse2")
     stat = _plain(stat, torch.float32, (2,), dev, "linear_cross_entropy: stat")
     g_loss = _plain(g_loss.reshape(1), torch.float32, (1,), dev, "linear_cross_entropy: cotangent")
+    return _linear_ce_bwd(x_, w_, labels, lse2, stat, g_loss, ignore_index, temperature, reduction, need_x, need_w, code)
+
+
+def _linear_ce_bwd(x, w, labels, lse2, stat, g_loss, ignore_index, temperature, reduction, need_x, need_w, code):
+    """linear_ce_bwd of checked tensors (x and w with contiguous rows, the others contiguous)"""
+    N, D = x.shape
+    V = w.shape[0]
+    gx = torch.empty((N, D), dtype=x.dtype, device=x.device) if need_x else None
+    gw = torch.empty((V, D), dtype=x.dtype, device=x.device) if need_w else None
+    if N == 0 or not (need_x or need_w):
+        return gx, gw.zero_() if need_w else None
     lib = _lib.load()
-    with _on(dev) as on:
+    with _on(x.device) as on:
         nb = lib.creste_linear_ce_workspace_bytes(N, V, D, code, 1)
-        work = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
-        _lib.check(lib.creste_linear_ce_backward(x_.data_ptr(), _row_stride(x_), w_.data_ptr(), _row_stride(w_), labels.data_ptr(), N, V,
-                                                 D, code, int(ignore_index), float(temperature), int(reduction == "mean"),
+        work = torch.empty(nb, dtype=torch.uint8, device=x.device)
+        _lib.check(lib.creste_linear_ce_backward(x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), labels.data_ptr(), N, V, D,
+                                                 code, int(ignore_index), float(temperature), int(reduction == "mean"),
                                                  lse2.data_ptr(), stat.data_ptr(), g_loss.data_ptr(),
                                                  gx.data_ptr() if need_x else None, gw.data_ptr() if need_w else None,
                                                  work.data_ptr(), nb, on.stream), "linear_ce_backward")

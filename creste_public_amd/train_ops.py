@@ -620,18 +620,21 @@ class DropoutFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, p, seed, offset, residual):
-        ctx.args = (p, None if isinstance(seed, torch.Tensor) else seed, offset)
+        y = ops.dropout(x, p, seed, offset, residual)
+        ctx.args = (p, seed, offset)
         if isinstance(seed, torch.Tensor):
+            ctx.args = (p, None, offset)
             ctx.save_for_backward(seed)
-        return ops.dropout(x, p, seed, offset, residual)
+        return y
 
     @staticmethod
     def backward(ctx, gy):                     # linear in gy: the same operator, differentiable once more if asked for
         p, seed, offset = ctx.args
         if seed is None:
             seed, = ctx.saved_tensors
-        drop = DropoutFn.apply if torch.is_grad_enabled() else ops.dropout
-        gx = drop(gy, p, seed, offset, None) if ctx.needs_input_grad[0] else None
+        gx = None
+        if ctx.needs_input_grad[0]:
+            gx = DropoutFn.apply(gy, p, seed, offset, None) if torch.is_grad_enabled() else ops.dropout(gy, p, seed, offset)
         return gx, None, None, None, gy if ctx.needs_input_grad[4] else None
 
 
@@ -651,7 +654,7 @@ class GatedRecurrenceFn(torch.autograd.Function):
             return ops.gated_recurrence(gate, x, h0, lengths)
         h, last, starts = ops.gated_recurrence(gate, x, h0, lengths, save=True)
         ctx.save_for_backward(gate, x, lengths, starts)
-        return h, last
+        return h, last                         # (the backward relies on these checks of its inputs)
 
     @staticmethod
     @once
@@ -661,7 +664,8 @@ class GatedRecurrenceFn(torch.autograd.Function):
         gate, x, lengths, starts = ctx.saved_tensors
         if gh is None:
             gh = torch.zeros((), dtype=gate.dtype, device=gate.device).expand(gate.shape)
-        gg, gx, gh0 = ops.gated_recurrence_bwd(gate, x, lengths, starts, gh, gh_last)
+        gg, gx, gh0 = ops._recurrence_bwd(ops._rows(gate), ops._rows(x), lengths if lengths is None else lengths.contiguous(), starts,
+                                          ops._rows(gh), gh_last if gh_last is None else gh_last.contiguous(), ops._DTYPE_CODE[gate.dtype])
         want = ctx.needs_input_grad
         return gg if want[0] else None, gx if want[1] else None, gh0 if want[2] else None, None
 
