@@ -21,6 +21,7 @@ namespace creste {
 
 typedef float cef4 __attribute__((ext_vector_type(4)));
 typedef float cef16 __attribute__((ext_vector_type(16)));
+typedef int cei4 __attribute__((ext_vector_type(4)));
 typedef short ces4 __attribute__((ext_vector_type(4)));
 typedef short ces8 __attribute__((ext_vector_type(8)));
 typedef _Float16 ceh8 __attribute__((ext_vector_type(8)));
@@ -50,7 +51,8 @@ struct CeArgs {
   const float* amax;                // [2] max|x|, max|w| (two-piece operands) or null
   float2* part;                     // LOSS: [class tile][n] (max, sum) in log2 units
   float* zlab;                      // LOSS: [n] label logit, log2 units
-  const float* lse2;                // GRAD: [n]
+  const float* row_l2;              // GRAD, DX, DW: [rows64] log-sum-exp minus log2 of G's scale, infinity where a row does not count
+  const int* row_lab;               // [rows64] label, -1 where none applies
   char* g;                          // GRAD: [n64][ldg] elements, pieces pg bytes apart
   int64_t ldg, pg;
   int n64;
@@ -60,6 +62,7 @@ struct CeArgs {
   int accumulate;
   void* out;
   int64_t ldo;
+  int m_out;                        // feature columns of the output
   int out_dt;
   const float *gl, *stat;           // dloss, {sum nll, count}
   int mean;
@@ -111,12 +114,12 @@ struct CeTile {
   }
 };
 
-template <int BX, int BK, bool KM>
+template <int BX, int BK, bool KM, int NW>
 __device__ __forceinline__ void ce_dma(char* lds, const char* base, int64_t ld, int64_t rows, int colbytes, int64_t row0, int x0,
                                        int k, int wave, int lane) {
   using L = CeTile<BX, BK, KM>;
 #pragma unroll
-  for (int i0 = 0; i0 < L::INSTR; i0 += 8) {
+  for (int i0 = 0; i0 < L::INSTR; i0 += NW) {
     const int i = i0 + wave;
     const int pos = i * 64 + lane, r = pos / L::CPR, c = (pos % L::CPR) ^ L::swz(r);
     int64_t row = (KM ? (int64_t)k : row0) + r;
@@ -151,17 +154,87 @@ __device__ __forceinline__ ces8 ce_frag(const char* lds, int x0, int kk, int lan
   }
 }
 
-// DT: 16-bit operand type (fp16 for two-piece fp32), P: pieces, BM: tile extent along the accumulator rows
-template <int MODE, int DT, int P, int BM>
-__global__ __launch_bounds__(512, 2) void ce_gemm_kernel(CeArgs p) {
+// a wave's own staging of 32 output rows of RB bytes (a multiple of 256): lanes write 8 or 16 bytes of "their" row, the rows leave in
+// whole 256-byte runs.  16-byte chunks are swizzled by the row so that neither side meets bank conflicts
+template <int RB>
+__device__ __forceinline__ char* ce_stage(char* st, int row, int byte) {
+  return st + row * RB + ((((byte >> 4) ^ (row & 15)) << 4) | (byte & 15));
+}
+
+// the wave's MT x NT accumulator tiles (registers = feature columns from d0, lanes = output rows from row0) to the output or the
+// split's partial sums, 128 columns of 32 rows at a time through the wave's 16 KB of LDS at st
+template <int DT, int MT, int NT>
+__device__ __forceinline__ void ce_store(const CeArgs& p, const cef16 (&acc)[MT][NT], char* st, int row0, int d0, int split, int lane) {
+  constexpr int TP = MT < 4 ? MT : 4, RB = TP * 128, LPR = RB / 16;      // tiles a pass, bytes and lanes of a row
+  static_assert(MT % TP == 0 && (LPR == 32 || LPR == 16), "");
+  const int li = lane & 31, lh = lane >> 5;
+  const float fs = p.partial ? 1.f : ce_out_scale(p);
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int h = 0; h < MT / TP; ++h) {
+#pragma unroll
+      for (int i = 0; i < TP; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const cef16& a = acc[h * TP + i][j];
+          *reinterpret_cast<cef4*>(ce_stage<RB>(st, li, (i * 32 + 8 * q + 4 * lh) * 4)) =
+              cef4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+        }
+      __builtin_amdgcn_wave_barrier();                  // (a wave's LDS operations stay in order)
+#pragma unroll
+      for (int r0 = 0; r0 < 32; r0 += 64 / LPR) {       // whole rows
+        const int r = r0 + lane / LPR, row = row0 + j * 32 + r, c = lane % LPR, d = d0 + h * (TP * 32) + c * 4;
+        cef4 v = *reinterpret_cast<const cef4*>(ce_stage<RB>(st, r, c * 16));
+        if (row >= p.n || d >= p.m_out) continue;
+        if (p.partial) {                                // rows of partials are padded to 4
+          cef4* dst = reinterpret_cast<cef4*>(p.partial + split * p.psplit + row * p.ldp + d);
+          *dst = p.accumulate ? *dst + v : v;
+          continue;
+        }
+        v *= fs;
+        const int64_t o = row * p.ldo + d;
+        if ((p.m_out & 3) == 0) {
+          if (p.out_dt == CRESTE_DT_F32) {
+            *reinterpret_cast<cef4*>((float*)p.out + o) = v;
+          } else {
+            ces4 s;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] = ce_cvt<DT>(v[e]);
+            *reinterpret_cast<ces4*>((short*)p.out + o) = s;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (d + e >= p.m_out) continue;
+            if (p.out_dt == CRESTE_DT_F32) ((float*)p.out)[o + e] = v[e];
+            else ((short*)p.out)[o + e] = ce_cvt<DT>(v[e]);
+          }
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The shape of a workgroup: tile BM x BN by WM x WN waves, BK / P contraction elements a stage, NS stages in LDS
+template <int BM_, int BN_, int WM_, int WN_, int BK_, int NS_>
+struct CeShape {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = BK_, NS = NS_, NW = WM * WN;
+};
+
+// DT: 16-bit operand type (fp16 for two-piece fp32), P: pieces
+template <int MODE, int DT, int P, typename S>
+__global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
   constexpr bool AKM = MODE == CE_DX || MODE == CE_DW, BKM = MODE == CE_DW;
-  constexpr int BN = kCeTile, BK = 64 / P, MT = BM / 64, NT = 2;
+  constexpr int BM = S::BM, BN = S::BN, BK = S::BK / P, NS = S::NS, NW = S::NW, WTM = BM / S::WM, WTN = BN / S::WN;
+  constexpr int MT = WTM / 32, NT = WTN / 32;
   using LA = CeTile<BM, BK, AKM>;
   using LB = CeTile<BN, BK, BKM>;
-  constexpr int STAGE = P * (LA::BYTES + LB::BYTES);
+  constexpr int STAGE = P * (LA::BYTES + LB::BYTES), kDma = STAGE / 1024 / NW;
+  static_assert(LA::INSTR % NW == 0 && LB::INSTR % NW == 0, "every wave issues as many loads");
   extern __shared__ __align__(1024) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, lh = lane >> 5;
-  const int wm = wave >> 2, wn = wave & 3;
+  const int wm = wave / S::WN, wn = wave % S::WN;
   int t = xcd_remap(blockIdx.x, gridDim.x);
   const int tm = t % p.mt;
   t /= p.mt;
@@ -182,57 +255,63 @@ __global__ __launch_bounds__(512, 2) void ce_gemm_kernel(CeArgs p) {
     char* st = smem + s * STAGE;
 #pragma unroll
     for (int q = 0; q < P; ++q) {
-      ce_dma<BM, BK, AKM>(st + q * LA::BYTES, p.a + q * p.pa, p.lda, p.ra, p.ca, m0, m0, k, wave, lane);
-      ce_dma<BN, BK, BKM>(st + P * LA::BYTES + q * LB::BYTES, p.b + q * p.pb, p.ldb, p.rb, p.cb, n0, n0, k, wave, lane);
+      ce_dma<BM, BK, AKM, NW>(st + q * LA::BYTES, p.a + q * p.pa, p.lda, p.ra, p.ca, m0, m0, k, wave, lane);
+      ce_dma<BN, BK, BKM, NW>(st + P * LA::BYTES + q * LB::BYTES, p.b + q * p.pb, p.ldb, p.rb, p.cb, n0, n0, k, wave, lane);
     }
   };
-
-  if (kb < ke) {
-    dma(kb, 0);
-    for (int k = kb, c = 0; k < ke; k += BK, ++c) {
-      __syncthreads();                                  // stage c has landed, everybody has left the other one
-      if (k + BK < ke) dma(k + BK, (c + 1) & 1);
-      const char* A = smem + (c & 1) * STAGE;
-      const char* B = A + P * LA::BYTES;
+  const int n = ke > kb ? (ke - kb) / BK : 0;
 #pragma unroll
-      for (int kk = 0; kk < BK / 16; ++kk) {
-        ces8 af[P][MT], bf[P][NT];
+  for (int s = 0; s < NS - 1; ++s)
+    if (s < n) dma(kb + s * BK, s);
+  int cur = 0, nxt = NS - 1;                            // stage in use, stage to fill
+  for (int c = 0; c < n; ++c) {
+    // this wave's loads of stage c have landed (younger ones: the NS - 2 stages behind it) -- and, past the barrier, everybody's;
+    // everybody has also left stage c - 1, which is the one to fill
+    if (NS > 2 && c + NS - 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * kDma) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (c + NS - 1 < n) dma(kb + (c + NS - 1) * BK, nxt);
+    const char* A = smem + cur * STAGE;
+    const char* B = A + P * LA::BYTES;
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
+    for (int kk = 0; kk < BK / 16; ++kk) {
+      ces8 af[P][MT], bf[P][NT];
 #pragma unroll
-          for (int i = 0; i < MT; ++i) af[q][i] = ce_frag<BM, BK, AKM>(A + q * LA::BYTES, wm * (BM / 2) + i * 32, kk, lane);
+      for (int q = 0; q < P; ++q) {
 #pragma unroll
-          for (int j = 0; j < NT; ++j) bf[q][j] = ce_frag<BN, BK, BKM>(B + q * LB::BYTES, wn * 64 + j * 32, kk, lane);
-        }
+        for (int i = 0; i < MT; ++i) af[q][i] = ce_frag<BM, BK, AKM>(A + q * LA::BYTES, wm * WTM + i * 32, kk, lane);
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            if constexpr (P == 2) {                     // small products first
-              acc[i][j] = ce_mfma<DT>(af[1][i], bf[0][j], acc[i][j]);
-              acc[i][j] = ce_mfma<DT>(af[0][i], bf[1][j], acc[i][j]);
-            }
-            acc[i][j] = ce_mfma<DT>(af[0][i], bf[0][j], acc[i][j]);
-          }
+        for (int j = 0; j < NT; ++j) bf[q][j] = ce_frag<BN, BK, BKM>(B + q * LB::BYTES, wn * WTN + j * 32, kk, lane);
       }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          if constexpr (P == 2) {                       // small products first
+            acc[i][j] = ce_mfma<DT>(af[1][i], bf[0][j], acc[i][j]);
+            acc[i][j] = ce_mfma<DT>(af[0][i], bf[1][j], acc[i][j]);
+          }
+          acc[i][j] = ce_mfma<DT>(af[0][i], bf[0][j], acc[i][j]);
+        }
     }
+    cur = cur + 1 == NS ? 0 : cur + 1;
+    nxt = nxt + 1 == NS ? 0 : nxt + 1;
   }
+  __syncthreads();                                      // the stages are free
 
   if constexpr (MODE == CE_LOSS || MODE == CE_GRAD) {
     const float c2 = ce_operand_inv(p.amax, 0) * ce_operand_inv(p.amax, 1) * p.inv_tau * kCeLog2e;
-    const int mw = m0 + wm * (BM / 2);                  // first class of this wave, within the piece
+    const int mw = m0 + wm * WTM;                       // first class of this wave, within the piece
     if constexpr (MODE == CE_LOSS) {
-      float2* sh = reinterpret_cast<float2*>(smem);     // [wm][256 rows]
-      __syncthreads();
+      float2* sh = reinterpret_cast<float2*>(smem);     // [wm][BN rows]
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int row = n0 + wn * 64 + j * 32 + li;
+        const int row = n0 + wn * WTN + j * 32 + li;
         // the label's class relative to this wave's first one (a label outside [0, classes) matches nothing)
         const int64_t y = row < p.n ? p.labels[row] : -1;
         const int64_t yr = y - mw;
-        const int lab = y >= 0 && y < p.classes && yr >= 0 && yr < BM / 2 ? (int)yr : -1;
+        const int lab = y >= 0 && y < p.classes && yr >= 0 && yr < WTM ? (int)yr : -1;
         float mx = -INFINITY, sum = 0.f, z = 0.f;
-        if (mw + BM / 2 > p.m) {                        // classes behind the last one: exp2 gives 0
+        if (mw + WTM > p.m) {                        // classes behind the last one: exp2 gives 0
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -257,30 +336,28 @@ __global__ __launch_bounds__(512, 2) void ce_gemm_kernel(CeArgs p) {
         const float mo = __shfl_xor(mx, 32, 64), so = __shfl_xor(sum, 32, 64);
         const float mm = fmaxf(mx, mo);
         sum = sum * __builtin_amdgcn_exp2f(mx - mm) + so * __builtin_amdgcn_exp2f(mo - mm);
-        if (lh == 0) sh[wm * 256 + wn * 64 + j * 32 + li] = make_float2(mm, sum);
+        if (lh == 0) sh[wm * BN + wn * WTN + j * 32 + li] = make_float2(mm, sum);
         if (lab >= 0 && ((lab >> 2) & 1) == lh) p.zlab[row] = z * c2;
       }
       __syncthreads();
       const int i = threadIdx.x;
-      if (i < 256 && n0 + i < p.n) {
-        const float2 u = sh[i], v = sh[256 + i];
+      static_assert(S::WM == 2, "");
+      if (i < BN && n0 + i < p.n) {
+        const float2 u = sh[i], v = sh[BN + i];
         const float mm = fmaxf(u.x, v.x);
         p.part[(int64_t)tm * p.n + n0 + i] =
             make_float2(mm, u.y * __builtin_amdgcn_exp2f(u.x - mm) + v.y * __builtin_amdgcn_exp2f(v.x - mm));
       }
     } else {
+      constexpr int RB = WTM * 2;
+      static_assert(RB == 256 && NW * P * 32 * RB <= NS * STAGE, "");
+      char* st = smem + wave * (P * 32 * RB);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int row = n0 + wn * 64 + j * 32 + li;
-        if (row >= p.n64) continue;
-        int64_t y = row < p.n ? p.labels[row] : p.ignore;
-        const bool on = row < p.n && y != p.ignore;
-        // a label that names no class: nll is NaN, and so is its row of G
-        const float scale = !on ? 0.f : (y < 0 || y >= p.classes) ? __builtin_nanf("") : p.gscale;
-        const float l2 = on ? p.lse2[row] : 0.f;
-        const int64_t yr = y - p.class0 - mw;
-        const int lab = on && yr >= 0 && yr < BM / 2 ? (int)yr : -1;
-        char* grow = p.g + row * p.ldg;
+        const int row = n0 + wn * WTN + j * 32 + li;
+        const float l2 = row < p.n64 ? p.row_l2[row] : INFINITY;
+        const int yr = (row < p.n64 ? p.row_lab[row] : -1) - p.class0 - mw;
+        const bool any = __any(yr >= 0 && yr < WTM);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -290,56 +367,284 @@ __global__ __launch_bounds__(512, 2) void ce_gemm_kernel(CeArgs p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float v = __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * q + e], c2, -l2));
-              v = cl + e == lab ? v - 1.f : v;
-              v = on && mw + cl + e < p.m ? v * scale : 0.f;
+              if (any) v = cl + e == yr ? v - p.gscale : v;
+              if (mw + WTM > p.m) v = mw + cl + e < p.m ? v : 0.f;
               const short h = ce_cvt<DT>(v);
               hi[e] = h;
               if constexpr (P == 2) lo[e] = ce_cvt<DT>(v - (float)__builtin_bit_cast(_Float16, h));
             }
-            *reinterpret_cast<ces4*>(grow + (int64_t)(mw + cl) * 2) = hi;
-            if constexpr (P == 2) *reinterpret_cast<ces4*>(grow + p.pg + (int64_t)(mw + cl) * 2) = lo;
+            *reinterpret_cast<ces4*>(ce_stage<RB>(st, li, cl * 2)) = hi;
+            if constexpr (P == 2) *reinterpret_cast<ces4*>(ce_stage<RB>(st + 32 * RB, li, cl * 2)) = lo;
           }
+        __builtin_amdgcn_wave_barrier();                // (a wave's LDS operations stay in order)
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+#pragma unroll
+          for (int r0 = 0; r0 < 32; r0 += 4) {          // 4 rows of 256 bytes per instruction
+            const int r = r0 + (lane >> 4), c = (lane & 15) * 16;
+            const int orow = n0 + wn * WTN + j * 32 + r;
+            const cef4 v = *reinterpret_cast<const cef4*>(ce_stage<RB>(st + q * 32 * RB, r, c));
+            if (orow < p.n64) *reinterpret_cast<cef4*>(p.g + q * p.pg + orow * p.ldg + (int64_t)mw * 2 + c) = v;
+          }
+        __builtin_amdgcn_wave_barrier();
       }
     }
   } else {
-    const float fs = p.partial ? 1.f : ce_out_scale(p);
+    static_assert(NW * 32 * 512 <= NS * STAGE, "");
+    ce_store<DT, MT, NT>(p, acc, smem + wave * (32 * 512), n0 + wn * WTN, m0 + wm * WTM, split, lane);
+  }
+}
+
+// -------------------------------------------------------------------------------------------- up to 256 feature columns
+// The features of a workgroup's OWN items (rows for LOSS and DX, classes for DW) fit in registers, so the other side is streamed past
+// them once: per 32 others a wave forms z (others in the accumulator registers, its own items in the lanes), turns it into G in
+// place and feeds G, still in registers, to the second product -- no G in memory at all, no second kernel.  What makes that free
+// of exchanges: the contraction of the second product may run over the others in any order, so the transposing reads of the
+// streamed tile take them in the order in which the accumulator holds them.  One tile in LDS serves both products (rows for z,
+// transposed for the second), its 16-byte chunks swizzled by the row: a bijection over 16 rows for the row reads, different 64-byte
+// windows for the 4 rows of a transposing read.
+template <int DP, int OTS, int P>
+struct CeStream {
+  static constexpr int ROWB = DP * 2, CPR = ROWB / 16, PIECE = OTS * ROWB, INFO = P * PIECE, BYTES = INFO + 1024, INSTR = PIECE / 1024;
+  static __device__ __forceinline__ int swz(int r) {
+    if constexpr (CPR >= 16) return (r & 3) << 2 | ((r >> 2) & 3);
+    else return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);   // two rows per 256 bytes
+  }
+  static constexpr int RPI = 64 / CPR;       // rows an instruction covers; instruction i + 8 covers the rows 8 * RPI further, whose
+                                             // swizzle is the same: one lane offset serves all of a wave's instructions
+  static __device__ __forceinline__ void dma(char* lds, const CeArgs& p, int64_t o0, int wave, int lane) {
+    const int r0 = wave * RPI + lane / CPR, c = (lane % CPR) ^ swz(r0);
+    const unsigned off = (unsigned)r0 * (unsigned)p.lda + c * 16;
+    const bool inside = o0 + OTS <= p.ra;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int row = n0 + wn * 64 + j * 32 + li;
-      if (row >= p.n) continue;
+    for (int q = 0; q < P; ++q)
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int i0 = 0; i0 < INSTR; i0 += 8) {
+        const char* base = p.a + q * p.pa + (o0 + i0 * RPI) * p.lda;
+        const char* src = base + off;
+        if (!inside) {                       // rows behind the last one: the last one again
+          const int64_t row = o0 + i0 * RPI + r0 < p.ra ? o0 + i0 * RPI + r0 : p.ra - 1;
+          src = p.a + q * p.pa + row * p.lda + c * 16;
+        }
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                         (__attribute__((address_space(3))) void*)(lds + q * PIECE + (i0 + wave) * 1024), 16, 0, 0);
+      }
+  }
+  // Fragment addresses: what depends on the lane alone, then exclusive-or with what the step selects (the selecting bits are those
+  // of the chunk, above them every term is a multiple of the row size)
+  static __device__ __forceinline__ unsigned row_base(int lane) {
+    const int r = lane & 31;
+    return r * ROWB + (((lane >> 5) ^ swz(r)) << 4);
+  }
+  static __device__ __forceinline__ ces8 row(const char* smem, unsigned base, int kk) {
+    return *reinterpret_cast<const ces8*>(smem + ((base ^ ((kk & 7) << 5)) + (kk >> 3) * 256));
+  }
+  // 16 others in the accumulator's order: of a half wave the 4 * lh .. and the 8 + 4 * lh .., feature columns d * 32 ..
+  static __device__ __forceinline__ unsigned across_base(int lane) {
+    const int l = lane & 15, g = lane >> 4, r = 4 * (g >> 1) + (l >> 2);
+    return r * ROWB + (((2 * (g & 1) + ((l & 3) >> 1)) ^ swz(r)) << 4) + (l & 1) * 8;
+  }
+  static __device__ __forceinline__ ces8 across(const char* smem, unsigned base, int d) {
+    ces8 v;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int d = m0 + wm * (BM / 2) + i * 32 + 8 * q + 4 * lh;
-          if (d >= p.m) continue;
-          cef4 v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-          if (p.partial) {                              // rows of partials are padded to 4
-            cef4* dst = reinterpret_cast<cef4*>(p.partial + split * p.psplit + row * p.ldp + d);
-            *dst = p.accumulate ? *dst + v : v;
-            continue;
+    for (int j = 0; j < 2; ++j) {
+      const char* at = smem + (((base + j * 8 * ROWB) ^ (((d & 3) << 6) | j << 5)) + (d >> 2) * 256);
+      const ces4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ces4*)at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * j + e] = t[e];
+    }
+    return v;
+  }
+  // DW: the rows' log-sum-exps (even waves) and labels (odd waves: every wave issues as many loads) behind the features
+  static __device__ __forceinline__ void dma_info(char* lds, const CeArgs& p, int64_t o0, int wave, int lane) {
+    static_assert(OTS == 64, "one 4-byte load per lane");
+    const char* src = wave & 1 ? (const char*)p.row_lab : (const char*)p.row_l2;
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + (o0 + lane) * 4),
+                                     (__attribute__((address_space(3))) void*)(lds + INFO + (wave & 1) * 256), 4, 0, 0);
+  }
+};
+
+constexpr int kCeStage = 64;                 // others per stage
+
+// a = the streamed side (p.m items), b = the own side (p.n items), NT x 32 own items per wave
+template <int MODE, int DT, int P, int DP, int NT>
+__global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
+  using L = CeStream<DP, kCeStage, P>;
+  constexpr int NS = 3, KS = DP / 16, kDma = P * L::INSTR / 8 + (MODE == CE_DW);
+  extern __shared__ __align__(1024) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, lh = lane >> 5;
+  int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int tn = t % p.nt, split = t / p.nt;
+  const int own0 = tn * (256 * NT) + wave * (32 * NT);
+  const int kb = split * p.ksplit, ke = min(p.k1, kb + p.ksplit);
+  const int n = ke > kb ? (ke - kb + kCeStage - 1) / kCeStage : 0;
+
+  ces8 x[P][NT][KS];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int64_t o = own0 + j * 32 + li, row = o < p.n ? o : p.n - 1;
+#pragma unroll
+    for (int q = 0; q < P; ++q)
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) x[q][j][kk] = *reinterpret_cast<const ces8*>(p.b + q * p.pb + row * p.ldb + kk * 32 + lh * 16);
+  }
+  const float c2 = ce_operand_inv(p.amax, 0) * ce_operand_inv(p.amax, 1) * p.inv_tau * kCeLog2e;
+  float l2[NT], mx[NT], sum[NT], zl[NT];
+  int lab[NT];                               // LOSS / DX: the row's label; DW: the own class
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int o = own0 + j * 32 + li;
+    mx[j] = -3.0e38f;
+    sum[j] = zl[j] = l2[j] = 0.f;
+    lab[j] = o;
+    if constexpr (MODE == CE_LOSS) {
+      const int64_t y = o < p.n ? p.labels[o] : -1;
+      lab[j] = y >= 0 && y < p.classes ? (int)y : -1;
+    }
+    if constexpr (MODE == CE_DX) {
+      l2[j] = o < p.n ? p.row_l2[o] : INFINITY;
+      lab[j] = o < p.n ? p.row_lab[o] : -1;
+    }
+  }
+  constexpr int AT = MODE == CE_LOSS ? 1 : DP / 32, AN = MODE == CE_LOSS ? 1 : NT;
+  cef16 acc[AT][AN];
+#pragma unroll
+  for (int d = 0; d < AT; ++d)
+#pragma unroll
+    for (int j = 0; j < AN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][j][r] = 0.f;
+
+  auto fill = [&](int c, int s) __attribute__((always_inline)) {
+    L::dma(smem + s * L::BYTES, p, kb + c * kCeStage, wave, lane);
+    if constexpr (MODE == CE_DW) L::dma_info(smem + s * L::BYTES, p, kb + c * kCeStage, wave, lane);
+  };
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (the counted waits below count stages only)
+#pragma unroll
+  for (int s = 0; s < NS - 1; ++s)
+    if (s < n) fill(s, s);
+  const unsigned rbase = L::row_base(lane), abase = L::across_base(lane);
+  int cur = 0, nxt = NS - 1;
+  for (int c = 0; c < n; ++c) {
+    if (c + NS - 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * kDma) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (c + NS - 1 < n) fill(c + NS - 1, nxt);
+    const char* st = smem + cur * L::BYTES;             // (the rows' values behind the features)
+#pragma unroll 1
+    for (int sub = 0; sub < kCeStage / 32; ++sub) {
+      const int o0 = kb + c * kCeStage + sub * 32;      // first other of this half stage
+      const unsigned stage = cur * L::BYTES + sub * 32 * L::ROWB;
+      cef16 z[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[j][r] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        ces8 a[P];
+#pragma unroll
+        for (int q = 0; q < P; ++q) a[q] = L::row(smem, stage + q * L::PIECE + rbase, kk);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          if constexpr (P == 2) {
+            z[j] = ce_mfma<DT>(a[1], x[0][j][kk], z[j]);
+            z[j] = ce_mfma<DT>(a[0], x[1][j][kk], z[j]);
           }
-          v *= fs;
-          const int64_t o = row * p.ldo + d;
-          if ((p.m & 3) == 0) {
-            if (p.out_dt == CRESTE_DT_F32) {
-              *reinterpret_cast<cef4*>((float*)p.out + o) = v;
-            } else {
-              ces4 s;
+          z[j] = ce_mfma<DT>(a[0], x[0][j][kk], z[j]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);                // (the phases' operands do not fit the registers side by side)
+      const bool edge = o0 + 32 > p.m;                  // others behind the last one
+      ces8 g[P][NT][2];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[e] = ce_cvt<DT>(v[e]);
-              *reinterpret_cast<ces4*>((short*)p.out + o) = s;
+      for (int j = 0; j < NT; ++j) {
+        if (edge && MODE != CE_DW)                      // (DW: such rows have l2 = infinity)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (o0 + (r & 3) + 8 * (r >> 2) + 4 * lh >= p.m) z[j][r] = -INFINITY;
+        if constexpr (MODE == CE_LOSS) {
+          const int rel = lab[j] - o0;
+          if (__any(rel >= 0 && rel < 32))
+#pragma unroll
+            for (int r = 0; r < 16; ++r) zl[j] = (r & 3) + 8 * (r >> 2) + 4 * lh == rel ? z[j][r] : zl[j];
+          float m = z[j][0];
+#pragma unroll
+          for (int r = 1; r < 16; ++r) m = fmaxf(m, z[j][r]);
+          m = fmaxf(mx[j], m * c2);
+          sum[j] *= __builtin_amdgcn_exp2f(mx[j] - m);
+          mx[j] = m;
+          float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s4[r & 3] += __builtin_amdgcn_exp2f(fmaf(z[j][r], c2, -m));
+          sum[j] += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        } else {
+          float v[16];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            cef4 rl;
+            cei4 rb;
+            if constexpr (MODE == CE_DW) {              // of the others, which are rows here (padded to whole stages)
+              rl = *reinterpret_cast<const cef4*>(st + L::INFO + (sub * 32 + 8 * q + 4 * lh) * 4);
+              rb = *reinterpret_cast<const cei4*>(st + L::INFO + 256 + (sub * 32 + 8 * q + 4 * lh) * 4);
             }
-          } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              if (d + e >= p.m) continue;
-              if (p.out_dt == CRESTE_DT_F32) ((float*)p.out)[o + e] = v[e];
-              else ((short*)p.out)[o + e] = ce_cvt<DT>(v[e]);
+              const int r = 4 * q + e;
+              v[r] = __builtin_amdgcn_exp2f(fmaf(z[j][r], c2, MODE == CE_DW ? -rl[e] : -l2[j]));
+              if constexpr (MODE == CE_DW) v[r] = rb[e] == lab[j] ? v[r] - p.gscale : v[r];
             }
           }
+          if constexpr (MODE == CE_DX) {
+            const int rel = lab[j] - o0;
+            if (__any(rel >= 0 && rel < 32))
+#pragma unroll
+              for (int r = 0; r < 16; ++r) v[r] = (r & 3) + 8 * (r >> 2) + 4 * lh == rel ? v[r] - p.gscale : v[r];
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const short h = ce_cvt<DT>(v[r]);
+            g[0][j][r >> 3][r & 7] = h;
+            if constexpr (P == 2) g[P - 1][j][r >> 3][r & 7] = ce_cvt<DT>(v[r] - (float)__builtin_bit_cast(_Float16, h));
+          }
         }
+      }
+      if constexpr (MODE != CE_LOSS) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < AT; ++d)
+#pragma unroll
+          for (int k2 = 0; k2 < 2; ++k2) {
+            ces8 a[P];
+#pragma unroll
+            for (int q = 0; q < P; ++q) a[q] = L::across(smem, stage + q * L::PIECE + k2 * 16 * L::ROWB + abase, d);
+#pragma unroll
+            for (int j = 0; j < AN; ++j) {
+              if constexpr (P == 2) {
+                acc[d][j] = ce_mfma<DT>(a[1], g[0][j][k2], acc[d][j]);
+                acc[d][j] = ce_mfma<DT>(a[0], g[P - 1][j][k2], acc[d][j]);
+              }
+              acc[d][j] = ce_mfma<DT>(a[0], g[0][j][k2], acc[d][j]);
+            }
+          }
+      }
     }
+    cur = cur + 1 == NS ? 0 : cur + 1;
+    nxt = nxt + 1 == NS ? 0 : nxt + 1;
+  }
+  if constexpr (MODE == CE_LOSS) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int row = own0 + j * 32 + li;
+      const float mo = __shfl_xor(mx[j], 32, 64), so = __shfl_xor(sum[j], 32, 64);
+      const float m = fmaxf(mx[j], mo);
+      const float s = sum[j] * __builtin_amdgcn_exp2f(mx[j] - m) + so * __builtin_amdgcn_exp2f(mo - m);
+      if (row >= p.n) continue;
+      if (lh == 0) p.part[(int64_t)split * p.n + row] = make_float2(m, s);
+      if (lab[j] >= kb && lab[j] < ke && ((lab[j] >> 2) & 1) == lh) p.zlab[row] = zl[j] * c2;
+    }
+  } else {
+    __syncthreads();
+    ce_store<DT, DP / 32, NT>(p, acc, smem + wave * (32 * 512), own0, 0, split, lane);
   }
 }
 
@@ -577,13 +882,26 @@ __global__ __launch_bounds__(256) void ce_reduce_kernel(CeArgs p, int splits) {
     const int d = (int)(i - row * p.ldp);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (d + e >= p.m) continue;
+      if (d + e >= p.m_out) continue;
       const int64_t o = row * p.ldo + d + e;
       if (p.out_dt == CRESTE_DT_F32) ((float*)p.out)[o] = v[e];
       else if (p.out_dt == CRESTE_DT_BF16) ((short*)p.out)[o] = ce_cvt<CRESTE_DT_BF16>(v[e]);
       else ((short*)p.out)[o] = ce_cvt<CRESTE_DT_F16>(v[e]);
     }
   }
+}
+
+// what the gradient kernels ask of a row, padded to whole tiles: rows that do not count get an infinite log-sum-exp (G = 0), a label
+// that names no class a NaN (as nll has)
+__global__ __launch_bounds__(256) void ce_rows_kernel(const float* __restrict__ lse2, const int64_t* __restrict__ labels, int n, int n64,
+                                                      int64_t ignore, int classes, float log2_scale, float* __restrict__ l2,
+                                                      int* __restrict__ lab) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n64) return;
+  const int64_t y = i < n ? labels[i] : ignore;
+  const bool on = i < n && y != ignore, ok = y >= 0 && y < classes;
+  l2[i] = !on ? INFINITY : ok ? lse2[i] - log2_scale : __builtin_nanf("");
+  lab[i] = on && ok ? (int)y : -1;
 }
 
 // --------------------------------------------------------------------------------------------------------- host side
@@ -594,17 +912,25 @@ int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 // Where everything sits in the caller's workspace.  The operands are used in place when a row is a multiple of 64 elements on
 // 16-byte boundaries, else copied once (padded; fp32 always: into its two pieces).
 struct CePlan {
-  int P, dt16, es, Dp, ldq, bm;
-  bool packx, packw;
-  int64_t amax, xp, wp, part, zlab, bsum, g, dxp, dwp, total;
+  int P, dt16, es, Dp, ldq, own;   // own: items a streaming workgroup holds
+  bool packx, packw, stream;
+  int64_t amax, xp, wp, part, zlab, bsum, row_l2, row_lab, g, dxp, dwp, total;
   int64_t vc, n64;                 // classes per piece, rows of G
-  int pieces, tiles, sx, sw;       // class tiles of the loss, splits of DX / DW
+  int pieces, tiles, sl, sx, sw;   // class tiles of the loss, splits of LOSS / DX / DW
 };
+
+// own items per wave / 32: two where the registers hold them (for LOSS their features alone)
+constexpr int ce_nt(int mode, int P, int DP) { return P == 1 && (mode == CE_LOSS || DP == 64) ? 2 : 1; }
+int ce_own(const CePlan& q, int mode) { return 256 * ce_nt(mode, q.P, q.Dp); }
 
 constexpr int64_t kCePieceBytes = 512ll << 20;     // bound on G
 
+// Up to 256 feature columns (fp32's two pieces: 128) the streaming kernels hold the own side in registers; beyond, G in memory
+bool ce_streams(int D, int dtype) { return D <= (dtype == CRESTE_DT_F32 ? 128 : 256); }
+int ce_padded(int D, int dtype) { return ce_streams(D, dtype) ? (D <= 64 ? 64 : D <= 128 ? 128 : 256) : (int)up(D, 64); }
+
 bool ce_direct(const void* x, int64_t ld, int D, int dtype) {
-  return dtype != CRESTE_DT_F32 && D % 64 == 0 && ld % 8 == 0 && ((uintptr_t)x & 15) == 0;
+  return dtype != CRESTE_DT_F32 && D == ce_padded(D, dtype) && ld % 8 == 0 && ld < (1 << 24) && ((uintptr_t)x & 15) == 0;
 }
 
 constexpr int kCeFewRows = 32;
@@ -615,16 +941,28 @@ bool ce_few(const void* x, int64_t ld, int D, int dtype) {
   return D * es % 32 == 0 && ld * es % 16 == 0 && ((uintptr_t)x & 15) == 0;
 }
 
+// splits of the contraction k: the count for which the rounds of workgroups times the length of one (`start`: what its beginning and
+// end cost, in units of k) is least
+int ce_splits(int64_t tiles, int64_t k, int per_round, int start) {
+  int best = 1;
+  int64_t cost = -1;
+  for (int64_t s = 1; s <= 256 && (s == 1 || (k + s - 1) / s >= 128); ++s) {
+    const int64_t c = (tiles * s + per_round - 1) / per_round * (up((k + s - 1) / s, 64) + start);
+    if (cost < 0 || c < cost) { cost = c; best = (int)s; }
+  }
+  return best;
+}
+
 CePlan ce_plan(int64_t N, int64_t V, int D, int dtype, bool packx, bool packw, bool train) {
   CePlan q{};
   q.P = dtype == CRESTE_DT_F32 ? 2 : 1;
   q.dt16 = dtype == CRESTE_DT_BF16 ? CRESTE_DT_BF16 : CRESTE_DT_F16;
   q.es = dtype == CRESTE_DT_F32 ? 4 : 2;
-  q.Dp = (int)up(D, 64);
+  q.stream = ce_streams(D, dtype);
+  q.Dp = ce_padded(D, dtype);
   q.ldq = (int)up(D, 4);
   q.packx = packx;
   q.packw = packw;
-  q.bm = D <= 128 ? 128 : 256;
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 1024); return at; };
   q.amax = take(64);
@@ -632,11 +970,24 @@ CePlan ce_plan(int64_t N, int64_t V, int D, int dtype, bool packx, bool packw, b
   q.wp = packw ? take(V * q.Dp * 2 * q.P) : 0;
   q.tiles = (int)((V + kCeTile - 1) / kCeTile);
   if (!train) {
-    q.part = take((int64_t)q.tiles * N * 8);
+    q.own = ce_own(q, CE_LOSS);
+    q.sl = q.stream ? ce_splits((N + q.own - 1) / q.own, V, 256, 320) : 0;
+    q.part = take((int64_t)(q.sl > q.tiles ? q.sl : q.tiles) * N * 8);
     q.zlab = take(N * 4);
     q.bsum = take((N + 63) / 64 * 8);
+    q.total = o;
+    return q;
+  }
+  q.n64 = up(N, 64);
+  q.row_l2 = take(q.n64 * 4);
+  q.row_lab = take(q.n64 * 4);
+  if (q.stream) {
+    q.own = ce_own(q, CE_DX);
+    q.pieces = 1;
+    q.vc = V;
+    q.sx = ce_splits((N + q.own - 1) / q.own, V, 256, 320);
+    q.sw = ce_splits((V + q.own - 1) / q.own, N, 256, 320);
   } else {
-    q.n64 = up(N, 64);
     const int64_t vall = up(V, kCeTile);
     int64_t vc = kCePieceBytes / (q.n64 * 2 * q.P) / kCeTile * kCeTile;
     vc = vc < kCeTile ? kCeTile : vc > vall ? vall : vc;
@@ -644,49 +995,69 @@ CePlan ce_plan(int64_t N, int64_t V, int D, int dtype, bool packx, bool packw, b
     q.vc = up((vall + q.pieces - 1) / q.pieces, kCeTile);        // pieces of one size
     q.pieces = (int)((vall + q.vc - 1) / q.vc);
     q.g = take(q.n64 * q.vc * 2 * q.P);
-    // splits of the contraction: enough workgroups for the 256 CUs, chunks of at least 512
-    const int64_t mt = (D + q.bm - 1) / q.bm;
-    auto splits = [&](int64_t tiles, int64_t k) {
-      int64_t s = (256 + tiles - 1) / tiles;
-      const int64_t most = (k + 511) / 512;
-      s = s > most ? most : s;
-      return (int)(s < 1 ? 1 : s);
-    };
-    q.sx = splits(mt * ((N + kCeTile - 1) / kCeTile), q.vc);
-    q.sw = splits(mt * (q.vc / kCeTile), q.n64);
-    if (q.sx > 1 || q.pieces > 1) q.dxp = take((int64_t)q.sx * N * q.ldq * 4);
-    if (q.sw > 1) q.dwp = take((int64_t)q.sw * q.vc * q.ldq * 4);
+    const int64_t mt = (D + kCeTile - 1) / kCeTile;
+    q.sx = ce_splits(mt * ((N + kCeTile - 1) / kCeTile), q.vc, 256, 256);
+    q.sw = ce_splits(mt * (q.vc / kCeTile), q.n64, 256, 256);
   }
+  if (q.sx > 1 || q.pieces > 1) q.dxp = take((int64_t)q.sx * N * q.ldq * 4);
+  if (q.sw > 1) q.dwp = take((int64_t)q.sw * q.vc * q.ldq * 4);
   q.total = o;
   return q;
 }
 
-template <int MODE, int DT, int P, int BM>
-int ce_launch(const CeArgs& a, int blocks, hipStream_t s) {
-  constexpr int bytes = 2 * (BM + kCeTile) * 64 * 2;
+using CeBig = CeShape<256, 256, 2, 4, 64, 2>;          // 128 KB of LDS: one workgroup per CU
+
+template <int MODE, int DT, int P, typename S>
+int ce_launch(CeArgs a, int splits, hipStream_t s) {
+  constexpr int bytes = S::NS * (S::BM + S::BN) * S::BK * 2;
   static std::atomic<uint64_t> mask{0};
-  CRESTE_HIP(ensure_dyn_smem((const void*)ce_gemm_kernel<MODE, DT, P, BM>, bytes, mask));
-  ce_gemm_kernel<MODE, DT, P, BM><<<blocks, 512, bytes, s>>>(a);
+  CRESTE_HIP(ensure_dyn_smem((const void*)ce_gemm_kernel<MODE, DT, P, S>, bytes, mask));
+  a.mt = cdiv(a.m, S::BM);
+  if (MODE == CE_GRAD) a.mt = (int)(a.ldg / 2 / S::BM);          // the zeros behind the last class too
+  a.nt = cdiv(a.n, S::BN);
+  const int64_t blocks = (int64_t)a.mt * a.nt * splits;
+  CRESTE_REQUIRE(blocks < (1ll << 31), "linear_ce: too many tiles");
+  ce_gemm_kernel<MODE, DT, P, S><<<(int)blocks, S::NW * 64, bytes, s>>>(a);
   CRESTE_CHECK_LAUNCH("linear_ce gemm");
   return CRESTE_OK;
 }
 
 template <int MODE>
-int ce_dispatch(const CePlan& q, const CeArgs& a, int blocks, hipStream_t s) {
-  const bool narrow = MODE >= CE_DX && q.bm == 128;
-  if (q.P == 2) {
-    if constexpr (MODE >= CE_DX)
-      if (narrow) return ce_launch<MODE, CRESTE_DT_F16, 2, 128>(a, blocks, s);
-    return ce_launch<MODE, CRESTE_DT_F16, 2, 256>(a, blocks, s);
-  }
-  if (q.dt16 == CRESTE_DT_BF16) {
-    if constexpr (MODE >= CE_DX)
-      if (narrow) return ce_launch<MODE, CRESTE_DT_BF16, 1, 128>(a, blocks, s);
-    return ce_launch<MODE, CRESTE_DT_BF16, 1, 256>(a, blocks, s);
-  }
-  if constexpr (MODE >= CE_DX)
-    if (narrow) return ce_launch<MODE, CRESTE_DT_F16, 1, 128>(a, blocks, s);
-  return ce_launch<MODE, CRESTE_DT_F16, 1, 256>(a, blocks, s);
+int ce_gemm(const CePlan& q, const CeArgs& a, int splits, hipStream_t s) {
+  if (q.P == 2) return ce_launch<MODE, CRESTE_DT_F16, 2, CeBig>(a, splits, s);
+  if (q.dt16 == CRESTE_DT_BF16) return ce_launch<MODE, CRESTE_DT_BF16, 1, CeBig>(a, splits, s);
+  return ce_launch<MODE, CRESTE_DT_F16, 1, CeBig>(a, splits, s);
+}
+
+template <int MODE, int DT, int P, int DP>
+int ce_stream_launch(CeArgs a, int splits, hipStream_t s) {
+  constexpr int NT = ce_nt(MODE, P, DP), stages = 3 * CeStream<DP, kCeStage, P>::BYTES, out = MODE == CE_LOSS ? 0 : 8 * 32 * 512;
+  constexpr int bytes = stages > out ? stages : out;
+  static std::atomic<uint64_t> mask{0};
+  CRESTE_HIP(ensure_dyn_smem((const void*)ce_stream_kernel<MODE, DT, P, DP, NT>, bytes, mask));
+  a.nt = cdiv(a.n, 256 * NT);
+  a.k1 = a.m;
+  a.ksplit = (int)up(cdiv(a.m, splits), kCeStage);
+  const int64_t blocks = (int64_t)a.nt * splits;
+  CRESTE_REQUIRE(blocks < (1ll << 31), "linear_ce: too many tiles");
+  ce_stream_kernel<MODE, DT, P, DP, NT><<<(int)blocks, 512, bytes, s>>>(a);
+  CRESTE_CHECK_LAUNCH("linear_ce stream");
+  return CRESTE_OK;
+}
+
+template <int MODE, int DT, int P>
+int ce_stream_typed(const CePlan& q, const CeArgs& a, int splits, hipStream_t s) {
+  if (q.Dp == 64) return ce_stream_launch<MODE, DT, P, 64>(a, splits, s);
+  if constexpr (P == 1)
+    if (q.Dp == 256) return ce_stream_launch<MODE, DT, P, 256>(a, splits, s);
+  return ce_stream_launch<MODE, DT, P, 128>(a, splits, s);
+}
+
+template <int MODE>
+int ce_stream(const CePlan& q, const CeArgs& a, int splits, hipStream_t s) {
+  if (q.P == 2) return ce_stream_typed<MODE, CRESTE_DT_F16, 2>(q, a, splits, s);
+  if (q.dt16 == CRESTE_DT_BF16) return ce_stream_typed<MODE, CRESTE_DT_BF16, 1>(q, a, splits, s);
+  return ce_stream_typed<MODE, CRESTE_DT_F16, 1>(q, a, splits, s);
 }
 
 int ce_grid(int64_t items) { return (int)(items < 1 ? 1 : items > 2048 ? 2048 : items); }
@@ -772,24 +1143,22 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
   a.a = W.p; a.lda = W.ld; a.pa = W.piece; a.ra = V;
   a.b = X.p; a.ldb = X.ld; a.pb = X.piece; a.rb = N;
   a.m = (int)V; a.n = (int)N;
-  a.mt = q.tiles; a.nt = cdiv(N, kCeTile);
   a.k1 = q.Dp;
   a.labels = labels; a.ignore = ignore_index; a.classes = (int)V;
   a.inv_tau = 1.f / temperature;
   a.amax = q.P == 2 ? (const float*)(wk + q.amax) : nullptr;
   a.part = (float2*)(wk + q.part); a.zlab = (float*)(wk + q.zlab);
-  CRESTE_REQUIRE((int64_t)a.mt * a.nt < (1ll << 31), "linear_ce: too many tiles");
   if (few) {
     if (dtype == CRESTE_DT_F32) ce_few_kernel<CRESTE_DT_F32><<<q.tiles, 256, 0, s>>>(a, D);
     else if (dtype == CRESTE_DT_BF16) ce_few_kernel<CRESTE_DT_BF16><<<q.tiles, 256, 0, s>>>(a, D);
     else ce_few_kernel<CRESTE_DT_F16><<<q.tiles, 256, 0, s>>>(a, D);
     CRESTE_CHECK_LAUNCH("linear_ce few rows");
   } else {
-    const int rg = ce_dispatch<CE_LOSS>(q, a, a.mt * a.nt, s);
+    const int rg = q.stream ? ce_stream<CE_LOSS>(q, a, q.sl, s) : ce_gemm<CE_LOSS>(q, a, 1, s);
     if (rg) return rg;
   }
   const int nb = cdiv(N, 64);
-  ce_join_kernel<<<nb, 1024, 0, s>>>(a.part, q.tiles, (int)N, a.zlab, labels, ignore_index, (int)V, nll, lse2, (float2*)(wk + q.bsum),
+  ce_join_kernel<<<nb, 1024, 0, s>>>(a.part, q.stream && !few ? q.sl : q.tiles, (int)N, a.zlab, labels, ignore_index, (int)V, nll, lse2, (float2*)(wk + q.bsum),
                                        mean, loss, stat);
   if (nb > 1) ce_final_kernel<<<1, 256, 0, s>>>((const float2*)(wk + q.bsum), nb, mean, loss, stat);
   CRESTE_CHECK_LAUNCH("linear_ce join");
@@ -811,60 +1180,78 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
   const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, dtype, wk, &X, &W, s);
   if (rc) return rc;
   CeArgs c{};                                       // what every product shares
-  c.labels = labels; c.ignore = ignore_index; c.classes = (int)V;
+  c.classes = (int)V;
   c.inv_tau = 1.f / temperature;
   c.amax = q.P == 2 ? (const float*)(wk + q.amax) : nullptr;
-  c.lse2 = lse2; c.stat = stat; c.gl = g_loss; c.mean = mean;
-  c.g = wk + q.g; c.ldg = q.vc * 2; c.pg = q.n64 * q.vc * 2; c.n64 = (int)q.n64;
+  c.stat = stat; c.gl = g_loss; c.mean = mean;
   c.gscale = q.dt16 == CRESTE_DT_F16 ? kCeF16Scale : 1.f;
+  c.row_l2 = (const float*)(wk + q.row_l2); c.row_lab = (const int*)(wk + q.row_lab);
+  c.n64 = (int)q.n64;
   c.out_dt = dtype;
-  CeArgs dx = c;
-  for (int piece = 0; piece < q.pieces; ++piece) {
-    const int64_t v0 = piece * q.vc, nv = V - v0 < q.vc ? V - v0 : q.vc;
-    CeArgs a = c;                                   // G of the piece
-    a.a = W.p + v0 * W.ld; a.lda = W.ld; a.pa = W.piece; a.ra = nv;
-    a.b = X.p; a.ldb = X.ld; a.pb = X.piece; a.rb = N;
-    a.m = (int)nv; a.n = (int)N; a.class0 = (int)v0;
-    a.mt = (int)(q.vc / kCeTile); a.nt = cdiv(N, kCeTile);
-    a.k1 = q.Dp;
-    int rg = ce_dispatch<CE_GRAD>(q, a, a.mt * a.nt, s);
-    if (rg) return rg;
+  c.ldo = c.m_out = D;
+  c.ldp = q.ldq;
+  ce_rows_kernel<<<cdiv(q.n64, 256), 256, 0, s>>>(lse2, labels, (int)N, (int)q.n64, ignore_index, (int)V, log2f(c.gscale),
+                                                  (float*)(wk + q.row_l2), (int*)(wk + q.row_lab));
+  CRESTE_CHECK_LAUNCH("linear_ce rows");
+  auto reduce = [&](const CeArgs& a, int splits) {
+    ce_reduce_kernel<<<ce_grid((int64_t)a.n * q.ldq / 1024 + 1), 256, 0, s>>>(a, splits);
+    CRESTE_CHECK_LAUNCH("linear_ce reduce");
+    return CRESTE_OK;
+  };
+  CeArgs dx = c, dw = c;
+  dx.n = (int)N; dx.out = gx; dx.which = 1; dx.psplit = N * q.ldq;
+  if (q.dxp) dx.partial = (float*)(wk + q.dxp);
+  dw.which = 0; dw.psplit = q.vc * q.ldq;
+  if (q.dwp) dw.partial = (float*)(wk + q.dwp);
+  if (q.stream) {
     if (gx) {
-      dx = c;
-      dx.a = W.p + v0 * W.ld; dx.lda = W.ld; dx.pa = W.piece; dx.ra = nv; dx.ca = q.Dp * 2;
-      dx.b = c.g; dx.ldb = c.ldg; dx.pb = c.pg; dx.rb = q.n64;
-      dx.m = D; dx.n = (int)N;
-      dx.mt = cdiv(D, q.bm); dx.nt = cdiv(N, kCeTile);
-      dx.k1 = (int)up(nv, 64);
-      dx.ksplit = q.sx > 1 ? (int)up(cdiv(q.vc, q.sx), 64) : 0;
-      if (q.sx > 1 || q.pieces > 1) dx.partial = (float*)(wk + q.dxp);
-      dx.ldp = q.ldq; dx.psplit = N * q.ldq; dx.accumulate = piece > 0;
-      dx.out = gx; dx.ldo = D; dx.which = 1;
-      rg = ce_dispatch<CE_DX>(q, dx, dx.mt * dx.nt * q.sx, s);
+      dx.a = W.p; dx.lda = W.ld; dx.pa = W.piece; dx.ra = V; dx.m = (int)V;
+      dx.b = X.p; dx.ldb = X.ld; dx.pb = X.piece;
+      const int rg = ce_stream<CE_DX>(q, dx, q.sx, s);
       if (rg) return rg;
     }
     if (gw) {
-      CeArgs b = c;
-      b.a = X.p; b.lda = X.ld; b.pa = X.piece; b.ra = N; b.ca = q.Dp * 2;
-      b.b = c.g; b.ldb = c.ldg; b.pb = c.pg; b.rb = q.n64; b.cb = (int)(q.vc * 2);
-      b.m = D; b.n = (int)nv;
-      b.mt = cdiv(D, q.bm); b.nt = cdiv(nv, kCeTile);
-      b.k1 = (int)q.n64;
-      b.ksplit = q.sw > 1 ? (int)up(cdiv(q.n64, q.sw), 64) : 0;
-      if (q.sw > 1) b.partial = (float*)(wk + q.dwp);
-      b.ldp = q.ldq; b.psplit = q.vc * q.ldq;
-      b.out = (char*)gw + v0 * D * q.es; b.ldo = D; b.which = 0;
-      rg = ce_dispatch<CE_DW>(q, b, b.mt * b.nt * q.sw, s);
+      dw.a = X.p; dw.lda = X.ld; dw.pa = X.piece; dw.ra = N; dw.m = (int)N;
+      dw.b = W.p; dw.ldb = W.ld; dw.pb = W.piece; dw.n = (int)V;
+      dw.out = gw;
+      const int rg = ce_stream<CE_DW>(q, dw, q.sw, s);
       if (rg) return rg;
-      if (b.partial) {
-        ce_reduce_kernel<<<ce_grid((int64_t)b.n * q.ldq / 1024 + 1), 256, 0, s>>>(b, q.sw);
-        CRESTE_CHECK_LAUNCH("linear_ce reduce");
+      if (dw.partial && reduce(dw, q.sw)) return CRESTE_ERR_HIP;
+    }
+  } else {
+    for (int piece = 0; piece < q.pieces; ++piece) {
+      const int64_t v0 = piece * q.vc, nv = V - v0 < q.vc ? V - v0 : q.vc;
+      CeArgs a = c;                                 // G of the piece
+      a.g = wk + q.g; a.ldg = q.vc * 2; a.pg = q.n64 * q.vc * 2;
+      a.a = W.p + v0 * W.ld; a.lda = W.ld; a.pa = W.piece; a.ra = nv;
+      a.b = X.p; a.ldb = X.ld; a.pb = X.piece; a.rb = N;
+      a.m = (int)nv; a.n = (int)N; a.class0 = (int)v0;
+      a.k1 = q.Dp;
+      int rg = ce_gemm<CE_GRAD>(q, a, 1, s);
+      if (rg) return rg;
+      if (gx) {
+        dx.a = a.a; dx.lda = W.ld; dx.pa = W.piece; dx.ra = nv; dx.ca = q.Dp * 2;
+        dx.b = a.g; dx.ldb = a.ldg; dx.pb = a.pg; dx.rb = q.n64;
+        dx.m = D;
+        dx.k1 = (int)up(nv, 64);
+        dx.ksplit = q.sx > 1 ? (int)up(cdiv(q.vc, q.sx), 64) : 0;
+        dx.accumulate = piece > 0;
+        rg = ce_gemm<CE_DX>(q, dx, q.sx, s);
+        if (rg) return rg;
+      }
+      if (gw) {
+        dw.a = X.p; dw.lda = X.ld; dw.pa = X.piece; dw.ra = N; dw.ca = q.Dp * 2;
+        dw.b = a.g; dw.ldb = a.ldg; dw.pb = a.pg; dw.rb = q.n64; dw.cb = (int)(q.vc * 2);
+        dw.m = D; dw.n = (int)nv;
+        dw.k1 = (int)q.n64;
+        dw.ksplit = q.sw > 1 ? (int)up(cdiv(q.n64, q.sw), 64) : 0;
+        dw.out = (char*)gw + v0 * D * q.es;
+        rg = ce_gemm<CE_DW>(q, dw, q.sw, s);
+        if (rg) return rg;
+        if (dw.partial && reduce(dw, q.sw)) return CRESTE_ERR_HIP;
       }
     }
   }
-  if (gx && dx.partial) {
-    ce_reduce_kernel<<<ce_grid(N * q.ldq / 1024 + 1), 256, 0, s>>>(dx, q.sx);
-    CRESTE_CHECK_LAUNCH("linear_ce reduce");
-  }
+  if (gx && dx.partial && reduce(dx, q.sx)) return CRESTE_ERR_HIP;
   return CRESTE_OK;
 }
