@@ -29,7 +29,7 @@ typedef __bf16 ceb8 __attribute__((ext_vector_type(8)));
 
 constexpr float kCeLog2e = 1.44269504088896341f, kCeLn2 = 0.693147180559945309f;
 constexpr int kCeTile = 256;                 // classes per LOSS / GRAD tile, rows (LOSS, GRAD, DX) or classes (DW) per tile
-constexpr float kCeF16Scale = 16384.f;       // G enters as G * 2^14 where it is stored in fp16
+constexpr float kCeF16Log2 = 14.f;           // G enters as G * 2^14 where it is fp16
 
 enum { CE_LOSS, CE_GRAD, CE_DX, CE_DW };
 
@@ -51,6 +51,7 @@ struct CeArgs {
   const float* amax;                // [2] max|x|, max|w| (two-piece operands) or null
   float2* part;                     // LOSS: [class tile][n] (max, sum) in log2 units
   float* zlab;                      // LOSS: [n] label logit, log2 units
+  unsigned* done;                   // LOSS: the joining kernel's counter, cleared here
   const float* row_l2;              // GRAD, DX, DW: [rows64] log-sum-exp minus log2 of G's scale, infinity where a row does not count
   const int* row_lab;               // [rows64] label, -1 where none applies
   char* g;                          // GRAD: [n64][ldg] elements, pieces pg bytes apart
@@ -235,6 +236,8 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
   extern __shared__ __align__(1024) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, lh = lane >> 5;
   const int wm = wave / S::WN, wn = wave % S::WN;
+  if constexpr (MODE == CE_LOSS)
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;
   int t = xcd_remap(blockIdx.x, gridDim.x);
   const int tm = t % p.mt;
   t /= p.mt;
@@ -465,6 +468,20 @@ struct CeStream {
 };
 
 constexpr int kCeStage = 64;                 // others per stage
+constexpr int kAhead = 4;                    // (8192 x 65536 x 256 bf16 training step: 1206 us with the compiler's own order, 1189 with 4)
+
+// order of the region in front: kAhead LDS reads, then matrix instructions with the remaining reads spread between them
+template <int READS, int MFMAS>
+__device__ __forceinline__ void ce_interleave() {
+  constexpr int A = kAhead < READS ? kAhead : READS, REST = READS - A;
+  __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
+#pragma unroll
+  for (int i = 0; i < MFMAS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+#pragma unroll
+    for (int r = i * REST / MFMAS; r < (i + 1) * REST / MFMAS; ++r) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+}
 
 // a = the streamed side (p.m items), b = the own side (p.n items), NT x 32 own items per wave
 template <int MODE, int DT, int P, int DP, int NT>
@@ -473,6 +490,8 @@ __global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
   constexpr int NS = 3, KS = DP / 16, kDma = P * L::INSTR / 8 + (MODE == CE_DW);
   extern __shared__ __align__(1024) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, lh = lane >> 5;
+  if constexpr (MODE == CE_LOSS)
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;
   int t = xcd_remap(blockIdx.x, gridDim.x);
   const int tn = t % p.nt, split = t / p.nt;
   const int own0 = tn * (256 * NT) + wave * (32 * NT);
@@ -553,6 +572,7 @@ __global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
           z[j] = ce_mfma<DT>(a[0], x[0][j][kk], z[j]);
         }
       }
+      ce_interleave<KS * P, NT * (P == 2 ? 3 : 1) * KS>();
       __builtin_amdgcn_sched_barrier(0);                // (the phases' operands do not fit the registers side by side)
       const bool edge = o0 + 32 > p.m;                  // others behind the last one
       ces8 g[P][NT][2];
@@ -626,6 +646,8 @@ __global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
               acc[d][j] = ce_mfma<DT>(a[0], g[0][j][k2], acc[d][j]);
             }
           }
+        ce_interleave<AT * 4 * P, AN * (P == 2 ? 3 : 1) * AT * 2>();
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     cur = cur + 1 == NS ? 0 : cur + 1;
@@ -658,6 +680,7 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeArgs p, int D) {
   constexpr int EB = DT == CRESTE_DT_F32 ? 4 : 2, STEP = 32 / EB;      // elements both halves take per load
   typedef int iv4 __attribute__((ext_vector_type(4)));
   __shared__ float2 sh[4][32];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, lh = lane >> 5;
   const int m0 = blockIdx.x * kCeTile + wave * 64;
   const int row = li < p.n ? li : p.n - 1;
@@ -745,58 +768,85 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeArgs p, int D) {
 }
 
 // ---------------------------------------------------------------------------------------------------- small kernels
-__global__ void ce_zero_kernel(float* p, int n) {
-  if ((int)threadIdx.x < n) p[threadIdx.x] = 0.f;
-}
+// both operands at once: blocks below `split` take the first, the others the second
+struct CeSide { const void* x; int64_t rows, ld; short* out; int64_t piece; };
 
-// max |x| of a [rows][cols] fp32 matrix with row stride ld
-__global__ __launch_bounds__(256) void ce_amax_kernel(const float* __restrict__ x, int64_t rows, int cols, int64_t ld,
-                                                      float* __restrict__ amax) {
-  __shared__ float scratch[4];
+// Each 16 lanes take whole rows, 4 columns a lane and step (no division by the row length).
+// amax: per block max |x| of its operand -> bmax[block]
+__global__ __launch_bounds__(256) void ce_amax_kernel(CeSide u, CeSide v, int cols, int split, float* __restrict__ bmax) {
+  __shared__ float sh[4];
+  const bool second = (int)blockIdx.x >= split;
+  const CeSide s = second ? v : u;
+  const int blk = second ? blockIdx.x - split : blockIdx.x, nb = second ? gridDim.x - split : split;
+  const int c0 = (threadIdx.x & 15) * 4;
   float m = 0.f;
-  const int64_t total = rows * cols;
-  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-    const int64_t r = i / cols;
-    m = fmaxf(m, fabsf(x[r * ld + (i - r * cols)]));
-  }
-  block_amax_update(m, amax, scratch);
-}
-
-// 16-bit copy of the features with rows of cp (a multiple of 64) elements, zero behind the last column.  fp32: two pieces
-template <typename T>
-__global__ __launch_bounds__(256) void ce_pack_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ld, int cp,
-                                                      const float* __restrict__ amax, short* __restrict__ out, int64_t piece) {
-  float inv = 1.f, s = 1.f;
-  if constexpr (sizeof(T) == 4) s = f16_operand_scale(*amax, &inv);
-  const int64_t total = rows * (cp / 4);
-  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-    const int64_t r = i / (cp / 4);
-    const int c = (int)(i - r * (cp / 4)) * 4;
-    ces4 hi, lo;
+  for (int64_t r = (int64_t)blk * 16 + (threadIdx.x >> 4); r < s.rows; r += (int64_t)nb * 16) {
+    const float* x = (const float*)s.x + r * s.ld;
+    for (int c = c0; c < cols; c += 64)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const T v = c + e < cols ? x[r * ld + c + e] : (T)0;
-      if constexpr (sizeof(T) == 4) {
-        const float a = v * s;
-        const short h = ce_cvt<CRESTE_DT_F16>(a);
-        hi[e] = h;
-        lo[e] = ce_cvt<CRESTE_DT_F16>(a - (float)__builtin_bit_cast(_Float16, h));
-      } else {
-        hi[e] = (short)v;
+      for (int e = 0; e < 4; ++e)
+        if (c + e < cols) m = fmaxf(m, fabsf(x[c + e]));
+  }
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) bmax[blockIdx.x] = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+}
+
+// 16-bit copy of the features with rows of cp (a multiple of 64) elements, zero behind the last column.  fp32: two pieces under
+// the power of two of the operand's max |x| (from the na[0] + na[1] block maxima; left in amax[0 / 1])
+template <typename T>
+__global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int cols, int cp, int split, const float* __restrict__ bmax,
+                                                      int na0, int na1, float* __restrict__ amax) {
+  const bool second = (int)blockIdx.x >= split;
+  const CeSide s = second ? v : u;
+  const int blk = second ? blockIdx.x - split : blockIdx.x, nb = second ? gridDim.x - split : split;
+  float scale = 1.f;
+  if constexpr (sizeof(T) == 4) {
+    __shared__ float sh[4];
+    float m = 0.f;
+    for (int i = threadIdx.x; i < (second ? na1 : na0); i += 256) m = fmaxf(m, bmax[(second ? na0 : 0) + i]);
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+    if (blk == 0 && threadIdx.x == 0) amax[second] = m;
+    float inv;
+    scale = f16_operand_scale(m, &inv);
+  }
+  const int c0 = (threadIdx.x & 15) * 4;
+  for (int64_t r = (int64_t)blk * 16 + (threadIdx.x >> 4); r < s.rows; r += (int64_t)nb * 16) {
+    const T* x = (const T*)s.x + r * s.ld;
+    for (int c = c0; c < cp; c += 64) {
+      ces4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const T v = c + e < cols ? x[c + e] : (T)0;
+        if constexpr (sizeof(T) == 4) {
+          const float a = v * scale;
+          const short h = ce_cvt<CRESTE_DT_F16>(a);       // (a scalar: bit casts of vector elements are miscompiled)
+          hi[e] = h;
+          lo[e] = ce_cvt<CRESTE_DT_F16>(a - (float)__builtin_bit_cast(_Float16, h));
+        } else {
+          hi[e] = (short)v;
+        }
       }
+      *reinterpret_cast<ces4*>(s.out + r * cp + c) = hi;
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<ces4*>(s.out + s.piece + r * cp + c) = lo;
     }
-    *reinterpret_cast<ces4*>(out + r * cp + c) = hi;
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<ces4*>(out + piece + r * cp + c) = lo;
   }
 }
 
-// per row: join the class tiles' (max, sum).  64 rows x 16 slices of the tiles per block; per block the sums of nll and count, or
-// the loss itself when there is one block
+// per row: join the class tiles' (max, sum); 64 rows x 16 slices of the tiles per block.  Leaves nll, what the gradient kernels ask of a
+// row (padded to whole tiles: rows that do not count get an infinite log-sum-exp, hence G = 0, a label that names no class a NaN), and,
+// from the last block to finish, the loss: sums of the blocks' sums in their order, so the result does not depend on which that was
 __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ part, int tiles, int n, const float* __restrict__ zlab,
                                                        const int64_t* __restrict__ labels, int64_t ignore, int classes,
-                                                       float* __restrict__ nll, float* __restrict__ lse2, float2* __restrict__ bsum,
+                                                       float log2_scale, float* __restrict__ nll, float* __restrict__ row_l2,
+                                                       int* __restrict__ row_lab, uint64_t* __restrict__ bsum, unsigned* __restrict__ done,
                                                        int mean, float* __restrict__ loss, float* __restrict__ stat) {
   __shared__ float2 sh[16][64];
+  __shared__ bool last;
   const int li = threadIdx.x & 63, sl = threadIdx.x >> 6;
   const int row = blockIdx.x * 64 + li;
   float mx = -3.0e38f, sum = 0.f;
@@ -810,98 +860,89 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
     }
   sh[sl][li] = make_float2(mx, sum);
   __syncthreads();
-  if (sl) return;
-  for (int s = 1; s < 16; ++s) {
-    const float2 v = sh[s][li];
-    const float m = fmaxf(mx, v.x);
-    sum = sum * __builtin_amdgcn_exp2f(mx - m) + v.y * __builtin_amdgcn_exp2f(v.x - m);
-    mx = m;
-  }
-  float l = 0.f, c = 0.f;
-  if (row < n) {
+  if (sl == 0) {
+    for (int s = 1; s < 16; ++s) {
+      const float2 v = sh[s][li];
+      const float m = fmaxf(mx, v.x);
+      sum = sum * __builtin_amdgcn_exp2f(mx - m) + v.y * __builtin_amdgcn_exp2f(v.x - m);
+      mx = m;
+    }
+    float l = 0.f, c = 0.f;
+    const int64_t y = row < n ? labels[row] : ignore;
+    const bool on = row < n && y != ignore, ok = y >= 0 && y < classes;
     const float z = mx + __builtin_amdgcn_logf(sum);
-    const int64_t y = labels[row];
-    const bool on = y != ignore;
-    lse2[row] = z;
     if (on) {
-      l = y >= 0 && y < classes ? (z - zlab[row]) * kCeLn2 : __builtin_nanf("");
+      l = ok ? (z - zlab[row]) * kCeLn2 : __builtin_nanf("");
       c = 1.f;
     }
-    nll[row] = l;
-  }
+    if (row < n) nll[row] = l;
+    row_l2[row] = !on ? INFINITY : ok ? z - log2_scale : __builtin_nanf("");
+    row_lab[row] = on && ok ? (int)y : -1;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    l += __shfl_xor(l, o, 64);
-    c += __shfl_xor(c, o, 64);
+    for (int o = 32; o > 0; o >>= 1) {
+      l += __shfl_xor(l, o, 64);
+      c += __shfl_xor(c, o, 64);
+    }
+    if (li == 0) {                                      // one word, written through; the count when it has arrived
+      __hip_atomic_store(bsum + blockIdx.x, (uint64_t)__float_as_uint(c) << 32 | __float_as_uint(l), __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      last = atomicAdd(done, 1u) == gridDim.x - 1;
+    }
   }
-  if (li) return;
-  if (gridDim.x > 1) {
-    bsum[blockIdx.x] = make_float2(l, c);
-  } else {
-    stat[0] = l;
-    stat[1] = c;
-    *loss = mean ? l / fmaxf(c, 1.f) : l;
-  }
-}
-
-// loss from the blocks' sums (fixed order), stat = {sum nll, count}
-__global__ __launch_bounds__(256) void ce_final_kernel(const float2* __restrict__ bsum, int nb, int mean, float* __restrict__ loss,
-                                                       float* __restrict__ stat) {
-  __shared__ double sl[256], sc[256];
-  double l = 0., c = 0.;
-  for (int i = threadIdx.x; i < nb; i += 256) {
-    l += bsum[i].x;
-    c += bsum[i].y;
-  }
-  sl[threadIdx.x] = l;
-  sc[threadIdx.x] = c;
   __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
+  if (!last) return;
+  __shared__ double sl_[1024], sc_[1024];
+  double l = 0., c = 0.;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += 1024) {
+    const uint64_t v = __hip_atomic_load(bsum + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    l += __uint_as_float((unsigned)v);
+    c += __uint_as_float((unsigned)(v >> 32));
+  }
+  sl_[threadIdx.x] = l;
+  sc_[threadIdx.x] = c;
+  __syncthreads();
+  for (int o = 512; o > 0; o >>= 1) {
     if ((int)threadIdx.x < o) {
-      sl[threadIdx.x] += sl[threadIdx.x + o];
-      sc[threadIdx.x] += sc[threadIdx.x + o];
+      sl_[threadIdx.x] += sl_[threadIdx.x + o];
+      sc_[threadIdx.x] += sc_[threadIdx.x + o];
     }
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    stat[0] = (float)sl[0];
-    stat[1] = (float)sc[0];
-    *loss = (float)(mean ? sl[0] / fmax(sc[0], 1.) : sl[0]);
+    stat[0] = (float)sl_[0];
+    stat[1] = (float)sc_[0];
+    *loss = (float)(mean ? sl_[0] / fmax(sc_[0], 1.) : sl_[0]);
   }
 }
 
-// out[n][m] = scale * sum over splits of partial[split][n][ldp]
-__global__ __launch_bounds__(256) void ce_reduce_kernel(CeArgs p, int splits) {
+// out[n][m] = scale * sum over splits of partial[split][n][ldp], for up to two outputs (blocks below `split` take the first)
+__global__ __launch_bounds__(256) void ce_reduce_kernel(CeArgs u, int su, CeArgs v, int sv, int split) {
+  const bool second = (int)blockIdx.x >= split;
+  const CeArgs& p = second ? v : u;
+  const int splits = second ? sv : su, blk = second ? blockIdx.x - split : blockIdx.x, nb = second ? gridDim.x - split : split;
   const float fs = ce_out_scale(p);
   const int64_t total = (int64_t)p.n * p.ldp;
-  for (int64_t i = (blockIdx.x * 256LL + threadIdx.x) * 4; i < total; i += gridDim.x * 1024LL) {
-    cef4 v = *reinterpret_cast<const cef4*>(p.partial + i);
-    for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const cef4*>(p.partial + s * p.psplit + i);
-    v *= fs;
-    const int64_t row = i / p.ldp;
-    const int d = (int)(i - row * p.ldp);
+  const int ldp = (int)p.ldp;
+  int64_t i = (blk * 256LL + threadIdx.x) * 4, row = i / ldp;
+  int d = (int)(i - row * ldp);
+  const int64_t step = nb * 1024LL, srow = step / ldp;
+  const int sd = (int)(step - srow * ldp);
+  for (; i < total; i += step, row += srow, d += sd) {
+    if (d >= ldp) { d -= ldp; ++row; }
+    cef4 a = *reinterpret_cast<const cef4*>(p.partial + i);
+#pragma unroll 8
+    for (int s = 1; s < splits; ++s) a += *reinterpret_cast<const cef4*>(p.partial + s * p.psplit + i);
+    a *= fs;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (d + e >= p.m_out) continue;
       const int64_t o = row * p.ldo + d + e;
-      if (p.out_dt == CRESTE_DT_F32) ((float*)p.out)[o] = v[e];
-      else if (p.out_dt == CRESTE_DT_BF16) ((short*)p.out)[o] = ce_cvt<CRESTE_DT_BF16>(v[e]);
-      else ((short*)p.out)[o] = ce_cvt<CRESTE_DT_F16>(v[e]);
+      if (p.out_dt == CRESTE_DT_F32) ((float*)p.out)[o] = a[e];
+      else if (p.out_dt == CRESTE_DT_BF16) ((short*)p.out)[o] = ce_cvt<CRESTE_DT_BF16>(a[e]);
+      else ((short*)p.out)[o] = ce_cvt<CRESTE_DT_F16>(a[e]);
     }
   }
-}
-
-// what the gradient kernels ask of a row, padded to whole tiles: rows that do not count get an infinite log-sum-exp (G = 0), a label
-// that names no class a NaN (as nll has)
-__global__ __launch_bounds__(256) void ce_rows_kernel(const float* __restrict__ lse2, const int64_t* __restrict__ labels, int n, int n64,
-                                                      int64_t ignore, int classes, float log2_scale, float* __restrict__ l2,
-                                                      int* __restrict__ lab) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= n64) return;
-  const int64_t y = i < n ? labels[i] : ignore;
-  const bool on = i < n && y != ignore, ok = y >= 0 && y < classes;
-  l2[i] = !on ? INFINITY : ok ? lse2[i] - log2_scale : __builtin_nanf("");
-  lab[i] = on && ok ? (int)y : -1;
 }
 
 // --------------------------------------------------------------------------------------------------------- host side
@@ -914,16 +955,20 @@ int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 struct CePlan {
   int P, dt16, es, Dp, ldq, own;   // own: items a streaming workgroup holds
   bool packx, packw, stream;
-  int64_t amax, xp, wp, part, zlab, bsum, row_l2, row_lab, g, dxp, dwp, total;
-  int64_t vc, n64;                 // classes per piece, rows of G
+  int64_t amax, xp, wp, part, zlab, bsum, done, g, dxp, dwp, total;
+  int64_t vc, n64, ldg;            // classes per piece, rows of G, bytes between them
   int pieces, tiles, sl, sx, sw;   // class tiles of the loss, splits of LOSS / DX / DW
 };
 
 // own items per wave / 32: two where the registers hold them (for LOSS their features alone)
 constexpr int ce_nt(int mode, int P, int DP) { return P == 1 && (mode == CE_LOSS || DP == 64) ? 2 : 1; }
+float ce_gscale_log2(const CePlan& q) { return q.dt16 == CRESTE_DT_F16 ? kCeF16Log2 : 0.f; }
 int ce_own(const CePlan& q, int mode) { return 256 * ce_nt(mode, q.P, q.Dp); }
 
-constexpr int64_t kCePieceBytes = 512ll << 20;     // bound on G
+constexpr int kCeMaxima = 512;                     // blocks that look for an operand's largest magnitude
+// A piece of G: 128 MiB, which the memory-side cache still holds when DX and DW read it, but not under 16384 classes (shorter
+// contractions and a partial sum of dx per piece cost more than the cache gives), and never over 512 MiB
+constexpr int64_t kCePieceSmall = 128ll << 20, kCePieceClasses = 16384, kCePieceBytes = 512ll << 20;
 
 // Up to 256 feature columns (fp32's two pieces: 128) the streaming kernels hold the own side in registers; beyond, G in memory
 bool ce_streams(int D, int dtype) { return D <= (dtype == CRESTE_DT_F32 ? 128 : 256); }
@@ -941,14 +986,18 @@ bool ce_few(const void* x, int64_t ld, int D, int dtype) {
   return D * es % 32 == 0 && ld * es % 16 == 0 && ((uintptr_t)x & 15) == 0;
 }
 
-// splits of the contraction k: the count for which the rounds of workgroups times the length of one (`start`: what its beginning and
-// end cost, in units of k) is least
-int ce_splits(int64_t tiles, int64_t k, int per_round, int start) {
+// splits of the contraction k, of those that fill one to eight rounds of workgroups: least rounds times the length of one (`start`: what its
+// beginning and end cost, in units of k)
+int ce_splits(int64_t tiles, int64_t k, int start) {
   int best = 1;
-  int64_t cost = -1;
-  for (int64_t s = 1; s <= 256 && (s == 1 || (k + s - 1) / s >= 128); ++s) {
-    const int64_t c = (tiles * s + per_round - 1) / per_round * (up((k + s - 1) / s, 64) + start);
-    if (cost < 0 || c < cost) { cost = c; best = (int)s; }
+  int64_t cost = (tiles + 255) / 256 * (k + start);
+  for (int r = 1; r <= 8; ++r) {
+    int64_t s = 256 * r / tiles;
+    const int64_t most = (k + 127) / 128;
+    s = s > most ? most : s;
+    if (s < 2) continue;
+    const int64_t c = (tiles * s + 255) / 256 * (up((k + s - 1) / s, 64) + start);
+    if (c < cost) { cost = c; best = (int)s; }
   }
   return best;
 }
@@ -965,39 +1014,42 @@ CePlan ce_plan(int64_t N, int64_t V, int D, int dtype, bool packx, bool packw, b
   q.packw = packw;
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 1024); return at; };
-  q.amax = take(64);
+  q.amax = take(64 + 2 * kCeMaxima * 4);           // the two maxima, the blocks' in front of them
   q.xp = packx ? take(N * q.Dp * 2 * q.P) : 0;
   q.wp = packw ? take(V * q.Dp * 2 * q.P) : 0;
   q.tiles = (int)((V + kCeTile - 1) / kCeTile);
   if (!train) {
     q.own = ce_own(q, CE_LOSS);
-    q.sl = q.stream ? ce_splits((N + q.own - 1) / q.own, V, 256, 320) : 0;
+    q.sl = q.stream ? ce_splits((N + q.own - 1) / q.own, V, 320) : 0;
     q.part = take((int64_t)(q.sl > q.tiles ? q.sl : q.tiles) * N * 8);
     q.zlab = take(N * 4);
     q.bsum = take((N + 63) / 64 * 8);
+    q.done = take(4);
     q.total = o;
     return q;
   }
   q.n64 = up(N, 64);
-  q.row_l2 = take(q.n64 * 4);
-  q.row_lab = take(q.n64 * 4);
   if (q.stream) {
     q.own = ce_own(q, CE_DX);
     q.pieces = 1;
     q.vc = V;
-    q.sx = ce_splits((N + q.own - 1) / q.own, V, 256, 320);
-    q.sw = ce_splits((V + q.own - 1) / q.own, N, 256, 320);
+    q.sx = ce_splits((N + q.own - 1) / q.own, V, 320);
+    q.sw = ce_splits((V + q.own - 1) / q.own, N, 320);
   } else {
     const int64_t vall = up(V, kCeTile);
-    int64_t vc = kCePieceBytes / (q.n64 * 2 * q.P) / kCeTile * kCeTile;
+    const int64_t col = q.n64 * 2 * q.P;                         // bytes of a class's column of G
+    int64_t vc = kCePieceSmall / col > kCePieceClasses ? kCePieceSmall / col : kCePieceClasses;
+    if (vc * col > kCePieceBytes) vc = kCePieceBytes / col;
+    vc = vc / kCeTile * kCeTile;
     vc = vc < kCeTile ? kCeTile : vc > vall ? vall : vc;
     q.pieces = (int)((vall + vc - 1) / vc);
     q.vc = up((vall + q.pieces - 1) / q.pieces, kCeTile);        // pieces of one size
     q.pieces = (int)((vall + q.vc - 1) / q.vc);
-    q.g = take(q.n64 * q.vc * 2 * q.P);
+    q.ldg = q.vc * 2 + 256;          // (rows a power of two apart would meet in the same memory channels)
+    q.g = take(q.n64 * q.ldg * q.P);
     const int64_t mt = (D + kCeTile - 1) / kCeTile;
-    q.sx = ce_splits(mt * ((N + kCeTile - 1) / kCeTile), q.vc, 256, 256);
-    q.sw = ce_splits(mt * (q.vc / kCeTile), q.n64, 256, 256);
+    q.sx = ce_splits(mt * ((N + kCeTile - 1) / kCeTile), q.vc, 256);
+    q.sw = ce_splits(mt * (q.vc / kCeTile), q.n64, 256);
   }
   if (q.sx > 1 || q.pieces > 1) q.dxp = take((int64_t)q.sx * N * q.ldq * 4);
   if (q.sw > 1) q.dwp = take((int64_t)q.sw * q.vc * q.ldq * 4);
@@ -1012,8 +1064,8 @@ int ce_launch(CeArgs a, int splits, hipStream_t s) {
   constexpr int bytes = S::NS * (S::BM + S::BN) * S::BK * 2;
   static std::atomic<uint64_t> mask{0};
   CRESTE_HIP(ensure_dyn_smem((const void*)ce_gemm_kernel<MODE, DT, P, S>, bytes, mask));
-  a.mt = cdiv(a.m, S::BM);
-  if (MODE == CE_GRAD) a.mt = (int)(a.ldg / 2 / S::BM);          // the zeros behind the last class too
+  static_assert(S::BM == kCeTile, "");
+  if (MODE != CE_GRAD) a.mt = cdiv(a.m, S::BM);          // (GRAD: given, the zeros behind the last class too)
   a.nt = cdiv(a.n, S::BN);
   const int64_t blocks = (int64_t)a.mt * a.nt * splits;
   CRESTE_REQUIRE(blocks < (1ll << 31), "linear_ce: too many tiles");
@@ -1062,46 +1114,32 @@ int ce_stream(const CePlan& q, const CeArgs& a, int splits, hipStream_t s) {
 
 int ce_grid(int64_t items) { return (int)(items < 1 ? 1 : items > 2048 ? 2048 : items); }
 
-int ce_pack(const void* src, int64_t ld, int64_t rows, int D, int dtype, const CePlan& q, float* amax, char* dst, hipStream_t s) {
-  const int nb = ce_grid(rows * (q.Dp / 4) / 256 + 1);
-  const int64_t piece = rows * q.Dp;
-  if (dtype == CRESTE_DT_F32) {
-    ce_amax_kernel<<<ce_grid(rows * D / 1024 + 1), 256, 0, s>>>((const float*)src, rows, D, ld, amax);
-    ce_pack_kernel<float><<<nb, 256, 0, s>>>((const float*)src, rows, D, ld, q.Dp, amax, (short*)dst, piece);
-  } else {
-    ce_pack_kernel<short><<<nb, 256, 0, s>>>((const short*)src, rows, D, ld, q.Dp, nullptr, (short*)dst, piece);
+struct CeOperand { const char* p; int64_t ld, piece; };
+
+int ce_operands(const CePlan& q, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int D, int dtype,
+                char* work, CeOperand* X, CeOperand* W, hipStream_t s) {
+  float *amax = (float*)(work + q.amax), *bmax = amax + 16;
+  *X = {(const char*)x, ldx * 2, 0};
+  *W = {(const char*)w, ldw * 2, 0};
+  if (q.packx) *X = {work + q.xp, (int64_t)q.Dp * 2, N * q.Dp * 2};
+  if (q.packw) *W = {work + q.wp, (int64_t)q.Dp * 2, V * q.Dp * 2};
+  const CeSide sx{x, N, ldx, (short*)(work + q.xp), N * q.Dp}, sw{w, V, ldw, (short*)(work + q.wp), V * q.Dp};
+  auto blocks = [](int64_t rows, int most) { const int64_t b = (rows + 15) / 16; return (int)(b > most ? most : b); };
+  const int px = q.packx ? blocks(N, 2048) : 0, pw = q.packw ? blocks(V, 2048) : 0;
+  if (q.P == 2) {                                  // (both are copied)
+    const int ax = blocks(N, kCeMaxima), aw = blocks(V, kCeMaxima);
+    ce_amax_kernel<<<ax + aw, 256, 0, s>>>(sx, sw, D, ax, bmax);
+    ce_pack_kernel<float><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, bmax, ax, aw, amax);
+  } else if (px + pw) {
+    ce_pack_kernel<short><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, nullptr, 0, 0, nullptr);
   }
   CRESTE_CHECK_LAUNCH("linear_ce pack");
   return CRESTE_OK;
 }
 
-struct CeOperand { const char* p; int64_t ld, piece; };
-
-int ce_operands(const CePlan& q, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int D, int dtype,
-                char* work, CeOperand* X, CeOperand* W, hipStream_t s) {
-  float* amax = (float*)(work + q.amax);
-  if (q.P == 2) {
-    ce_zero_kernel<<<1, 64, 0, s>>>(amax, 2);
-    CRESTE_CHECK_LAUNCH("linear_ce zero");
-  }
-  *X = {(const char*)x, ldx * 2, 0};
-  *W = {(const char*)w, ldw * 2, 0};
-  if (q.packx) {
-    const int rc = ce_pack(x, ldx, N, D, dtype, q, amax, work + q.xp, s);
-    if (rc) return rc;
-    *X = {work + q.xp, (int64_t)q.Dp * 2, N * q.Dp * 2};
-  }
-  if (q.packw) {
-    const int rc = ce_pack(w, ldw, V, D, dtype, q, amax + 1, work + q.wp, s);
-    if (rc) return rc;
-    *W = {work + q.wp, (int64_t)q.Dp * 2, V * q.Dp * 2};
-  }
-  return CRESTE_OK;
-}
-
-int ce_check(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* labels, int64_t N, int64_t V, int D, int dtype,
+int ce_check(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* labels_or_rows, int64_t N, int64_t V, int D, int dtype,
              float tau) {
-  CRESTE_REQUIRE(x && w && labels, "linear_ce: null pointer");
+  CRESTE_REQUIRE(x && w && labels_or_rows, "linear_ce: null pointer");
   CRESTE_REQUIRE(dtype >= CRESTE_DT_F32 && dtype <= CRESTE_DT_F16, "linear_ce: dtype %d", dtype);
   CRESTE_REQUIRE(N > 0 && V > 0 && D > 0 && N < (1ll << 30) && V < (1ll << 30) && D <= 65536, "linear_ce: N %lld V %lld D %d",
                  (long long)N, (long long)V, D);
@@ -1124,13 +1162,13 @@ extern "C" int64_t creste_linear_ce_workspace_bytes(int64_t N, int64_t V, int D,
 
 extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* labels, int64_t N,
                                         int64_t V, int D, int dtype, int64_t ignore_index, float temperature, int mean,
-                                        float* loss, float* nll, float* lse2, float* stat, void* work, int64_t work_bytes,
+                                        float* loss, float* nll, float* rows, float* stat, void* work, int64_t work_bytes,
                                         void* stream) {
   const int bad = ce_check(x, ldx, w, ldw, labels, N, V, D, dtype, temperature);
   if (bad) return bad;
   const bool few = N <= kCeFewRows && ce_few(x, ldx, D, dtype) && ce_few(w, ldw, D, dtype);
   const CePlan q = ce_plan(N, V, D, dtype, !few && !ce_direct(x, ldx, D, dtype), !few && !ce_direct(w, ldw, D, dtype), false);
-  CRESTE_REQUIRE(loss && nll && lse2 && stat && work && work_bytes >= q.total, "linear_ce_forward: outputs / workspace (%lld of %lld bytes)",
+  CRESTE_REQUIRE(loss && nll && rows && stat && work && work_bytes >= q.total, "linear_ce_forward: outputs / workspace (%lld of %lld bytes)",
                  (long long)work_bytes, (long long)q.total);
   hipStream_t s = (hipStream_t)stream;
   char* wk = (char*)work;
@@ -1147,7 +1185,7 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
   a.labels = labels; a.ignore = ignore_index; a.classes = (int)V;
   a.inv_tau = 1.f / temperature;
   a.amax = q.P == 2 ? (const float*)(wk + q.amax) : nullptr;
-  a.part = (float2*)(wk + q.part); a.zlab = (float*)(wk + q.zlab);
+  a.part = (float2*)(wk + q.part); a.zlab = (float*)(wk + q.zlab); a.done = (unsigned*)(wk + q.done);
   if (few) {
     if (dtype == CRESTE_DT_F32) ce_few_kernel<CRESTE_DT_F32><<<q.tiles, 256, 0, s>>>(a, D);
     else if (dtype == CRESTE_DT_BF16) ce_few_kernel<CRESTE_DT_BF16><<<q.tiles, 256, 0, s>>>(a, D);
@@ -1158,22 +1196,21 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
     if (rg) return rg;
   }
   const int nb = cdiv(N, 64);
-  ce_join_kernel<<<nb, 1024, 0, s>>>(a.part, q.stream && !few ? q.sl : q.tiles, (int)N, a.zlab, labels, ignore_index, (int)V, nll, lse2, (float2*)(wk + q.bsum),
-                                       mean, loss, stat);
-  if (nb > 1) ce_final_kernel<<<1, 256, 0, s>>>((const float2*)(wk + q.bsum), nb, mean, loss, stat);
+  ce_join_kernel<<<nb, 1024, 0, s>>>(a.part, q.stream && !few ? q.sl : q.tiles, (int)N, a.zlab, labels, ignore_index, (int)V,
+                                     ce_gscale_log2(q), nll, rows, (int*)(rows + up(N, 64)), (uint64_t*)(wk + q.bsum), a.done, mean,
+                                     loss, stat);
   CRESTE_CHECK_LAUNCH("linear_ce join");
   return CRESTE_OK;
 }
 
-extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* labels, int64_t N,
-                                         int64_t V, int D, int dtype, int64_t ignore_index, float temperature, int mean,
-                                         const float* lse2, const float* stat, const float* g_loss, void* gx, void* gw, void* work,
-                                         int64_t work_bytes, void* stream) {
-  const int bad = ce_check(x, ldx, w, ldw, labels, N, V, D, dtype, temperature);
+extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* rows, int64_t N, int64_t V,
+                                         int D, int dtype, float temperature, int mean, const float* stat, const float* g_loss,
+                                         void* gx, void* gw, void* work, int64_t work_bytes, void* stream) {
+  const int bad = ce_check(x, ldx, w, ldw, rows, N, V, D, dtype, temperature);
   if (bad) return bad;
   const CePlan q = ce_plan(N, V, D, dtype, !ce_direct(x, ldx, D, dtype), !ce_direct(w, ldw, D, dtype), true);
-  CRESTE_REQUIRE(lse2 && stat && g_loss && (gx || gw) && work && work_bytes >= q.total,
-                 "linear_ce_backward: inputs / workspace (%lld of %lld bytes)", (long long)work_bytes, (long long)q.total);
+  CRESTE_REQUIRE(stat && g_loss && (gx || gw) && work && work_bytes >= q.total, "linear_ce_backward: inputs / workspace (%lld of %lld bytes)",
+                 (long long)work_bytes, (long long)q.total);
   hipStream_t s = (hipStream_t)stream;
   char* wk = (char*)work;
   CeOperand X, W;
@@ -1184,17 +1221,16 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
   c.inv_tau = 1.f / temperature;
   c.amax = q.P == 2 ? (const float*)(wk + q.amax) : nullptr;
   c.stat = stat; c.gl = g_loss; c.mean = mean;
-  c.gscale = q.dt16 == CRESTE_DT_F16 ? kCeF16Scale : 1.f;
-  c.row_l2 = (const float*)(wk + q.row_l2); c.row_lab = (const int*)(wk + q.row_lab);
+  c.gscale = exp2f(ce_gscale_log2(q));
+  c.row_l2 = rows; c.row_lab = (const int*)(rows + q.n64);
   c.n64 = (int)q.n64;
   c.out_dt = dtype;
   c.ldo = c.m_out = D;
   c.ldp = q.ldq;
-  ce_rows_kernel<<<cdiv(q.n64, 256), 256, 0, s>>>(lse2, labels, (int)N, (int)q.n64, ignore_index, (int)V, log2f(c.gscale),
-                                                  (float*)(wk + q.row_l2), (int*)(wk + q.row_lab));
-  CRESTE_CHECK_LAUNCH("linear_ce rows");
-  auto reduce = [&](const CeArgs& a, int splits) {
-    ce_reduce_kernel<<<ce_grid((int64_t)a.n * q.ldq / 1024 + 1), 256, 0, s>>>(a, splits);
+  auto reduce = [&](const CeArgs* u, int su, const CeArgs* v, int sv) {      // one or two sums of partials in one launch
+    auto blocks = [&](const CeArgs& a) { return ce_grid((int64_t)a.n * q.ldq / 1024 + 1); };
+    const int bu = u ? blocks(*u) : 0, bv = v ? blocks(*v) : 0;
+    ce_reduce_kernel<<<bu + bv, 256, 0, s>>>(u ? *u : *v, su, v ? *v : *u, sv, bu);
     CRESTE_CHECK_LAUNCH("linear_ce reduce");
     return CRESTE_OK;
   };
@@ -1216,13 +1252,12 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
       dw.out = gw;
       const int rg = ce_stream<CE_DW>(q, dw, q.sw, s);
       if (rg) return rg;
-      if (dw.partial && reduce(dw, q.sw)) return CRESTE_ERR_HIP;
     }
   } else {
     for (int piece = 0; piece < q.pieces; ++piece) {
       const int64_t v0 = piece * q.vc, nv = V - v0 < q.vc ? V - v0 : q.vc;
       CeArgs a = c;                                 // G of the piece
-      a.g = wk + q.g; a.ldg = q.vc * 2; a.pg = q.n64 * q.vc * 2;
+      a.g = wk + q.g; a.ldg = q.ldg; a.pg = q.n64 * q.ldg; a.mt = (int)(q.vc / kCeTile);
       a.a = W.p + v0 * W.ld; a.lda = W.ld; a.pa = W.piece; a.ra = nv;
       a.b = X.p; a.ldb = X.ld; a.pb = X.piece; a.rb = N;
       a.m = (int)nv; a.n = (int)N; a.class0 = (int)v0;
@@ -1248,10 +1283,10 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
         dw.out = (char*)gw + v0 * D * q.es;
         rg = ce_gemm<CE_DW>(q, dw, q.sw, s);
         if (rg) return rg;
-        if (dw.partial && reduce(dw, q.sw)) return CRESTE_ERR_HIP;
+        if (dw.partial && q.pieces > 1 && reduce(nullptr, 0, &dw, q.sw)) return CRESTE_ERR_HIP;
       }
     }
   }
-  if (gx && dx.partial && reduce(dx, q.sx)) return CRESTE_ERR_HIP;
-  return CRESTE_OK;
+  const bool rx = gx && dx.partial, rw = gw && dw.partial && q.pieces == 1;
+  return rx || rw ? reduce(rx ? &dx : nullptr, q.sx, rw ? &dw : nullptr, q.sw) : CRESTE_OK;
 }

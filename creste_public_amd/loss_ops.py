@@ -170,18 +170,18 @@ class LinearCEFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, labels, ignore_index, temperature, reduction):
-        loss, nll, lse2, stat = ops.linear_ce(x, weight, labels, ignore_index, temperature, reduction)
-        ctx.save_for_backward(x, weight, labels, lse2, stat)
-        ctx.args = (ignore_index, temperature, reduction)
+        loss, nll, rows, stat = ops.linear_ce(x, weight, labels, ignore_index, temperature, reduction)
+        ctx.save_for_backward(x, weight, rows, stat)
+        ctx.args = (temperature, reduction)
         ctx.mark_non_differentiable(nll)
         return loss, nll
 
     @staticmethod
     @once
     def backward(ctx, gl, _):
-        x, weight, labels, lse2, stat = ctx.saved_tensors
-        gx, gw = ops._linear_ce_bwd(ops._rows(x), ops._rows(weight), labels.contiguous(), lse2, stat, gl, *ctx.args,
-                                    ctx.needs_input_grad[0], ctx.needs_input_grad[1], ops._DTYPE_CODE[x.dtype])
+        x, weight, rows, stat = ctx.saved_tensors
+        gx, gw = ops._linear_ce_bwd(ops._rows(x), ops._rows(weight), rows, stat, gl, *ctx.args, ctx.needs_input_grad[0],
+                                    ctx.needs_input_grad[1], ops._DTYPE_CODE[x.dtype])
         return gx, gw, None, None, None, None
 
 

@@ -1630,17 +1630,16 @@ def _recurrence_bwd(gate, x, lengths, starts, gh, gh_last, code):
     return gg, gx, gh0
 
 
-def _linear_ce_args(x, w, labels, temperature, reduction):
+def _linear_ce_args(x, w, temperature, reduction):
     code = _features(x, "linear_cross_entropy: x", 2)
     _features(w, "linear_cross_entropy: weight", 2, like=x)
     if w.shape[1] != x.shape[1] or w.shape[0] < 1 or w.shape[1] < 1:
         raise HipLibraryError(f"linear_cross_entropy: x {tuple(x.shape)} beside weight {tuple(w.shape)}")
-    labels = _plain(labels, torch.int64, (x.shape[0],), x.device, "linear_cross_entropy: labels")
     if reduction not in ("mean", "sum"):
         raise HipLibraryError(f"linear_cross_entropy: reduction {reduction!r} (mean or sum)")
     if not 0.0 < float(temperature) < float("inf"):
         raise HipLibraryError(f"linear_cross_entropy: temperature {temperature}")
-    return code, _rows(x.detach()), _rows(w.detach()), labels
+    return code, _rows(x.detach()), _rows(w.detach())
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -1648,38 +1647,39 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def linear_ce(x, w, labels, ignore_index: int = -100, temperature: float = 1.0, reduction: str = "mean"):
-    """forward of loss_ops.linear_cross_entropy -> (loss [], nll [N], lse2 [N], stat [2]), fp32"""
-    code, x_, w_, labels = _linear_ce_args(x, w, labels, temperature, reduction)
+    """forward of loss_ops.linear_cross_entropy for x [N,D] -> (loss [], nll [N], rows, stat), fp32; rows and stat are what
+    linear_ce_bwd needs of it"""
+    code, x_, w_ = _linear_ce_args(x, w, temperature, reduction)
     N, D = x_.shape
     V, dev = w_.shape[0], x_.device
+    labels = _plain(labels, torch.int64, (N,), dev, "linear_cross_entropy: labels")
     loss, stat = torch.empty((), dtype=torch.float32, device=dev), torch.empty(2, dtype=torch.float32, device=dev)
-    nll, lse2 = torch.empty(N, dtype=torch.float32, device=dev), torch.empty(N, dtype=torch.float32, device=dev)
+    nll, rows = torch.empty(N, dtype=torch.float32, device=dev), torch.empty((2, -(-N // 64) * 64), dtype=torch.float32, device=dev)
     if N == 0:
-        return loss.zero_(), nll, lse2, stat.zero_()
+        return loss.zero_(), nll, rows, stat.zero_()
     lib = _lib.load()
     with _on(dev) as on:
         nb = lib.creste_linear_ce_workspace_bytes(N, V, D, code, 0)
         work = torch.empty(nb, dtype=torch.uint8, device=dev)
         _lib.check(lib.creste_linear_ce_forward(x_.data_ptr(), _row_stride(x_), w_.data_ptr(), _row_stride(w_), labels.data_ptr(), N, V, D,
-                                                code, int(ignore_index), float(temperature), int(reduction == "mean"),
-                                                loss.data_ptr(), nll.data_ptr(), lse2.data_ptr(), stat.data_ptr(),
-                                                work.data_ptr(), nb, on.stream), "linear_ce_forward")
-    return loss, nll, lse2, stat
+                                                code, _int64(ignore_index, "linear_cross_entropy: ignore_index"), float(temperature),
+                                                int(reduction == "mean"), loss.data_ptr(), nll.data_ptr(), rows.data_ptr(),
+                                                stat.data_ptr(), work.data_ptr(), nb, on.stream), "linear_ce_forward")
+    return loss, nll, rows, stat
 
 
-def linear_ce_bwd(x, w, labels, lse2, stat, g_loss, ignore_index: int = -100, temperature: float = 1.0, reduction: str = "mean",
-                  need_x: bool = True, need_w: bool = True):
+def linear_ce_bwd(x, w, rows, stat, g_loss, temperature: float = 1.0, reduction: str = "mean", need_x: bool = True,
+                  need_w: bool = True):
     """gradient of linear_ce for the cotangent g_loss (one fp32 element) -> (gx, gw); None for what is not needed"""
-    code, x_, w_, labels = _linear_ce_args(x, w, labels, temperature, reduction)
-    N, D = x_.shape
-    V, dev = w_.shape[0], x_.device
-    lse2 = _plain(lse2, torch.float32, (N,), dev, "linear_cross_entropy: lse2")
+    code, x_, w_ = _linear_ce_args(x, w, temperature, reduction)
+    N, dev = x_.shape[0], x_.device
+    rows = _plain(rows, torch.float32, (2, -(-N // 64) * 64), dev, "linear_cross_entropy: rows")
     stat = _plain(stat, torch.float32, (2,), dev, "linear_cross_entropy: stat")
     g_loss = _plain(g_loss.reshape(1), torch.float32, (1,), dev, "linear_cross_entropy: cotangent")
-    return _linear_ce_bwd(x_, w_, labels, lse2, stat, g_loss, ignore_index, temperature, reduction, need_x, need_w, code)
+    return _linear_ce_bwd(x_, w_, rows, stat, g_loss, temperature, reduction, need_x, need_w, code)
 
 
-def _linear_ce_bwd(x, w, labels, lse2, stat, g_loss, ignore_index, temperature, reduction, need_x, need_w, code):
+def _linear_ce_bwd(x, w, rows, stat, g_loss, temperature, reduction, need_x, need_w, code):
     """linear_ce_bwd of checked tensors (x and w with contiguous rows, the others contiguous)"""
     N, D = x.shape
     V = w.shape[0]
@@ -1691,9 +1691,9 @@ def _linear_ce_bwd(x, w, labels, lse2, stat, g_loss, ignore_index, temperature, 
     with _on(x.device) as on:
         nb = lib.creste_linear_ce_workspace_bytes(N, V, D, code, 1)
         work = torch.empty(nb, dtype=torch.uint8, device=x.device)
-        _lib.check(lib.creste_linear_ce_backward(x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), labels.data_ptr(), N, V, D,
-                                                 code, int(ignore_index), float(temperature), int(reduction == "mean"),
-                                                 lse2.data_ptr(), stat.data_ptr(), g_loss.data_ptr(),
-                                                 gx.data_ptr() if need_x else None, gw.data_ptr() if need_w else None,
-                                                 work.data_ptr(), nb, on.stream), "linear_ce_backward")
+        _lib.check(lib.creste_linear_ce_backward(x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), rows.data_ptr(), N, V, D,
+                                                 code, float(temperature), int(reduction == "mean"), stat.data_ptr(),
+                                                 g_loss.data_ptr(), gx.data_ptr() if need_x else None,
+                                                 gw.data_ptr() if need_w else None, work.data_ptr(), nb, on.stream),
+                   "linear_ce_backward")
     return gx, gw

@@ -702,18 +702,17 @@ int creste_irl_visitation_mix_f32(const float* exp_svf_raw, const uint8_t* fov, 
  * Softmax cross entropy over V classes straight from the features (csrc/linear_ce.hip): z = x w^T / temperature, x [N][ldx],
  * w [V][ldw] (strides in elements, D of them used), labels [N] int64; a row whose label is ignore_index does not count, one whose
  * label names no class makes loss and gradients NaN.  No N x V buffer.
- *   forward : loss [1] (mean over the counted rows, 0 if there are none, or sum), nll [N] (0 where ignored), lse2 [N] (log-sum-exp
- *             in log2 units) and stat [2] = {sum nll, count} for the backward.
+ *   forward : loss [1] (mean over the counted rows, 0 if there are none, or sum), nll [N] (0 where ignored), and for the backward
+ *             rows [2][N rounded up to 64] 4-byte words (scaled log-sum-exps; labels) and stat [2] = {sum nll, count}.
  *   backward: gx [N][D], gw [V][D] (contiguous, the features' type; either may be NULL) for the cotangent g_loss [1].
  * work: workspace_bytes(..., train = 0) for the forward, train = 1 for the backward; -1 = sizes out of range. */
 int64_t creste_linear_ce_workspace_bytes(int64_t N, int64_t V, int D, int dtype, int train);
 int creste_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* labels, int64_t N, int64_t V,
                              int D, int dtype, int64_t ignore_index, float temperature, int mean, float* loss, float* nll,
-                             float* lse2, float* stat, void* work, int64_t work_bytes, void* stream);
-int creste_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* labels, int64_t N, int64_t V,
-                              int D, int dtype, int64_t ignore_index, float temperature, int mean, const float* lse2,
-                              const float* stat, const float* g_loss, void* gx, void* gw, void* work, int64_t work_bytes,
-                              void* stream);
+                             float* rows, float* stat, void* work, int64_t work_bytes, void* stream);
+int creste_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* rows, int64_t N, int64_t V, int D,
+                              int dtype, float temperature, int mean, const float* stat, const float* g_loss, void* gx, void* gw,
+                              void* work, int64_t work_bytes, void* stream);
 
 /* Dropout (csrc/dropout.hip): y_i = keep_i ? x_i / (1 - p) : 0 (+ residual_i), 0 <= p <= 1, n elements.  keep_i = word_i >=
  * round(p 2^32), word_i = word i mod 4 of Philox4x32-10 with counter (i div 4, offset) and key seed, 64 bits each.  The backward is
