@@ -380,10 +380,10 @@ namespace {
 int64_t rec_chunks(int64_t T) { return (T + kRecChunkB - 1) / kRecChunkB; }     // the smaller of the two chunks
 
 // The workspace, all zero at the start: a ticket line per column group (sized as if a lane took one column), the published pairs
-// and values; a multiple of 16 bytes in all
+// and values; a multiple of 16 bytes in all, none for a single chunk
 int64_t rec_tickets(int64_t BC) { return (BC + 63) / 64 * kRecTicket * 4; }
 int64_t rec_work(int64_t BC, int64_t chunks) {
-  return chunks == 1 ? 16 : rec_tickets(BC) + ((chunks + chunks / kRecWindow) * BC + 1) / 2 * 16;
+  return chunks == 1 ? 0 : rec_tickets(BC) + ((chunks + chunks / kRecWindow) * BC + 1) / 2 * 16;
 }
 
 template <typename T, int VEC, int LF, int LB>
@@ -429,6 +429,11 @@ int rec_run(RecArgs& p, int dtype, bool bwd, char* work, hipStream_t s) {
   return CRESTE_ERR_ARG;
 }
 
+bool rec_work_ok(const void* work, int64_t bytes, int64_t B, int64_t T, int64_t C) {
+  const int64_t need = rec_work(B * C, rec_chunks(T));
+  return need == 0 || (work && ((uintptr_t)work & 15) == 0 && bytes >= need);
+}
+
 int rec_check(int64_t B, int64_t T, int64_t C) {
   CRESTE_REQUIRE(B > 0 && T > 0 && C > 0 && B < (1ll << 31) && C < (1ll << 31) && B * C < (1ll << 40) && T < (1ll << 36),
                  "gated_recurrence: B %lld T %lld C %lld", (long long)B, (long long)T, (long long)C);
@@ -453,7 +458,7 @@ extern "C" int creste_gated_recurrence_forward(const void* gate, int64_t gate_sb
                                                int64_t work_bytes, void* stream) {
   const int rc = rec_check(B, T, C);
   if (rc) return rc;
-  CRESTE_REQUIRE(gate && x && h && h_last && work && ((uintptr_t)work & 15) == 0 && work_bytes >= creste_gated_recurrence_workspace_bytes(B, T, C),
+  CRESTE_REQUIRE(gate && x && h && h_last && rec_work_ok(work, work_bytes, B, T, C),
                  "gated_recurrence_forward: null pointer or workspace of %lld bytes", (long long)work_bytes);
   RecArgs p{};
   p.gate = gate; p.g_sb = gate_sb; p.g_st = gate_st;
@@ -471,8 +476,7 @@ extern "C" int creste_gated_recurrence_backward(const void* gate, int64_t gate_s
                                                 int64_t work_bytes, void* stream) {
   const int rc = rec_check(B, T, C);
   if (rc) return rc;
-  CRESTE_REQUIRE(gate && x && gh && starts && ggate && gx && work && ((uintptr_t)work & 15) == 0 &&
-                     work_bytes >= creste_gated_recurrence_workspace_bytes(B, T, C),
+  CRESTE_REQUIRE(gate && x && gh && starts && ggate && gx && rec_work_ok(work, work_bytes, B, T, C),
                  "gated_recurrence_backward: null pointer or workspace of %lld bytes", (long long)work_bytes);
   RecArgs p{};
   p.gate = gate; p.g_sb = gate_sb; p.g_st = gate_st;

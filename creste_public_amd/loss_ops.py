@@ -7,7 +7,7 @@ import torch
 
 from . import _lib, ops
 from .ops import HipLibraryError, _stream
-from .train_ops import as_act, once
+from .train_ops import as_act, once, recorded
 
 
 def _work(dev):
@@ -170,8 +170,8 @@ class LinearCEFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, labels, ignore_index, temperature, reduction):
-        loss, nll, rows, stat = ops.linear_ce(x, weight, labels, ignore_index, temperature, reduction)
-        ctx.save_for_backward(x, weight, rows, stat)
+        loss, nll, saved = ops.linear_ce(x, weight, labels, ignore_index, temperature, reduction)
+        ctx.save_for_backward(x, weight, saved)
         ctx.args = (temperature, reduction)
         ctx.mark_non_differentiable(nll)
         return loss, nll
@@ -179,8 +179,8 @@ class LinearCEFn(torch.autograd.Function):
     @staticmethod
     @once
     def backward(ctx, gl, _):
-        x, weight, rows, stat = ctx.saved_tensors
-        gx, gw = ops._linear_ce_bwd(ops._rows(x), ops._rows(weight), rows, stat, gl, *ctx.args, ctx.needs_input_grad[0],
+        x, weight, saved = ctx.saved_tensors
+        gx, gw = ops._linear_ce_bwd(ops._rows(x), ops._rows(weight), saved, gl, *ctx.args, ctx.needs_input_grad[0],
                                     ctx.needs_input_grad[1], ops._DTYPE_CODE[x.dtype])
         return gx, gw, None, None, None, None
 
@@ -197,7 +197,11 @@ def linear_cross_entropy(x, weight, labels, ignore_index: int = -100, temperatur
     lead = x.shape[:-1]
     if not isinstance(labels, torch.Tensor) or labels.shape != lead:
         raise HipLibraryError(f"linear_cross_entropy: labels must have the shape {tuple(lead)} of the features' rows")
-    if x.dim() == 2:
-        return LinearCEFn.apply(x, weight, labels, ignore_index, temperature, reduction)
-    loss, nll = LinearCEFn.apply(x.reshape(labels.numel(), x.shape[-1]), weight, labels.reshape(-1), ignore_index, temperature, reduction)
-    return loss, nll.reshape(lead)
+    flat = x.dim() == 2
+    args = (x if flat else x.reshape(labels.numel(), x.shape[-1]), weight, labels if flat else labels.reshape(-1), ignore_index,
+            temperature, reduction)
+    if recorded(x, weight):
+        loss, nll = LinearCEFn.apply(*args)
+    else:
+        loss, nll, _ = ops.linear_ce(*args)
+    return loss, nll if flat else nll.reshape(lead)

@@ -1481,10 +1481,10 @@ def _features(t, name: str, ndim=None, like=None) -> int:
 
 def _plain(t, dtype, shape, device, name: str) -> torch.Tensor:
     """a contiguous tensor of this type, shape and device -- or an error (values are copied if only the strides differ)"""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape or t.device != device:
-        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
-        raise HipLibraryError(f"{name}: expected {dtype} {tuple(shape)} on {device}, got {got}")
-    return t.contiguous()
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device:
+        return t.contiguous()
+    got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+    raise HipLibraryError(f"{name}: expected {dtype} {tuple(shape)} on {device}, got {got}")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -1585,11 +1585,11 @@ def gated_recurrence(gate: torch.Tensor, x: torch.Tensor, h0: torch.Tensor | Non
         if save:
             starts = torch.empty((-(-T // lib.creste_gated_recurrence_chunk_steps()), B, Cc), dtype=torch.float32, device=dev)
         nb = lib.creste_gated_recurrence_workspace_bytes(B, T, Cc)
-        work = torch.empty(nb, dtype=torch.uint8, device=dev)
+        work = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
         _lib.check(lib.creste_gated_recurrence_forward(
             g_.data_ptr(), g_.stride(0), g_.stride(1), x_.data_ptr(), x_.stride(0), x_.stride(1),
             h0.data_ptr() if h0 is not None else None, lengths.data_ptr() if lengths is not None else None, B, T, Cc, code,
-            h.data_ptr(), last.data_ptr(), starts.data_ptr() if save else None, work.data_ptr(), nb, on.stream),
+            h.data_ptr(), last.data_ptr(), starts.data_ptr() if save else None, work.data_ptr() if nb else None, nb, on.stream),
             "gated_recurrence_forward")
     return (h, last, starts) if save else (h, last)
 
@@ -1621,11 +1621,12 @@ def _recurrence_bwd(gate, x, lengths, starts, gh, gh_last, code):
     lib = _lib.load()
     with _on(gate.device) as on:
         nb = lib.creste_gated_recurrence_workspace_bytes(B, T, Cc)
-        work = torch.empty(nb, dtype=torch.uint8, device=gate.device)
+        work = torch.empty(nb, dtype=torch.uint8, device=gate.device) if nb else None
         _lib.check(lib.creste_gated_recurrence_backward(
             gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1), gh.data_ptr(), gh.stride(0),
             gh.stride(1), gh_last.data_ptr() if gh_last is not None else None, lengths.data_ptr() if lengths is not None else None,
-            starts.data_ptr(), B, T, Cc, code, gg.data_ptr(), gx.data_ptr(), gh0.data_ptr(), work.data_ptr(), nb, on.stream),
+            starts.data_ptr(), B, T, Cc, code, gg.data_ptr(), gx.data_ptr(), gh0.data_ptr(), work.data_ptr() if nb else None, nb,
+            on.stream),
             "gated_recurrence_backward")
     return gg, gx, gh0
 
@@ -1642,44 +1643,46 @@ def _linear_ce_args(x, w, temperature, reduction):
     return code, _rows(x.detach()), _rows(w.detach())
 
 
+def _ce_saved(N: int) -> int:
+    return 4 + 2 * (-(-N // 64) * 64)          # {sum, count, -, -}, [2][N rounded up to 64]
+
+
 def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def linear_ce(x, w, labels, ignore_index: int = -100, temperature: float = 1.0, reduction: str = "mean"):
-    """forward of loss_ops.linear_cross_entropy for x [N,D] -> (loss [], nll [N], rows, stat), fp32; rows and stat are what
-    linear_ce_bwd needs of it"""
+    """forward of loss_ops.linear_cross_entropy for x [N,D] -> (loss [], nll [N], saved), fp32; `saved` is what linear_ce_bwd needs of it
+    (sum and count, then two words per row)"""
     code, x_, w_ = _linear_ce_args(x, w, temperature, reduction)
     N, D = x_.shape
     V, dev = w_.shape[0], x_.device
     labels = _plain(labels, torch.int64, (N,), dev, "linear_cross_entropy: labels")
-    loss, stat = torch.empty((), dtype=torch.float32, device=dev), torch.empty(2, dtype=torch.float32, device=dev)
-    nll, rows = torch.empty(N, dtype=torch.float32, device=dev), torch.empty((2, -(-N // 64) * 64), dtype=torch.float32, device=dev)
+    loss, nll = torch.empty((), dtype=torch.float32, device=dev), torch.empty(N, dtype=torch.float32, device=dev)
+    saved = torch.empty(_ce_saved(N), dtype=torch.float32, device=dev)
     if N == 0:
-        return loss.zero_(), nll, rows, stat.zero_()
+        return loss.zero_(), nll, saved.zero_()
     lib = _lib.load()
     with _on(dev) as on:
         nb = lib.creste_linear_ce_workspace_bytes(N, V, D, code, 0)
         work = torch.empty(nb, dtype=torch.uint8, device=dev)
         _lib.check(lib.creste_linear_ce_forward(x_.data_ptr(), _row_stride(x_), w_.data_ptr(), _row_stride(w_), labels.data_ptr(), N, V, D,
                                                 code, _int64(ignore_index, "linear_cross_entropy: ignore_index"), float(temperature),
-                                                int(reduction == "mean"), loss.data_ptr(), nll.data_ptr(), rows.data_ptr(),
-                                                stat.data_ptr(), work.data_ptr(), nb, on.stream), "linear_ce_forward")
-    return loss, nll, rows, stat
+                                                int(reduction == "mean"), loss.data_ptr(), nll.data_ptr(), saved.data_ptr() + 16,
+                                                saved.data_ptr(), work.data_ptr(), nb, on.stream), "linear_ce_forward")
+    return loss, nll, saved
 
 
-def linear_ce_bwd(x, w, rows, stat, g_loss, temperature: float = 1.0, reduction: str = "mean", need_x: bool = True,
+def linear_ce_bwd(x, w, saved, g_loss, temperature: float = 1.0, reduction: str = "mean", need_x: bool = True,
                   need_w: bool = True):
     """gradient of linear_ce for the cotangent g_loss (one fp32 element) -> (gx, gw); None for what is not needed"""
     code, x_, w_ = _linear_ce_args(x, w, temperature, reduction)
-    N, dev = x_.shape[0], x_.device
-    rows = _plain(rows, torch.float32, (2, -(-N // 64) * 64), dev, "linear_cross_entropy: rows")
-    stat = _plain(stat, torch.float32, (2,), dev, "linear_cross_entropy: stat")
-    g_loss = _plain(g_loss.reshape(1), torch.float32, (1,), dev, "linear_cross_entropy: cotangent")
-    return _linear_ce_bwd(x_, w_, rows, stat, g_loss, temperature, reduction, need_x, need_w, code)
+    saved = _plain(saved, torch.float32, (_ce_saved(x_.shape[0]),), x_.device, "linear_cross_entropy: saved")
+    g_loss = _plain(g_loss.reshape(1), torch.float32, (1,), x_.device, "linear_cross_entropy: cotangent")
+    return _linear_ce_bwd(x_, w_, saved, g_loss, temperature, reduction, need_x, need_w, code)
 
 
-def _linear_ce_bwd(x, w, rows, stat, g_loss, temperature, reduction, need_x, need_w, code):
+def _linear_ce_bwd(x, w, saved, g_loss, temperature, reduction, need_x, need_w, code):
     """linear_ce_bwd of checked tensors (x and w with contiguous rows, the others contiguous)"""
     N, D = x.shape
     V = w.shape[0]
@@ -1691,8 +1694,8 @@ def _linear_ce_bwd(x, w, rows, stat, g_loss, temperature, reduction, need_x, nee
     with _on(x.device) as on:
         nb = lib.creste_linear_ce_workspace_bytes(N, V, D, code, 1)
         work = torch.empty(nb, dtype=torch.uint8, device=x.device)
-        _lib.check(lib.creste_linear_ce_backward(x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), rows.data_ptr(), N, V, D,
-                                                 code, float(temperature), int(reduction == "mean"), stat.data_ptr(),
+        _lib.check(lib.creste_linear_ce_backward(x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), saved.data_ptr() + 16, N, V,
+                                                 D, code, float(temperature), int(reduction == "mean"), saved.data_ptr(),
                                                  g_loss.data_ptr(), gx.data_ptr() if need_x else None,
                                                  gw.data_ptr() if need_w else None, work.data_ptr(), nb, on.stream),
                    "linear_ce_backward")

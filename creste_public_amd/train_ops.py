@@ -608,10 +608,15 @@ def reward_forward_train(net, x: torch.Tensor) -> torch.Tensor:
     return RewardFn.apply(eng, x, *eng.params())
 
 
+def recorded(*tensors) -> bool:
+    """does autograd record an operation on these (else the Function around it is only overhead)"""
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
 def once(fn):
     """@once_differentiable whose bookkeeping is only paid when the backward itself is recorded (create_graph=True)"""
-    recorded = once_differentiable(fn)
-    return lambda ctx, *g: recorded(ctx, *g) if torch.is_grad_enabled() else fn(ctx, *g)
+    kept = once_differentiable(fn)
+    return lambda ctx, *g: kept(ctx, *g) if torch.is_grad_enabled() else fn(ctx, *g)
 
 
 class DropoutFn(torch.autograd.Function):
@@ -641,7 +646,7 @@ class DropoutFn(torch.autograd.Function):
 def dropout(x, p: float, seed, offset: int = 0, residual=None):
     """y = x / (1 - p) where an element is kept, else 0 (+ residual); see ops.dropout for what decides.  Differentiable in x and
     residual.  fp32 / bf16 / fp16, any shape."""
-    return DropoutFn.apply(x, p, seed, offset, residual)
+    return (DropoutFn.apply if recorded(x, residual) else ops.dropout)(x, p, seed, offset, residual)
 
 
 class GatedRecurrenceFn(torch.autograd.Function):
@@ -650,8 +655,6 @@ class GatedRecurrenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, h0, lengths):
         ctx.set_materialize_grads(False)
-        if not any(ctx.needs_input_grad[:3]):
-            return ops.gated_recurrence(gate, x, h0, lengths)
         h, last, starts = ops.gated_recurrence(gate, x, h0, lengths, save=True)
         ctx.save_for_backward(gate, x, lengths, starts)
         return h, last                         # (the backward relies on these checks of its inputs)
@@ -673,4 +676,4 @@ class GatedRecurrenceFn(torch.autograd.Function):
 def gated_recurrence(gate, x, h0=None, lengths=None):
     """h_t = f_t h_(t-1) + (1 - f_t) x_t, f = sigmoid(gate), over [B,T,C] sequences -> (h [B,T,C], h_last [B,C] fp32); arguments as
     ops.gated_recurrence.  Differentiable in gate, x and h0, through both outputs."""
-    return GatedRecurrenceFn.apply(gate, x, h0, lengths)
+    return (GatedRecurrenceFn.apply if recorded(gate, x, h0) else ops.gated_recurrence)(gate, x, h0, lengths)

@@ -725,6 +725,7 @@ int creste_dropout(const void* x, const void* residual, void* y, int64_t n, int 
  * channel, state in fp32.  gate / x / gh: element (b, t, c) at b * sb + t * st + c; h / ggate / gx: contiguous [B][T][C]; h0 / h_last /
  * gh_last / gh0: [B][C] fp32 (h0 NULL: zeros; gh_last NULL: zeros; gh0 NULL: not wanted).  lengths [B] int64 (NULL: all T):
  * steps behind a sequence's length are 0 in h and the gradients and leave the state alone.
+ * work: workspace_bytes, 16-byte aligned; may be NULL where that is 0.
  *   starts: state before every chunk_steps() steps, [chunks][B * C] fp32, chunks = ceil(T / chunk_steps()); forward writes it when
  *           not NULL, backward reads it. */
 int creste_gated_recurrence_chunk_steps(void);

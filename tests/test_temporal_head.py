@@ -83,7 +83,8 @@ def test_entry_points_report_bad_arguments():
     err(rec(gate=None), b"null pointer")
     err(rec(T=0), b"T 0")
     err(rec(B=1 << 31), b"B 2147483648")
-    err(rec(nb=3), b"workspace")
+    err(rec(T=300, nb=3), b"workspace")
+    assert lib.creste_gated_recurrence_workspace_bytes(2, 3, 4) == 0          # a single chunk of steps needs none
     err(rec(dt=9), b"dtype")
     err(lib.creste_gated_recurrence_backward(p, 12, 4, p, 12, 4, p, 12, 4, None, None, None, 2, 3, 4, 0, p, p, None, p, 1 << 40, None),
         b"null pointer")

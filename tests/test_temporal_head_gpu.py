@@ -550,8 +550,8 @@ def test_head_in_two_captured_graphs(dt):
     def step(rng):
         h, last, st = ops.gated_recurrence(gate, x, h0, save=True)
         y = ops.dropout(h, 0.2, rng)
-        loss, nll, rows, stat = ops.linear_ce(y.reshape(-1, Cc), w, labels, temperature=0.5)
-        gy, gw = ops.linear_ce_bwd(y.reshape(-1, Cc), w, rows, stat, one, temperature=0.5)
+        loss, nll, saved = ops.linear_ce(y.reshape(-1, Cc), w, labels, temperature=0.5)
+        gy, gw = ops.linear_ce_bwd(y.reshape(-1, Cc), w, saved, one, temperature=0.5)
         gg, gx, gh0 = ops.gated_recurrence_bwd(gate, x, None, st, ops.dropout(gy, 0.2, rng).reshape(B, T, Cc), last)
         return loss, nll, gw, gg, gx, gh0
     rngs = [torch.tensor([5, i], device="cuda") for i in range(2)]
