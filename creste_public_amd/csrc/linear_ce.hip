@@ -11,6 +11,9 @@
 // LDS.  Operands arrive by 16-byte LDS-DMA in the order they have in memory.  Where the contraction runs along memory, fragments
 // are plain 16-byte reads; where it runs across (w in DX, both in DW) they are transposing 8-byte reads, so no operand is ever
 // stored transposed.  Both layouts are swizzled in 16-byte chunks (on the global address of the DMA, whose LDS side is fixed).
+// A row's softmax is kept as (maximum, rest): sum of exponentials = exp(maximum) (1 + rest).  For fp32 features the maximum's own term
+// is left out of `rest` exactly, differences to the maximum are taken before scaling, and the label's entry of G is expm1(-nll): a
+// confident row (rest << 1) keeps its loss and gradient to a few 2^-24 instead of 2^-24 / rest.
 // Precision.  16-bit features enter as they are, fp32 features as two fp16 pieces under one power-of-two scale per tensor
 // (22 significand bits; three products hi*hi + hi*lo + lo*hi, error <= 2^-21 of |x||w|).  Accumulation, the softmax statistics and
 // the sums over splits are fp32.  G is rounded once to the operand type (bf16: 2^-8; fp16: 2^-11 relative, scaled by 2^14 so that
@@ -52,8 +55,11 @@ struct CeArgs {
   float2* part;                     // LOSS: [class tile][n] (max, sum) in log2 units
   float* zlab;                      // LOSS: [n] label logit, log2 units
   unsigned* done;                   // LOSS: the joining kernel's counter, cleared here
-  const float* row_l2;              // GRAD, DX, DW: [rows64] log-sum-exp minus log2 of G's scale, infinity where a row does not count
-  const int* row_lab;               // [rows64] label, -1 where none applies
+  // GRAD, DX, DW, per row (padded to 64).  16-bit features: row_l2 = log-sum-exp (log2 units) minus log2 of G's scale, infinity where a
+  // row does not count.  fp32: row_l2 = the maximum (log2 units, rounded), row_rest = what is left of the log-sum-exp, with the maximum's
+  // rounding, minus log2 of G's scale, or infinity, and row_g = the label's entry of G
+  const float *row_l2, *row_rest, *row_g;
+  const int* row_lab;               // label, -1 where none applies
   char* g;                          // GRAD: [n64][ldg] elements, pieces pg bytes apart
   int64_t ldg, pg;
   int n64;
@@ -83,6 +89,13 @@ __device__ __forceinline__ float ce_out_scale(const CeArgs& p) {
   float s = p.gl[0] * p.inv_tau;
   if (p.mean) s = s / fmaxf(p.stat[1], 1.f);
   return s * (ce_operand_inv(p.amax, p.which) / p.gscale);
+}
+
+// join two (maximum, rest); c2: log2 units per unit of the maximum.  (-3e38, -1) is the empty sum
+__device__ __forceinline__ float2 ce_merge(float2 a, float2 b, float c2) {
+  const bool first = a.x >= b.x;
+  const float2 u = first ? a : b, v = first ? b : a;
+  return make_float2(u.x, u.y + (1.f + v.y) * __builtin_amdgcn_exp2f((v.x - u.x) * c2));
 }
 
 template <int DT>
@@ -306,6 +319,7 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
     const int mw = m0 + wm * WTM;                       // first class of this wave, within the piece
     if constexpr (MODE == CE_LOSS) {
       float2* sh = reinterpret_cast<float2*>(smem);     // [wm][BN rows]
+      const float cm = P == 2 ? c2 : 1.f;               // the maximum's unit: raw products (fp32) or log2
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int row = n0 + wn * WTN + j * 32 + li;
@@ -331,26 +345,35 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) z = i * 32 + (r & 3) + 8 * (r >> 2) + 4 * lh == lab ? acc[i][j][r] : z;
         }
-        mx = fmaxf(mx * c2, -3.0e38f);                  // (a half tile without classes has no maximum)
+        float2 st;                                      // (a half tile without classes: the empty sum)
+        if constexpr (P == 2) {
+          mx = fmaxf(mx, -3.0e38f);
+          float cnt = 0.f;
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+          for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c2, -mx));
-        const float mo = __shfl_xor(mx, 32, 64), so = __shfl_xor(sum, 32, 64);
-        const float mm = fmaxf(mx, mo);
-        sum = sum * __builtin_amdgcn_exp2f(mx - mm) + so * __builtin_amdgcn_exp2f(mo - mm);
-        if (lh == 0) sh[wm * BN + wn * WTN + j * 32 + li] = make_float2(mm, sum);
-        if (lab >= 0 && ((lab >> 2) & 1) == lh) p.zlab[row] = z * c2;
+            for (int r = 0; r < 16; ++r) {
+              const float t = acc[i][j][r] - mx;
+              sum += t == 0.f ? 0.f : __builtin_amdgcn_exp2f(t * c2);
+              cnt += t == 0.f ? 1.f : 0.f;
+            }
+          st = make_float2(mx, sum + (cnt - 1.f));
+        } else {
+          mx = fmaxf(mx * c2, -3.0e38f);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c2, -mx));
+          st = make_float2(mx, sum - 1.f);
+        }
+        st = ce_merge(st, make_float2(__shfl_xor(st.x, 32, 64), __shfl_xor(st.y, 32, 64)), cm);
+        if (lh == 0) sh[wm * BN + wn * WTN + j * 32 + li] = st;
+        if (lab >= 0 && ((lab >> 2) & 1) == lh) p.zlab[row] = P == 2 ? z : z * c2;
       }
       __syncthreads();
       const int i = threadIdx.x;
       static_assert(S::WM == 2, "");
-      if (i < BN && n0 + i < p.n) {
-        const float2 u = sh[i], v = sh[BN + i];
-        const float mm = fmaxf(u.x, v.x);
-        p.part[(int64_t)tm * p.n + n0 + i] =
-            make_float2(mm, u.y * __builtin_amdgcn_exp2f(u.x - mm) + v.y * __builtin_amdgcn_exp2f(v.x - mm));
-      }
+      if (i < BN && n0 + i < p.n) p.part[(int64_t)tm * p.n + n0 + i] = ce_merge(sh[i], sh[BN + i], cm);
     } else {
       constexpr int RB = WTM * 2;
       static_assert(RB == 256 && NW * P * 32 * RB <= NS * STAGE, "");
@@ -359,6 +382,7 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
       for (int j = 0; j < NT; ++j) {
         const int row = n0 + wn * WTN + j * 32 + li;
         const float l2 = row < p.n64 ? p.row_l2[row] : INFINITY;
+        const float rest = P == 2 && row < p.n64 ? p.row_rest[row] : 0.f, gl = P == 2 && row < p.n64 ? p.row_g[row] : 0.f;
         const int yr = (row < p.n64 ? p.row_lab[row] : -1) - p.class0 - mw;
         const bool any = __any(yr >= 0 && yr < WTM);
 #pragma unroll
@@ -369,8 +393,10 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
             ces4 hi, lo;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float v = __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * q + e], c2, -l2));
-              if (any) v = cl + e == yr ? v - p.gscale : v;
+              const float z = acc[i][j][4 * q + e];
+              float v = fmaf(z, c2, -l2);
+              v = __builtin_amdgcn_exp2f(P == 2 ? v - rest : v);
+              if (any) v = cl + e == yr ? (P == 2 ? gl : v - p.gscale) : v;
               if (mw + WTM > p.m) v = mw + cl + e < p.m ? v : 0.f;
               const short h = ce_cvt<DT>(v);
               hi[e] = h;
@@ -458,12 +484,13 @@ struct CeStream {
     }
     return v;
   }
-  // DW: the rows' log-sum-exps (even waves) and labels (odd waves: every wave issues as many loads) behind the features
+  // DW: what a row brings along, behind the features (every wave issues as many loads: some twice)
   static __device__ __forceinline__ void dma_info(char* lds, const CeArgs& p, int64_t o0, int wave, int lane) {
     static_assert(OTS == 64, "one 4-byte load per lane");
-    const char* src = wave & 1 ? (const char*)p.row_lab : (const char*)p.row_l2;
+    const int which = P == 2 ? wave & 3 : wave & 1;
+    const char* src = which == 3 ? (const char*)p.row_g : which == 2 ? (const char*)p.row_rest : which ? (const char*)p.row_lab : (const char*)p.row_l2;
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + (o0 + lane) * 4),
-                                     (__attribute__((address_space(3))) void*)(lds + INFO + (wave & 1) * 256), 4, 0, 0);
+                                     (__attribute__((address_space(3))) void*)(lds + INFO + which * 256), 4, 0, 0);
   }
 };
 
@@ -508,13 +535,14 @@ __global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
       for (int kk = 0; kk < KS; ++kk) x[q][j][kk] = *reinterpret_cast<const ces8*>(p.b + q * p.pb + row * p.ldb + kk * 32 + lh * 16);
   }
   const float c2 = ce_operand_inv(p.amax, 0) * ce_operand_inv(p.amax, 1) * p.inv_tau * kCeLog2e;
-  float l2[NT], mx[NT], sum[NT], zl[NT];
+  float l2[NT], rest[NT], gl[NT], mx[NT], sum[NT], zl[NT];
   int lab[NT];                               // LOSS / DX: the row's label; DW: the own class
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int o = own0 + j * 32 + li;
     mx[j] = -3.0e38f;
-    sum[j] = zl[j] = l2[j] = 0.f;
+    sum[j] = P == 2 ? -1.f : 0.f;             // (P == 2: rest)
+    zl[j] = l2[j] = rest[j] = gl[j] = 0.f;
     lab[j] = o;
     if constexpr (MODE == CE_LOSS) {
       const int64_t y = o < p.n ? p.labels[o] : -1;
@@ -522,6 +550,10 @@ __global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
     }
     if constexpr (MODE == CE_DX) {
       l2[j] = o < p.n ? p.row_l2[o] : INFINITY;
+      if constexpr (P == 2) {
+        rest[j] = o < p.n ? p.row_rest[o] : 0.f;
+        gl[j] = o < p.n ? p.row_g[o] : 0.f;
+      }
       lab[j] = o < p.n ? p.row_lab[o] : -1;
     }
   }
@@ -590,35 +622,54 @@ __global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
           float m = z[j][0];
 #pragma unroll
           for (int r = 1; r < 16; ++r) m = fmaxf(m, z[j][r]);
-          m = fmaxf(mx[j], m * c2);
-          sum[j] *= __builtin_amdgcn_exp2f(mx[j] - m);
-          mx[j] = m;
           float s4[4] = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (P == 2) {
+            m = fmaxf(mx[j], m);
+            float cnt = m > mx[j] ? -1.f : 0.f;         // a new maximum's own term stays out of the rest
+            sum[j] = m > mx[j] ? (1.f + sum[j]) * __builtin_amdgcn_exp2f((mx[j] - m) * c2) : sum[j];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s4[r & 3] += __builtin_amdgcn_exp2f(fmaf(z[j][r], c2, -m));
+            for (int r = 0; r < 16; ++r) {
+              const float t = z[j][r] - m;
+              s4[r & 3] += t == 0.f ? 0.f : __builtin_amdgcn_exp2f(t * c2);
+              cnt += t == 0.f ? 1.f : 0.f;
+            }
+            sum[j] += cnt;
+          } else {
+            m = fmaxf(mx[j], m * c2);
+            sum[j] *= __builtin_amdgcn_exp2f(mx[j] - m);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s4[r & 3] += __builtin_amdgcn_exp2f(fmaf(z[j][r], c2, -m));
+          }
+          mx[j] = m;
           sum[j] += (s4[0] + s4[1]) + (s4[2] + s4[3]);
         } else {
           float v[16];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            cef4 rl;
+            cef4 rl, rr, rg;
             cei4 rb;
             if constexpr (MODE == CE_DW) {              // of the others, which are rows here (padded to whole stages)
               rl = *reinterpret_cast<const cef4*>(st + L::INFO + (sub * 32 + 8 * q + 4 * lh) * 4);
               rb = *reinterpret_cast<const cei4*>(st + L::INFO + 256 + (sub * 32 + 8 * q + 4 * lh) * 4);
+              if constexpr (P == 2) {
+                rr = *reinterpret_cast<const cef4*>(st + L::INFO + 512 + (sub * 32 + 8 * q + 4 * lh) * 4);
+                rg = *reinterpret_cast<const cef4*>(st + L::INFO + 768 + (sub * 32 + 8 * q + 4 * lh) * 4);
+              }
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = 4 * q + e;
-              v[r] = __builtin_amdgcn_exp2f(fmaf(z[j][r], c2, MODE == CE_DW ? -rl[e] : -l2[j]));
-              if constexpr (MODE == CE_DW) v[r] = rb[e] == lab[j] ? v[r] - p.gscale : v[r];
+              const float a = MODE == CE_DW ? rl[e] : l2[j];
+              const float u = fmaf(z[j][r], c2, -a);
+              v[r] = __builtin_amdgcn_exp2f(P == 2 ? u - (MODE == CE_DW ? rr[e] : rest[j]) : u);
+              if constexpr (MODE == CE_DW) v[r] = rb[e] == lab[j] ? (P == 2 ? rg[e] : v[r] - p.gscale) : v[r];
             }
           }
           if constexpr (MODE == CE_DX) {
             const int rel = lab[j] - o0;
             if (__any(rel >= 0 && rel < 32))
 #pragma unroll
-              for (int r = 0; r < 16; ++r) v[r] = (r & 3) + 8 * (r >> 2) + 4 * lh == rel ? v[r] - p.gscale : v[r];
+              for (int r = 0; r < 16; ++r) v[r] = (r & 3) + 8 * (r >> 2) + 4 * lh == rel ? (P == 2 ? gl[j] : v[r] - p.gscale) : v[r];
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
@@ -657,12 +708,11 @@ __global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int row = own0 + j * 32 + li;
-      const float mo = __shfl_xor(mx[j], 32, 64), so = __shfl_xor(sum[j], 32, 64);
-      const float m = fmaxf(mx[j], mo);
-      const float s = sum[j] * __builtin_amdgcn_exp2f(mx[j] - m) + so * __builtin_amdgcn_exp2f(mo - m);
+      const float2 mine = make_float2(mx[j], P == 2 ? sum[j] : sum[j] - 1.f);
+      const float2 m = ce_merge(mine, make_float2(__shfl_xor(mine.x, 32, 64), __shfl_xor(mine.y, 32, 64)), P == 2 ? c2 : 1.f);
       if (row >= p.n) continue;
-      if (lh == 0) p.part[(int64_t)split * p.n + row] = make_float2(m, s);
-      if (lab[j] >= kb && lab[j] < ke && ((lab[j] >> 2) & 1) == lh) p.zlab[row] = zl[j] * c2;
+      if (lh == 0) p.part[(int64_t)split * p.n + row] = m;
+      if (lab[j] >= kb && lab[j] < ke && ((lab[j] >> 2) & 1) == lh) p.zlab[row] = P == 2 ? zl[j] : zl[j] * c2;
     }
   } else {
     __syncthreads();
@@ -745,25 +795,30 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeArgs p, int D) {
       z = cl == lab ? acc[i][r] : z;
       mx = fmaxf(mx, acc[i][r]);
     }
-  mx = fmaxf(mx * c2, -3.0e38f);
+  constexpr bool F = DT == CRESTE_DT_F32;
+  mx = fmaxf(F ? mx : mx * c2, -3.0e38f);
+  float cnt = -1.f;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][r], c2, -mx));
-  const float mo = __shfl_xor(mx, 32, 64), so = __shfl_xor(sum, 32, 64);
-  float mm = fmaxf(mx, mo);
-  sum = sum * __builtin_amdgcn_exp2f(mx - mm) + so * __builtin_amdgcn_exp2f(mo - mm);
-  if (lh == 0) sh[wave][li] = make_float2(mm, sum);
-  if (lab >= 0 && ((lab >> 2) & 1) == lh) p.zlab[li] = z * c2;
+    for (int r = 0; r < 16; ++r) {
+      const float t = acc[i][r] - mx;
+      if constexpr (F) {
+        sum += t == 0.f ? 0.f : __builtin_amdgcn_exp2f(t * c2);
+        cnt += t == 0.f ? 1.f : 0.f;
+      } else {
+        sum += __builtin_amdgcn_exp2f(fmaf(acc[i][r], c2, -mx));
+      }
+    }
+  const float cm = F ? c2 : 1.f;
+  float2 st = make_float2(mx, sum + cnt);
+  st = ce_merge(st, make_float2(__shfl_xor(st.x, 32, 64), __shfl_xor(st.y, 32, 64)), cm);
+  if (lh == 0) sh[wave][li] = st;
+  if (lab >= 0 && ((lab >> 2) & 1) == lh) p.zlab[li] = F ? z : z * c2;
   __syncthreads();
   if (threadIdx.x < 32 && (int)threadIdx.x < p.n) {
-    for (int j = 1; j < 4; ++j) {
-      const float2 v = sh[j][li];
-      const float m = fmaxf(mm, v.x);
-      sum = sum * __builtin_amdgcn_exp2f(mm - m) + v.y * __builtin_amdgcn_exp2f(v.x - m);
-      mm = m;
-    }
-    p.part[(int64_t)blockIdx.x * p.n + li] = make_float2(mm, sum);
+    for (int j = 1; j < 4; ++j) st = ce_merge(st, sh[j][li], cm);
+    p.part[(int64_t)blockIdx.x * p.n + li] = st;
   }
 }
 
@@ -837,47 +892,43 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int co
   }
 }
 
-// per row: join the class tiles' (max, sum); 64 rows x 16 slices of the tiles per block.  Leaves nll, what the gradient kernels ask of a
-// row (padded to whole tiles: rows that do not count get an infinite log-sum-exp, hence G = 0, a label that names no class a NaN), and,
-// from the last block to finish, the loss: sums of the blocks' sums in their order, so the result does not depend on which that was
+// per row: join the class tiles' (maximum, rest); 64 rows x 16 slices of the tiles per block.  Leaves nll, what the gradient kernels ask
+// of a row (padded to whole tiles: rows that do not count get an infinite log-sum-exp, hence G = 0, a label that names no class a
+// NaN), and, from the last block to finish, the loss: sums of the blocks' sums in their order, so the result does not depend on which
+// that was.  raw: maxima and label logits in the units of the products (fp32 features), scaled here
 __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ part, int tiles, int n, const float* __restrict__ zlab,
-                                                       const int64_t* __restrict__ labels, int64_t ignore, int classes,
-                                                       float log2_scale, float* __restrict__ nll, float* __restrict__ row_l2,
-                                                       int* __restrict__ row_lab, uint64_t* __restrict__ bsum, unsigned* __restrict__ done,
-                                                       int mean, float* __restrict__ loss, float* __restrict__ stat) {
+                                                       const int64_t* __restrict__ labels, int64_t ignore, int classes, int raw,
+                                                       const float* __restrict__ amax, float inv_tau, float log2_scale,
+                                                       float* __restrict__ nll, float* __restrict__ rows, uint64_t* __restrict__ bsum,
+                                                       unsigned* __restrict__ done, int mean, float* __restrict__ loss,
+                                                       float* __restrict__ stat) {
   __shared__ float2 sh[16][64];
   __shared__ bool last;
   const int li = threadIdx.x & 63, sl = threadIdx.x >> 6;
-  const int row = blockIdx.x * 64 + li;
-  float mx = -3.0e38f, sum = 0.f;
+  const int row = blockIdx.x * 64 + li, n64 = gridDim.x * 64;
+  const float c2 = raw ? ce_operand_inv(amax, 0) * ce_operand_inv(amax, 1) * inv_tau * kCeLog2e : 1.f;   // (as the loss kernel)
+  float2 st = make_float2(-3.0e38f, -1.f);
   if (row < n)
 #pragma unroll 4
-    for (int t = sl; t < tiles; t += 16) {
-      const float2 v = part[(int64_t)t * n + row];
-      const float m = fmaxf(mx, v.x);
-      sum = sum * __builtin_amdgcn_exp2f(mx - m) + v.y * __builtin_amdgcn_exp2f(v.x - m);
-      mx = m;
-    }
-  sh[sl][li] = make_float2(mx, sum);
+    for (int t = sl; t < tiles; t += 16) st = ce_merge(st, part[(int64_t)t * n + row], c2);
+  sh[sl][li] = st;
   __syncthreads();
   if (sl == 0) {
-    for (int s = 1; s < 16; ++s) {
-      const float2 v = sh[s][li];
-      const float m = fmaxf(mx, v.x);
-      sum = sum * __builtin_amdgcn_exp2f(mx - m) + v.y * __builtin_amdgcn_exp2f(v.x - m);
-      mx = m;
-    }
+    for (int s = 1; s < 16; ++s) st = ce_merge(st, sh[s][li], c2);
     float l = 0.f, c = 0.f;
     const int64_t y = row < n ? labels[row] : ignore;
     const bool on = row < n && y != ignore, ok = y >= 0 && y < classes;
-    const float z = mx + __builtin_amdgcn_logf(sum);
+    const float lr = log1pf(st.y);
     if (on) {
-      l = ok ? (z - zlab[row]) * kCeLn2 : __builtin_nanf("");
+      l = ok ? (st.x - zlab[row]) * c2 * kCeLn2 + lr : __builtin_nanf("");
       c = 1.f;
     }
     if (row < n) nll[row] = l;
-    row_l2[row] = !on ? INFINITY : ok ? z - log2_scale : __builtin_nanf("");
-    row_lab[row] = on && ok ? (int)y : -1;
+    const float m2 = st.x * c2, rest = (lr * kCeLog2e + fmaf(st.x, c2, -m2)) - log2_scale;
+    rows[row] = !on ? (raw ? 0.f : INFINITY) : !ok ? __builtin_nanf("") : raw ? m2 : m2 + rest;
+    reinterpret_cast<int*>(rows)[n64 + row] = on && ok ? (int)y : -1;
+    rows[2 * n64 + row] = !raw ? 0.f : on ? rest : INFINITY;
+    rows[3 * n64 + row] = raw && on ? expm1f(-l) * exp2f(log2_scale) : 0.f;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       l += __shfl_xor(l, o, 64);
@@ -1196,9 +1247,9 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
     if (rg) return rg;
   }
   const int nb = cdiv(N, 64);
-  ce_join_kernel<<<nb, 1024, 0, s>>>(a.part, q.stream && !few ? q.sl : q.tiles, (int)N, a.zlab, labels, ignore_index, (int)V,
-                                     ce_gscale_log2(q), nll, rows, (int*)(rows + up(N, 64)), (uint64_t*)(wk + q.bsum), a.done, mean,
-                                     loss, stat);
+  ce_join_kernel<<<nb, 1024, 0, s>>>(a.part, q.stream && !few ? q.sl : q.tiles, (int)N, a.zlab, labels, ignore_index, (int)V, q.P == 2,
+                                     few ? nullptr : a.amax, a.inv_tau, ce_gscale_log2(q), nll, rows, (uint64_t*)(wk + q.bsum), a.done,
+                                     mean, loss, stat);
   CRESTE_CHECK_LAUNCH("linear_ce join");
   return CRESTE_OK;
 }
@@ -1222,7 +1273,7 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
   c.amax = q.P == 2 ? (const float*)(wk + q.amax) : nullptr;
   c.stat = stat; c.gl = g_loss; c.mean = mean;
   c.gscale = exp2f(ce_gscale_log2(q));
-  c.row_l2 = rows; c.row_lab = (const int*)(rows + q.n64);
+  c.row_l2 = rows; c.row_lab = (const int*)(rows + q.n64); c.row_rest = rows + 2 * q.n64; c.row_g = rows + 3 * q.n64;
   c.n64 = (int)q.n64;
   c.out_dt = dtype;
   c.ldo = c.m_out = D;

@@ -1644,7 +1644,7 @@ def _linear_ce_args(x, w, temperature, reduction):
 
 
 def _ce_saved(N: int) -> int:
-    return 4 + 2 * (-(-N // 64) * 64)          # {sum, count, -, -}, [2][N rounded up to 64]
+    return 4 + 4 * (-(-N // 64) * 64)          # {sum, count, -, -}, [4][N rounded up to 64]
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -1653,7 +1653,7 @@ def _row_stride(t: torch.Tensor) -> int:
 
 def linear_ce(x, w, labels, ignore_index: int = -100, temperature: float = 1.0, reduction: str = "mean"):
     """forward of loss_ops.linear_cross_entropy for x [N,D] -> (loss [], nll [N], saved), fp32; `saved` is what linear_ce_bwd needs of it
-    (sum and count, then two words per row)"""
+    (sum and count, then four words per row)"""
     code, x_, w_ = _linear_ce_args(x, w, temperature, reduction)
     N, D = x_.shape
     V, dev = w_.shape[0], x_.device

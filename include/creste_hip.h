@@ -703,7 +703,7 @@ int creste_irl_visitation_mix_f32(const float* exp_svf_raw, const uint8_t* fov, 
  * w [V][ldw] (strides in elements, D of them used), labels [N] int64; a row whose label is ignore_index does not count, one whose
  * label names no class makes loss and gradients NaN.  No N x V buffer.
  *   forward : loss [1] (mean over the counted rows, 0 if there are none, or sum), nll [N] (0 where ignored), and for the backward
- *             rows [2][N rounded up to 64] 4-byte words (scaled log-sum-exps; labels) and stat [2] = {sum nll, count}.
+ *             rows [4][N rounded up to 64] 4-byte words (log-sum-exps, labels) and stat [2] = {sum nll, count}.
  *   backward: gx [N][D], gw [V][D] (contiguous, the features' type; either may be NULL) for the cotangent g_loss [1].
  * work: workspace_bytes(..., train = 0) for the forward, train = 1 for the backward; -1 = sizes out of range. */
 int64_t creste_linear_ce_workspace_bytes(int64_t N, int64_t V, int D, int dtype, int train);
