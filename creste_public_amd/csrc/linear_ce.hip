@@ -44,7 +44,7 @@ struct CeArgs {
   int ca, cb;                       // bytes of a memory row that exist (transposed operands: loads clamp to the last 16)
   int m, n;                         // extents of the output
   int mt, nt;                       // tiles along m, n
-  int k0, k1, ksplit;               // contraction range; ksplit > 0: split s works [k0 + s * ksplit, + ksplit)
+  int k1, ksplit;                   // contraction length; ksplit > 0: split s works [s * ksplit, + ksplit)
   // LOSS / GRAD
   const int64_t* labels;
   int64_t ignore;
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
   t /= p.mt;
   const int tn = t % p.nt, split = t / p.nt;
   const int m0 = tm * BM, n0 = tn * BN;
-  const int kb = p.k0 + split * p.ksplit;
+  const int kb = split * p.ksplit;
   const int ke = p.ksplit ? min(p.k1, kb + p.ksplit) : p.k1;
 
   cef16 acc[MT][NT];
@@ -1221,6 +1221,7 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
   const CePlan q = ce_plan(N, V, D, dtype, !few && !ce_direct(x, ldx, D, dtype), !few && !ce_direct(w, ldw, D, dtype), false);
   CRESTE_REQUIRE(loss && nll && rows && stat && work && work_bytes >= q.total, "linear_ce_forward: outputs / workspace (%lld of %lld bytes)",
                  (long long)work_bytes, (long long)q.total);
+  CRESTE_REQUIRE(((uintptr_t)work & 15) == 0, "linear_ce_forward: work on a 16-byte boundary");
   hipStream_t s = (hipStream_t)stream;
   char* wk = (char*)work;
   CeOperand X{(const char*)x, ldx * q.es, 0}, W{(const char*)w, ldw * q.es, 0};
@@ -1262,6 +1263,7 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
   const CePlan q = ce_plan(N, V, D, dtype, !ce_direct(x, ldx, D, dtype), !ce_direct(w, ldw, D, dtype), true);
   CRESTE_REQUIRE(stat && g_loss && (gx || gw) && work && work_bytes >= q.total, "linear_ce_backward: inputs / workspace (%lld of %lld bytes)",
                  (long long)work_bytes, (long long)q.total);
+  CRESTE_REQUIRE((((uintptr_t)gx | (uintptr_t)gw | (uintptr_t)work) & 15) == 0, "linear_ce_backward: gx, gw and work on 16-byte boundaries");
   hipStream_t s = (hipStream_t)stream;
   char* wk = (char*)work;
   CeOperand X, W;

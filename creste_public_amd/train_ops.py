@@ -609,8 +609,15 @@ def reward_forward_train(net, x: torch.Tensor) -> torch.Tensor:
 
 
 def recorded(*tensors) -> bool:
-    """does autograd record an operation on these (else the Function around it is only overhead)"""
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+    """does autograd record an operation on these (else the Function around it is only overhead).  Not inside a stream capture: a
+    captured backward whose leaves also belong to a live eager graph ties the capture to the eager stream and ends the process, and
+    whether such a graph lives cannot be seen from here.  A captured step calls the two halves in `ops` itself."""
+    if not torch.is_grad_enabled() or not any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        return False
+    if any(isinstance(t, torch.Tensor) and t.is_cuda for t in tensors) and torch.cuda.is_current_stream_capturing():
+        raise HipLibraryError("autograd under stream capture: capture the forward and backward entry points of creste_public_amd.ops "
+                              "(dropout, gated_recurrence / _bwd, linear_ce / _bwd), under torch.no_grad() or on detached tensors")
+    return True
 
 
 def once(fn):
@@ -645,7 +652,7 @@ class DropoutFn(torch.autograd.Function):
 
 def dropout(x, p: float, seed, offset: int = 0, residual=None):
     """y = x / (1 - p) where an element is kept, else 0 (+ residual); see ops.dropout for what decides.  Differentiable in x and
-    residual.  fp32 / bf16 / fp16, any shape."""
+    residual, as often as wanted.  fp32 / bf16 / fp16, any shape.  Not recorded inside a stream capture: see `recorded`."""
     return (DropoutFn.apply if recorded(x, residual) else ops.dropout)(x, p, seed, offset, residual)
 
 
@@ -675,5 +682,6 @@ class GatedRecurrenceFn(torch.autograd.Function):
 
 def gated_recurrence(gate, x, h0=None, lengths=None):
     """h_t = f_t h_(t-1) + (1 - f_t) x_t, f = sigmoid(gate), over [B,T,C] sequences -> (h [B,T,C], h_last [B,C] fp32); arguments as
-    ops.gated_recurrence.  Differentiable in gate, x and h0, through both outputs."""
+    ops.gated_recurrence.  Differentiable (once) in gate, x and h0, through both outputs.  Not recorded inside a stream capture: see
+    `recorded`."""
     return (GatedRecurrenceFn.apply if recorded(gate, x, h0) else ops.gated_recurrence)(gate, x, h0, lengths)

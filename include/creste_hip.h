@@ -704,8 +704,8 @@ int creste_irl_visitation_mix_f32(const float* exp_svf_raw, const uint8_t* fov, 
  * label names no class makes loss and gradients NaN.  No N x V buffer.
  *   forward : loss [1] (mean over the counted rows, 0 if there are none, or sum), nll [N] (0 where ignored), and for the backward
  *             rows [4][N rounded up to 64] 4-byte words (log-sum-exps, labels) and stat [2] = {sum nll, count}.
- *   backward: gx [N][D], gw [V][D] (contiguous, the features' type; either may be NULL) for the cotangent g_loss [1].
- * work: workspace_bytes(..., train = 0) for the forward, train = 1 for the backward; -1 = sizes out of range. */
+ *   backward: gx [N][D], gw [V][D] (contiguous, 16-byte aligned, the features' type; either may be NULL) for the cotangent g_loss [1].
+ * work (16-byte aligned): workspace_bytes(..., train = 0) for the forward, train = 1 for the backward; -1 = sizes out of range. */
 int64_t creste_linear_ce_workspace_bytes(int64_t N, int64_t V, int D, int dtype, int train);
 int creste_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* labels, int64_t N, int64_t V,
                              int D, int dtype, int64_t ignore_index, float temperature, int mean, float* loss, float* nll,

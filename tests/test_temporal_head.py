@@ -70,6 +70,9 @@ def test_entry_points_report_bad_arguments():
     err(fwd(nb=1000), b"workspace")
     err(fwd(work=None), b"workspace")
     err(lib.creste_linear_ce_backward(p, 16, p, 16, p, 4, 8, 16, 0, 1.0, 1, p, p, None, None, p, 1 << 40, None), b"inputs")
+    odd = C.c_void_p(4104)
+    err(fwd(work=odd), b"16-byte")
+    err(lib.creste_linear_ce_backward(p, 16, p, 16, p, 4, 8, 16, 0, 1.0, 1, p, p, odd, None, p, 1 << 40, None), b"16-byte")
     for bad in ((0, 8, 16, 0), (4, 0, 16, 0), (4, 8, 0, 0), (4, 8, 16, 5), (1 << 31, 8, 16, 0)):
         assert lib.creste_linear_ce_workspace_bytes(*bad, 1) == -1
 

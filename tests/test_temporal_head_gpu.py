@@ -461,6 +461,71 @@ def test_linear_ce_beyond_32_bits():
     within(gx, (p @ w[rows].detach().double()).cpu(), (2.0 ** -7 * p.abs() @ w[rows].detach().double().abs()).cpu(), "dx")
 
 
+def test_linear_ce_streamed_beyond_32_bits():
+    """the same for up to 256 feature columns, on either side of the products"""
+    V, D, N = 9000000, 256, 70
+    w = torch.zeros(V, D, dtype=BF16, device="cuda")
+    rows = torch.tensor([0, 1, V - 2, V - 1], device="cuda")
+    w[rows] = torch.randn(4, D, generator=gen(4)).to(BF16).cuda()
+    lab = rows[torch.arange(N, device="cuda") % 4]
+    xa = (w[lab] / 32).requires_grad_(True)
+    wa = w.requires_grad_(True)
+    loss, nll = loss_ops.linear_cross_entropy(xa, wa, lab, reduction="sum")
+    xd, wd = xa.detach().double(), w[rows].detach().double()
+    z = xd @ wd.t()
+    lse = torch.log(torch.exp(z).sum(1) + (V - 4))
+    bound = torch.full((N,), float(z.abs().max()) * 2 * (D + 16) * O.U32 + 600 * O.U32, dtype=torch.double)
+    within(nll, (lse - z.gather(1, (torch.arange(N, device="cuda") % 4)[:, None])[:, 0]).cpu(), bound, "nll")
+    gx, gw = torch.autograd.grad(loss, (xa, wa))
+    p = torch.exp(z - lse[:, None]) - torch.nn.functional.one_hot(torch.arange(N, device="cuda") % 4, 4)
+    within(gw[rows], (p.t() @ xd).cpu(), (2.0 ** -7 * (p.abs().t() @ xd.abs())).cpu(), "dw")
+    within(gx, (p @ wd).cpu(), (2.0 ** -7 * (p.abs() @ wd.abs())).cpu(), "dx")
+    del wa, w, gw
+    N, V = 9000000, 70                                                # the rows are the long side
+    x = torch.zeros(N, D, dtype=BF16, device="cuda")
+    w = torch.randn(V, D, generator=gen(5)).to(BF16).cuda()
+    at = torch.tensor([0, 1, N - 2, N - 1], device="cuda")
+    lab = torch.full((N,), -100, device="cuda")
+    lab[at] = torch.tensor([3, 69, 0, 68], device="cuda")
+    x[at] = torch.randn(4, D, generator=gen(6)).to(BF16).cuda() / 8
+    xa, wa = x.requires_grad_(True), w.requires_grad_(True)
+    loss, nll = loss_ops.linear_cross_entropy(xa, wa, lab, reduction="sum")
+    gx, gw = torch.autograd.grad(loss, (xa, wa))
+    r = O.linear_ce(x[at].detach(), w.detach(), lab[at], -100, 1.0, False)
+    within(nll[at], r["nll"], r["e_nll"], "nll")
+    within(gx[at], r["gx"], r["e_gx"], "dx")
+    within(gw, r["gw"], r["e_gw"], "dw")
+    assert not gx[2:-2].any() and not nll[2:-2].any()
+
+
+@pytest.mark.parametrize("V", [2, 3, 40])
+def test_linear_ce_confident_rows_f32(V):
+    """the loss of a confident row is about exp(-margin): relative to it, only the margin's absolute error (twice a logit's) and a few
+    roundings count, not the rounding of 1 + exp(-margin).  The same for its gradient, nll (w_other - w_label) in norm"""
+    N, D = 300, 48
+    g = gen(V)
+    w = torch.randn(V, D, generator=g)
+    w = (w / w.norm(dim=1, keepdim=True)).cuda()
+    lab = torch.randint(0, V, (N,), generator=g).cuda()
+    x = w[lab] + 0.05 * torch.randn(N, D, generator=g).cuda()
+    for tau in (0.1, 0.05):
+        r = O.linear_ce(x, w, lab, -100, tau, False)
+        xa, wa = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        loss, nll = loss_ops.linear_cross_entropy(xa, wa, lab, temperature=tau, reduction="sum")
+        gx, gw = torch.autograd.grad(loss, (xa, wa))
+        big = float((x.double().abs() @ w.double().abs().t()).max()) / tau
+        rel = 2 * big * (2.0 ** -21 + (D + 8) * O.U32) + 64 * O.U32
+        assert float(r["nll"].min()) < 1e-2
+        within(nll, r["nll"], rel * r["nll"], "nll")
+        z = x.double().cpu() @ w.double().cpu().t() / tau
+        p = torch.softmax(z, 1)
+        hot = torch.nn.functional.one_hot(lab.cpu(), V).double()
+        other = (p * (1 - hot)).sum(1, keepdim=True)
+        mag = (p * (1 - hot) + other * hot) / tau                     # |G|
+        bound = (rel + 2.0 ** -20 + (V + 64) * O.U32) * (mag @ w.double().cpu().abs()) + O.U32 * r["gx"].abs()
+        within(gx, r["gx"], 1.01 * bound + 2.0 ** -39 / tau * w.double().cpu().abs().sum(0), "dx")
+
+
 def test_linear_ce_gradient_against_differences():
     """central differences with step 2^-5 along unit directions: log-sum-exp's third derivative is below |w|^3 / tau^3 = 1 here and
     the step small, so 2^-10 / 6 of truncation; fp32 losses around 5 (2^-22 each) over 2^-4: 2^-16.  2e-3 absolute holds both"""
@@ -535,6 +600,66 @@ def test_head_forward_and_backward(dt):
         again = step()
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+def test_two_calls_at_once():
+    """the same operators on two streams at the same time (the recurrence's workgroups wait for each other within a call only)"""
+    jobs = []
+    for k in range(2):
+        gate, x, gh, h0, gl = _rec_inputs(4, 3000 + 500 * k, 256, BF16, seed=k)
+        xs, w, lab = _ce_inputs(3000, 2000, 128, BF16, seed=k)
+        jobs.append((gate, x, gh, h0, gl, xs, w, lab))
+
+    def work(j):
+        gate, x, gh, h0, gl, xs, w, lab = j
+        h, last, st = ops.gated_recurrence(gate, x, h0, save=True)
+        back = ops.gated_recurrence_bwd(gate, x, None, st, gh, gl)
+        loss, nll, saved = ops.linear_ce(xs, w, lab, temperature=0.1)
+        return (h, last) + back + (loss, nll) + ops.linear_ce_bwd(xs, w, saved, torch.ones_like(loss), temperature=0.1)
+    want = [[t.clone() for t in work(j)] for j in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for rep in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(work(jobs[i]))
+    torch.cuda.synchronize()
+    for w_, got in zip(want, outs):
+        for o in got:
+            assert all(torch.equal(a, b) for a, b in zip(w_, o))
+
+
+def test_dropout_twice_differentiable():
+    x = torch.randn(300, generator=gen(3)).cuda().requires_grad_(True)
+    y = train_ops.dropout(x, 0.3, 9)
+    g, = torch.autograd.grad((y ** 3).sum(), x, create_graph=True)
+    gg, = torch.autograd.grad(g.sum(), x)
+    k = O.keep_mask(0, 300, 0.3, 9, 0).cuda() / 0.7
+    want = 6 * x.detach().double() * k ** 3
+    within(gg, want.cpu(), (16 * O.U32 * want.abs()).cpu(), "second derivative")
+    gate, xx, gh, h0, gl = _rec_inputs(1, 3, 2, F32)
+    h, _ = train_ops.gated_recurrence(gate.requires_grad_(True), xx, h0)
+    g, = torch.autograd.grad(h.sum(), gate, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+        torch.autograd.grad(g.sum(), gate)
+
+
+def test_autograd_is_refused_inside_a_capture():
+    x = torch.randn(2, 3, 64, device="cuda", requires_grad=True)
+    w, lab = torch.randn(5, 64, device="cuda"), torch.zeros(2, 3, dtype=torch.long, device="cuda")
+    calls = (lambda t: train_ops.dropout(t, 0.5, 1), lambda t: train_ops.gated_recurrence(t, t), lambda t: loss_ops.linear_cross_entropy(t, w, lab))
+    for f in calls:
+        f(x.detach())
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for f in calls:
+            with pytest.raises(E, match="under stream capture"):
+                f(x)
+            f(x.detach())
+    g.replay()
+    torch.cuda.synchronize()
 
 
 @pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
