@@ -2,7 +2,8 @@
 //   word_i = Philox4x32-10(counter = (i div 4, offset), key = seed)[i mod 4]   (Salmon et al., SC 2011)
 //   y_i = word_i >= round(p 2^32) ? x_i / (1 - p) : 0   (+ residual_i);  the backward is the same call on the cotangent.
 // A dropped element is SELECTED away, so an infinity or NaN there does not reach the output.  fp32 arithmetic, one rounding.
-// Bound: HBM for fp32 (8 bytes per element); for 16-bit types the generator (20 wide multiplies per four elements) comes close.
+// Bound: HBM.  40 M fp32 elements: 53 us, 6.0 TB/s; 34 M bf16 with a residual: 31 us, 6.5 TB/s (part of it from the cache; a large
+// copy: 5.1).  The generator's 20 wide multiplies per four elements stay below that.
 #include "common.h"
 
 namespace creste {
@@ -80,7 +81,8 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropArgs p) {
       vec yv;
 #pragma unroll
       for (int e = 0; e < VE; ++e) yv[e] = (T)a[e];
-      *reinterpret_cast<vec*>(y + i0) = yv;
+      // past the caches: 160 MB fp32 57 -> 53 us, 67 MB bf16 with a residual 34 -> 31 us
+      __builtin_nontemporal_store(yv, reinterpret_cast<vec*>(y + i0));
     } else {
 #pragma unroll
       for (int e = 0; e < VE; ++e)
