@@ -11,9 +11,10 @@
 // LDS.  Operands arrive by 16-byte LDS-DMA in the order they have in memory.  Where the contraction runs along memory, fragments
 // are plain 16-byte reads; where it runs across (w in DX, both in DW) they are transposing 8-byte reads, so no operand is ever
 // stored transposed.  Both layouts are swizzled in 16-byte chunks (on the global address of the DMA, whose LDS side is fixed).
-// A row's softmax is kept as (maximum, rest): sum of exponentials = exp(maximum) (1 + rest).  For fp32 features the maximum's own term
-// is left out of `rest` exactly, differences to the maximum are taken before scaling, and the label's entry of G is expm1(-nll): a
-// confident row (rest << 1) keeps its loss and gradient to a few 2^-24 instead of 2^-24 / rest.
+// A row's softmax is kept as (maximum, rest): sum of exponentials = exp(maximum) (1 + rest).  For fp32 features and for small class sets the
+// maximum's own term is left out of `rest` exactly (a comparison and two selections per logit: 4 % of a training step at 65536 classes,
+// where rows are rarely that sure), so that a confident row (rest << 1) keeps its loss to a few 2^-24 instead of 2^-24 / rest; for fp32
+// features the label's entry of G is expm1(-nll), so its gradient does too.
 // Precision.  16-bit features enter as they are, fp32 features as two fp16 pieces under one power-of-two scale per tensor
 // (22 significand bits; three products hi*hi + hi*lo + lo*hi, error <= 2^-21 of |x||w|).  Accumulation, the softmax statistics and
 // the sums over splits are fp32.  G is rounded once to the operand type (bf16: 2^-8; fp16: 2^-11 relative, scaled by 2^14 so that
@@ -31,6 +32,7 @@ typedef _Float16 ceh8 __attribute__((ext_vector_type(8)));
 typedef __bf16 ceb8 __attribute__((ext_vector_type(8)));
 
 constexpr float kCeLog2e = 1.44269504088896341f, kCeLn2 = 0.693147180559945309f;
+constexpr int kCeExactRest = 1024;            // class sets up to this size: `rest` without the maximum's own term
 constexpr int kCeTile = 256;                 // classes per LOSS / GRAD tile, rows (LOSS, GRAD, DX) or classes (DW) per tile
 constexpr float kCeF16Log2 = 14.f;           // G enters as G * 2^14 where it is fp16
 
@@ -52,8 +54,8 @@ struct CeArgs {
   int classes;                      // all classes
   float inv_tau;
   const float* amax;                // [2] max|x|, max|w| (two-piece operands) or null
-  float2* part;                     // LOSS: [class tile][n] (max, sum) in log2 units
-  float* zlab;                      // LOSS: [n] label logit, log2 units
+  float2* part;                     // LOSS: [class tile][n] (maximum, rest)
+  float* zlab;                      // LOSS: [n] label logit, as maxima in the units of the products
   unsigned* done;                   // LOSS: the joining kernel's counter, cleared here
   // GRAD, DX, DW, per row (padded to 64).  16-bit features: row_l2 = log-sum-exp (log2 units) minus log2 of G's scale, infinity where a
   // row does not count.  fp32: row_l2 = the maximum (log2 units, rounded), row_rest = what is left of the log-sum-exp, with the maximum's
@@ -319,7 +321,6 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
     const int mw = m0 + wm * WTM;                       // first class of this wave, within the piece
     if constexpr (MODE == CE_LOSS) {
       float2* sh = reinterpret_cast<float2*>(smem);     // [wm][BN rows]
-      const float cm = P == 2 ? c2 : 1.f;               // the maximum's unit: raw products (fp32) or log2
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int row = n0 + wn * WTN + j * 32 + li;
@@ -345,35 +346,33 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) z = i * 32 + (r & 3) + 8 * (r >> 2) + 4 * lh == lab ? acc[i][j][r] : z;
         }
-        float2 st;                                      // (a half tile without classes: the empty sum)
-        if constexpr (P == 2) {
-          mx = fmaxf(mx, -3.0e38f);
-          float cnt = 0.f;
+        mx = fmaxf(mx, -3.0e38f);                       // (a half tile without classes: the empty sum)
+        float own = -1.f;                               // the maximum's own term
+        if (P == 2 || p.classes <= kCeExactRest) {
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const float t = acc[i][j][r] - mx;
               sum += t == 0.f ? 0.f : __builtin_amdgcn_exp2f(t * c2);
-              cnt += t == 0.f ? 1.f : 0.f;
+              own += t == 0.f ? 1.f : 0.f;
             }
-          st = make_float2(mx, sum + (cnt - 1.f));
         } else {
-          mx = fmaxf(mx * c2, -3.0e38f);
+          const float m2 = fmaxf(mx * c2, -3.0e38f);
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c2, -mx));
-          st = make_float2(mx, sum - 1.f);
+            for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c2, -m2));
         }
-        st = ce_merge(st, make_float2(__shfl_xor(st.x, 32, 64), __shfl_xor(st.y, 32, 64)), cm);
+        float2 st = make_float2(mx, sum + own);
+        st = ce_merge(st, make_float2(__shfl_xor(st.x, 32, 64), __shfl_xor(st.y, 32, 64)), c2);
         if (lh == 0) sh[wm * BN + wn * WTN + j * 32 + li] = st;
-        if (lab >= 0 && ((lab >> 2) & 1) == lh) p.zlab[row] = P == 2 ? z : z * c2;
+        if (lab >= 0 && ((lab >> 2) & 1) == lh) p.zlab[row] = z;
       }
       __syncthreads();
       const int i = threadIdx.x;
       static_assert(S::WM == 2, "");
-      if (i < BN && n0 + i < p.n) p.part[(int64_t)tm * p.n + n0 + i] = ce_merge(sh[i], sh[BN + i], cm);
+      if (i < BN && n0 + i < p.n) p.part[(int64_t)tm * p.n + n0 + i] = ce_merge(sh[i], sh[BN + i], c2);
     } else {
       constexpr int RB = WTM * 2;
       static_assert(RB == 256 && NW * P * 32 * RB <= NS * STAGE, "");
@@ -535,13 +534,14 @@ __global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
       for (int kk = 0; kk < KS; ++kk) x[q][j][kk] = *reinterpret_cast<const ces8*>(p.b + q * p.pb + row * p.ldb + kk * 32 + lh * 16);
   }
   const float c2 = ce_operand_inv(p.amax, 0) * ce_operand_inv(p.amax, 1) * p.inv_tau * kCeLog2e;
+  const bool exact = P == 2 || p.classes <= kCeExactRest;      // sum: the rest, else with the maximum's own term
   float l2[NT], rest[NT], gl[NT], mx[NT], sum[NT], zl[NT];
   int lab[NT];                               // LOSS / DX: the row's label; DW: the own class
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int o = own0 + j * 32 + li;
     mx[j] = -3.0e38f;
-    sum[j] = P == 2 ? -1.f : 0.f;             // (P == 2: rest)
+    sum[j] = exact ? -1.f : 0.f;
     zl[j] = l2[j] = rest[j] = gl[j] = 0.f;
     lab[j] = o;
     if constexpr (MODE == CE_LOSS) {
@@ -623,22 +623,23 @@ __global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
 #pragma unroll
           for (int r = 1; r < 16; ++r) m = fmaxf(m, z[j][r]);
           float s4[4] = {0.f, 0.f, 0.f, 0.f};
-          if constexpr (P == 2) {
-            m = fmaxf(mx[j], m);
-            float cnt = m > mx[j] ? -1.f : 0.f;         // a new maximum's own term stays out of the rest
-            sum[j] = m > mx[j] ? (1.f + sum[j]) * __builtin_amdgcn_exp2f((mx[j] - m) * c2) : sum[j];
+          m = fmaxf(mx[j], m);
+          const float down = __builtin_amdgcn_exp2f((mx[j] - m) * c2);
+          if (exact) {
+            float own = m > mx[j] ? -1.f : 0.f;         // a new maximum's own term stays out
+            sum[j] = m > mx[j] ? (1.f + sum[j]) * down : sum[j];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const float t = z[j][r] - m;
               s4[r & 3] += t == 0.f ? 0.f : __builtin_amdgcn_exp2f(t * c2);
-              cnt += t == 0.f ? 1.f : 0.f;
+              own += t == 0.f ? 1.f : 0.f;
             }
-            sum[j] += cnt;
+            sum[j] += own;
           } else {
-            m = fmaxf(mx[j], m * c2);
-            sum[j] *= __builtin_amdgcn_exp2f(mx[j] - m);
+            sum[j] *= down;
+            const float m2 = fmaxf(m * c2, -3.0e38f);   // (a half wave's classes may all lie behind the last one)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s4[r & 3] += __builtin_amdgcn_exp2f(fmaf(z[j][r], c2, -m));
+            for (int r = 0; r < 16; ++r) s4[r & 3] += __builtin_amdgcn_exp2f(fmaf(z[j][r], c2, -m2));
           }
           mx[j] = m;
           sum[j] += (s4[0] + s4[1]) + (s4[2] + s4[3]);
@@ -708,11 +709,11 @@ __global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int row = own0 + j * 32 + li;
-      const float2 mine = make_float2(mx[j], P == 2 ? sum[j] : sum[j] - 1.f);
-      const float2 m = ce_merge(mine, make_float2(__shfl_xor(mine.x, 32, 64), __shfl_xor(mine.y, 32, 64)), P == 2 ? c2 : 1.f);
+      const float2 mine = make_float2(mx[j], exact ? sum[j] : sum[j] - 1.f);
+      const float2 m = ce_merge(mine, make_float2(__shfl_xor(mine.x, 32, 64), __shfl_xor(mine.y, 32, 64)), c2);
       if (row >= p.n) continue;
       if (lh == 0) p.part[(int64_t)split * p.n + row] = m;
-      if (lab[j] >= kb && lab[j] < ke && ((lab[j] >> 2) & 1) == lh) p.zlab[row] = P == 2 ? zl[j] : zl[j] * c2;
+      if (lab[j] >= kb && lab[j] < ke && ((lab[j] >> 2) & 1) == lh) p.zlab[row] = zl[j];
     }
   } else {
     __syncthreads();
@@ -795,29 +796,23 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeArgs p, int D) {
       z = cl == lab ? acc[i][r] : z;
       mx = fmaxf(mx, acc[i][r]);
     }
-  constexpr bool F = DT == CRESTE_DT_F32;
-  mx = fmaxf(F ? mx : mx * c2, -3.0e38f);
-  float cnt = -1.f;
+  mx = fmaxf(mx, -3.0e38f);
+  float own = -1.f;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const float t = acc[i][r] - mx;
-      if constexpr (F) {
-        sum += t == 0.f ? 0.f : __builtin_amdgcn_exp2f(t * c2);
-        cnt += t == 0.f ? 1.f : 0.f;
-      } else {
-        sum += __builtin_amdgcn_exp2f(fmaf(acc[i][r], c2, -mx));
-      }
+      sum += t == 0.f ? 0.f : __builtin_amdgcn_exp2f(t * c2);
+      own += t == 0.f ? 1.f : 0.f;
     }
-  const float cm = F ? c2 : 1.f;
-  float2 st = make_float2(mx, sum + cnt);
-  st = ce_merge(st, make_float2(__shfl_xor(st.x, 32, 64), __shfl_xor(st.y, 32, 64)), cm);
+  float2 st = make_float2(mx, sum + own);
+  st = ce_merge(st, make_float2(__shfl_xor(st.x, 32, 64), __shfl_xor(st.y, 32, 64)), c2);
   if (lh == 0) sh[wave][li] = st;
-  if (lab >= 0 && ((lab >> 2) & 1) == lh) p.zlab[li] = F ? z : z * c2;
+  if (lab >= 0 && ((lab >> 2) & 1) == lh) p.zlab[li] = z;
   __syncthreads();
   if (threadIdx.x < 32 && (int)threadIdx.x < p.n) {
-    for (int j = 1; j < 4; ++j) st = ce_merge(st, sh[j][li], cm);
+    for (int j = 1; j < 4; ++j) st = ce_merge(st, sh[j][li], c2);
     p.part[(int64_t)blockIdx.x * p.n + li] = st;
   }
 }
@@ -895,9 +890,9 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int co
 // per row: join the class tiles' (maximum, rest); 64 rows x 16 slices of the tiles per block.  Leaves nll, what the gradient kernels ask
 // of a row (padded to whole tiles: rows that do not count get an infinite log-sum-exp, hence G = 0, a label that names no class a
 // NaN), and, from the last block to finish, the loss: sums of the blocks' sums in their order, so the result does not depend on which
-// that was.  raw: maxima and label logits in the units of the products (fp32 features), scaled here
+// that was.  Maxima and label logits come in the units of the products.  two: fp32 features, the log-sum-exp in two parts
 __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ part, int tiles, int n, const float* __restrict__ zlab,
-                                                       const int64_t* __restrict__ labels, int64_t ignore, int classes, int raw,
+                                                       const int64_t* __restrict__ labels, int64_t ignore, int classes, int two,
                                                        const float* __restrict__ amax, float inv_tau, float log2_scale,
                                                        float* __restrict__ nll, float* __restrict__ rows, uint64_t* __restrict__ bsum,
                                                        unsigned* __restrict__ done, int mean, float* __restrict__ loss,
@@ -906,7 +901,7 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
   __shared__ bool last;
   const int li = threadIdx.x & 63, sl = threadIdx.x >> 6;
   const int row = blockIdx.x * 64 + li, n64 = gridDim.x * 64;
-  const float c2 = raw ? ce_operand_inv(amax, 0) * ce_operand_inv(amax, 1) * inv_tau * kCeLog2e : 1.f;   // (as the loss kernel)
+  const float c2 = ce_operand_inv(amax, 0) * ce_operand_inv(amax, 1) * inv_tau * kCeLog2e;      // (as the loss kernels')
   float2 st = make_float2(-3.0e38f, -1.f);
   if (row < n)
 #pragma unroll 4
@@ -925,10 +920,10 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
     }
     if (row < n) nll[row] = l;
     const float m2 = st.x * c2, rest = (lr * kCeLog2e + fmaf(st.x, c2, -m2)) - log2_scale;
-    rows[row] = !on ? (raw ? 0.f : INFINITY) : !ok ? __builtin_nanf("") : raw ? m2 : m2 + rest;
+    rows[row] = !on ? (two ? 0.f : INFINITY) : !ok ? __builtin_nanf("") : two ? m2 : m2 + rest;
     reinterpret_cast<int*>(rows)[n64 + row] = on && ok ? (int)y : -1;
-    rows[2 * n64 + row] = !raw ? 0.f : on ? rest : INFINITY;
-    rows[3 * n64 + row] = raw && on ? expm1f(-l) * exp2f(log2_scale) : 0.f;
+    rows[2 * n64 + row] = !two ? 0.f : on ? rest : INFINITY;
+    rows[3 * n64 + row] = two && on ? expm1f(-l) * exp2f(log2_scale) : 0.f;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       l += __shfl_xor(l, o, 64);

@@ -321,7 +321,8 @@ def _ce_check(x, w, labels, tau=0.1, ignore=-100, reduction="mean", gl=1.0):
 
 @pytest.mark.parametrize("dt", ALL, ids=IDS)
 @pytest.mark.parametrize("N,V,D", [(1, 1, 1), (1, 2, 8), (2, 3, 7), (5, 257, 64), (31, 255, 65), (32, 256, 128), (33, 1003, 24), (64, 64, 63), (257, 513, 130),
-                                   (300, 1000, 256), (700, 129, 33), (1531, 700, 200), (100, 5000, 320), (16, 20000, 64)])
+                                   (300, 1000, 256), (700, 129, 33), (1531, 700, 200), (100, 5000, 320), (16, 20000, 64),
+                                   (70, 5377, 37), (70, 1345, 100), (70, 1345, 250), (70, 1281, 260), (40, 4097, 64)])
 def test_linear_ce(N, V, D, dt):
     _ce_check(*_ce_inputs(N, V, D, dt))
 
