@@ -163,9 +163,10 @@ SIGNATURES = {
     "creste_trajectory_scores_grouped_f32": (_i, [_vp, _i, _i, _f, _i, _i, _vp, _vp, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
     "creste_irl_visitation_mix_f32": (_i, [_vp, _vp, _vp, _vp, _vp, _f, _i, _i64, _vp, _vp, _vp, _vp, _vp]),
     "creste_linear_ce_workspace_bytes": (_i64, [_i64, _i64, _i, _i, _i]),
-    "creste_linear_ce_forward": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i, _i, _i64, _f, _i, _vp, _vp, _vp, _vp, _vp, _i64,
+    "creste_linear_ce_packs_bytes": (_i64, [_vp, _i64, _vp, _i64, _i64, _i64, _i, _i]),
+    "creste_linear_ce_forward": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i, _i, _i64, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
                                       _vp]),
-    "creste_linear_ce_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i, _i, _f, _i, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "creste_linear_ce_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i, _i, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "creste_dropout": (_i, [_vp, _vp, _vp, _i64, _i, C.c_double, _i64, _i64, _vp, _vp]),
     "creste_gated_recurrence_chunk_steps": (_i, []),
     "creste_gated_recurrence_workspace_bytes": (_i64, [_i64, _i64, _i64]),

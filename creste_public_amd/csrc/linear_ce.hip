@@ -511,14 +511,14 @@ __device__ __forceinline__ void ce_interleave() {
 
 // a = the streamed side (p.m items), b = the own side (p.n items), NT x 32 own items per wave
 template <int MODE, int DT, int P, int DP, int NT>
-__global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
+__device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int blocks) {
   using L = CeStream<DP, kCeStage, P>;
   constexpr int NS = 3, KS = DP / 16, kDma = P * L::INSTR / 8 + (MODE == CE_DW);
   extern __shared__ __align__(1024) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, lh = lane >> 5;
   if constexpr (MODE == CE_LOSS)
-    if (blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;
-  int t = xcd_remap(blockIdx.x, gridDim.x);
+    if (block == 0 && threadIdx.x == 0) *p.done = 0;
+  const int t = xcd_remap(block, blocks);
   const int tn = t % p.nt, split = t / p.nt;
   const int own0 = tn * (256 * NT) + wave * (32 * NT);
   const int kb = split * p.ksplit, ke = min(p.k1, kb + p.ksplit);
@@ -719,6 +719,21 @@ __global__ __launch_bounds__(512, 2) void ce_stream_kernel(CeArgs p) {
     __syncthreads();
     ce_store<DT, DP / 32, NT>(p, acc, smem + wave * (32 * 512), own0, 0, split, lane);
   }
+}
+
+// own items per wave / 32: two where the registers hold them (for LOSS their features alone)
+constexpr int ce_nt(int mode, int P, int DP) { return P == 1 && (mode == CE_LOSS || DP == 64) ? 2 : 1; }
+
+template <int DT, int P, int DP>
+__global__ __launch_bounds__(512, 2) void ce_loss_kernel(CeArgs p) {
+  ce_stream_body<CE_LOSS, DT, P, DP, ce_nt(CE_LOSS, P, DP)>(p, blockIdx.x, gridDim.x);
+}
+
+// both gradients in one launch, the first nx workgroups dx: small problems leave CUs to each other
+template <int DT, int P, int DP>
+__global__ __launch_bounds__(512, 2) void ce_grad_kernel(CeArgs dx, CeArgs dw, int nx) {
+  if ((int)blockIdx.x < nx) ce_stream_body<CE_DX, DT, P, DP, ce_nt(CE_DX, P, DP)>(dx, blockIdx.x, nx);
+  else ce_stream_body<CE_DW, DT, P, DP, ce_nt(CE_DW, P, DP)>(dw, blockIdx.x - nx, gridDim.x - nx);
 }
 
 // ------------------------------------------------------------------------------------------------------- few rows
@@ -1002,12 +1017,11 @@ struct CePlan {
   int P, dt16, es, Dp, ldq, own;   // own: items a streaming workgroup holds
   bool packx, packw, stream;
   int64_t amax, xp, wp, part, zlab, bsum, done, g, dxp, dwp, total;
+  int64_t packs;                   // bytes of the copied operands, at the front of the workspace
   int64_t vc, n64, ldg;            // classes per piece, rows of G, bytes between them
   int pieces, tiles, sl, sx, sw;   // class tiles of the loss, splits of LOSS / DX / DW
 };
 
-// own items per wave / 32: two where the registers hold them (for LOSS their features alone)
-constexpr int ce_nt(int mode, int P, int DP) { return P == 1 && (mode == CE_LOSS || DP == 64) ? 2 : 1; }
 float ce_gscale_log2(const CePlan& q) { return q.dt16 == CRESTE_DT_F16 ? kCeF16Log2 : 0.f; }
 int ce_own(const CePlan& q, int mode) { return 256 * ce_nt(mode, q.P, q.Dp); }
 
@@ -1063,6 +1077,7 @@ CePlan ce_plan(int64_t N, int64_t V, int D, int dtype, bool packx, bool packw, b
   q.amax = take(64 + 2 * kCeMaxima * 4);           // the two maxima, the blocks' in front of them
   q.xp = packx ? take(N * q.Dp * 2 * q.P) : 0;
   q.wp = packw ? take(V * q.Dp * 2 * q.P) : 0;
+  q.packs = packx || packw ? o + 16 * packx + 32 * packw : 0;        // the size tells which (all else is in whole 1024 bytes)
   q.tiles = (int)((V + kCeTile - 1) / kCeTile);
   if (!train) {
     q.own = ce_own(q, CE_LOSS);
@@ -1127,48 +1142,60 @@ int ce_gemm(const CePlan& q, const CeArgs& a, int splits, hipStream_t s) {
   return ce_launch<MODE, CRESTE_DT_F16, 1, CeBig>(a, splits, s);
 }
 
-template <int MODE, int DT, int P, int DP>
-int ce_stream_launch(CeArgs a, int splits, hipStream_t s) {
-  constexpr int NT = ce_nt(MODE, P, DP), stages = 3 * CeStream<DP, kCeStage, P>::BYTES, out = MODE == CE_LOSS ? 0 : 8 * 32 * 512;
-  constexpr int bytes = stages > out ? stages : out;
-  static std::atomic<uint64_t> mask{0};
-  CRESTE_HIP(ensure_dyn_smem((const void*)ce_stream_kernel<MODE, DT, P, DP, NT>, bytes, mask));
-  a.nt = cdiv(a.n, 256 * NT);
+// number of workgroups of one of the streaming kernels' halves; completes its arguments
+int64_t ce_stream_blocks(CeArgs& a, int own, int splits) {
+  a.nt = cdiv(a.n, own);
   a.k1 = a.m;
   a.ksplit = (int)up(cdiv(a.m, splits), kCeStage);
-  const int64_t blocks = (int64_t)a.nt * splits;
-  CRESTE_REQUIRE(blocks < (1ll << 31), "linear_ce: too many tiles");
-  ce_stream_kernel<MODE, DT, P, DP, NT><<<(int)blocks, 512, bytes, s>>>(a);
+  return (int64_t)a.nt * splits;
+}
+
+// LOSS (loss given), or the gradients that are wanted (dx, dw: the others null)
+template <int DT, int P, int DP>
+int ce_stream_launch(const CePlan& q, CeArgs* loss, CeArgs* dx, CeArgs* dw, hipStream_t s) {
+  constexpr int stages = 3 * CeStream<DP, kCeStage, P>::BYTES, out = 8 * 32 * 512, grad = stages > out ? stages : out;
+  static std::atomic<uint64_t> mask_loss{0}, mask_grad{0};
+  const int64_t nl = loss ? ce_stream_blocks(*loss, q.own, q.sl) : 0, nx = dx ? ce_stream_blocks(*dx, q.own, q.sx) : 0,
+                nw = dw ? ce_stream_blocks(*dw, q.own, q.sw) : 0;
+  CRESTE_REQUIRE(nl + nx + nw < (1ll << 31), "linear_ce: too many tiles");
+  if (loss) {
+    CRESTE_HIP(ensure_dyn_smem((const void*)ce_loss_kernel<DT, P, DP>, stages, mask_loss));
+    ce_loss_kernel<DT, P, DP><<<(int)nl, 512, stages, s>>>(*loss);
+  } else {
+    CRESTE_HIP(ensure_dyn_smem((const void*)ce_grad_kernel<DT, P, DP>, grad, mask_grad));
+    ce_grad_kernel<DT, P, DP><<<(int)(nx + nw), 512, grad, s>>>(dx ? *dx : *dw, dw ? *dw : *dx, (int)nx);
+  }
   CRESTE_CHECK_LAUNCH("linear_ce stream");
   return CRESTE_OK;
 }
 
-template <int MODE, int DT, int P>
-int ce_stream_typed(const CePlan& q, const CeArgs& a, int splits, hipStream_t s) {
-  if (q.Dp == 64) return ce_stream_launch<MODE, DT, P, 64>(a, splits, s);
+template <int DT, int P>
+int ce_stream_typed(const CePlan& q, CeArgs* loss, CeArgs* dx, CeArgs* dw, hipStream_t s) {
+  if (q.Dp == 64) return ce_stream_launch<DT, P, 64>(q, loss, dx, dw, s);
   if constexpr (P == 1)
-    if (q.Dp == 256) return ce_stream_launch<MODE, DT, P, 256>(a, splits, s);
-  return ce_stream_launch<MODE, DT, P, 128>(a, splits, s);
+    if (q.Dp == 256) return ce_stream_launch<DT, P, 256>(q, loss, dx, dw, s);
+  return ce_stream_launch<DT, P, 128>(q, loss, dx, dw, s);
 }
 
-template <int MODE>
-int ce_stream(const CePlan& q, const CeArgs& a, int splits, hipStream_t s) {
-  if (q.P == 2) return ce_stream_typed<MODE, CRESTE_DT_F16, 2>(q, a, splits, s);
-  if (q.dt16 == CRESTE_DT_BF16) return ce_stream_typed<MODE, CRESTE_DT_BF16, 1>(q, a, splits, s);
-  return ce_stream_typed<MODE, CRESTE_DT_F16, 1>(q, a, splits, s);
+int ce_stream(const CePlan& q, CeArgs* loss, CeArgs* dx, CeArgs* dw, hipStream_t s) {
+  if (q.P == 2) return ce_stream_typed<CRESTE_DT_F16, 2>(q, loss, dx, dw, s);
+  if (q.dt16 == CRESTE_DT_BF16) return ce_stream_typed<CRESTE_DT_BF16, 1>(q, loss, dx, dw, s);
+  return ce_stream_typed<CRESTE_DT_F16, 1>(q, loss, dx, dw, s);
 }
 
 int ce_grid(int64_t items) { return (int)(items < 1 ? 1 : items > 2048 ? 2048 : items); }
 
 struct CeOperand { const char* p; int64_t ld, piece; };
 
-int ce_operands(const CePlan& q, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int D, int dtype,
+// the operands as the kernels read them, from `work` (the maxima and the copies at the offsets of the plan); copied there unless `ready`
+int ce_operands(const CePlan& q, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int D, bool ready,
                 char* work, CeOperand* X, CeOperand* W, hipStream_t s) {
   float *amax = (float*)(work + q.amax), *bmax = amax + 16;
   *X = {(const char*)x, ldx * 2, 0};
   *W = {(const char*)w, ldw * 2, 0};
   if (q.packx) *X = {work + q.xp, (int64_t)q.Dp * 2, N * q.Dp * 2};
   if (q.packw) *W = {work + q.wp, (int64_t)q.Dp * 2, V * q.Dp * 2};
+  if (ready) return CRESTE_OK;
   const CeSide sx{x, N, ldx, (short*)(work + q.xp), N * q.Dp}, sw{w, V, ldw, (short*)(work + q.wp), V * q.Dp};
   auto blocks = [](int64_t rows, int most) { const int64_t b = (rows + 15) / 16; return (int)(b > most ? most : b); };
   const int px = q.packx ? blocks(N, 2048) : 0, pw = q.packw ? blocks(V, 2048) : 0;
@@ -1206,22 +1233,35 @@ extern "C" int64_t creste_linear_ce_workspace_bytes(int64_t N, int64_t V, int D,
   return ce_plan(N, V, D, dtype, true, true, train != 0).total;      // as if both operands had to be copied
 }
 
+// whether the forward takes the few-rows kernel, which copies nothing
+static bool ce_takes_few(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int D, int dtype) {
+  return N <= kCeFewRows && ce_few(x, ldx, D, dtype) && ce_few(w, ldw, D, dtype);
+}
+
+extern "C" int64_t creste_linear_ce_packs_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int D,
+                                                int dtype) {
+  if (creste_linear_ce_workspace_bytes(N, V, D, dtype, 0) < 0) return -1;
+  if (ce_takes_few(x, ldx, w, ldw, N, D, dtype)) return 0;
+  return ce_plan(N, V, D, dtype, !ce_direct(x, ldx, D, dtype), !ce_direct(w, ldw, D, dtype), false).packs;
+}
+
 extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* labels, int64_t N,
                                         int64_t V, int D, int dtype, int64_t ignore_index, float temperature, int mean,
-                                        float* loss, float* nll, float* rows, float* stat, void* work, int64_t work_bytes,
-                                        void* stream) {
+                                        float* loss, float* nll, float* rows, float* stat, void* packs, void* work,
+                                        int64_t work_bytes, void* stream) {
   const int bad = ce_check(x, ldx, w, ldw, labels, N, V, D, dtype, temperature);
   if (bad) return bad;
-  const bool few = N <= kCeFewRows && ce_few(x, ldx, D, dtype) && ce_few(w, ldw, D, dtype);
+  const bool few = ce_takes_few(x, ldx, w, ldw, N, D, dtype);
   const CePlan q = ce_plan(N, V, D, dtype, !few && !ce_direct(x, ldx, D, dtype), !few && !ce_direct(w, ldw, D, dtype), false);
   CRESTE_REQUIRE(loss && nll && rows && stat && work && work_bytes >= q.total, "linear_ce_forward: outputs / workspace (%lld of %lld bytes)",
                  (long long)work_bytes, (long long)q.total);
-  CRESTE_REQUIRE(((uintptr_t)work & 15) == 0, "linear_ce_forward: work on a 16-byte boundary");
+  CRESTE_REQUIRE((((uintptr_t)work | (uintptr_t)packs) & 15) == 0, "linear_ce_forward: work and packs on 16-byte boundaries");
   hipStream_t s = (hipStream_t)stream;
   char* wk = (char*)work;
   CeOperand X{(const char*)x, ldx * q.es, 0}, W{(const char*)w, ldw * q.es, 0};
+  char* const copies = packs ? (char*)packs : wk;
   if (!few) {
-    const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, dtype, wk, &X, &W, s);
+    const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, false, copies, &X, &W, s);
     if (rc) return rc;
   }
   CeArgs a{};
@@ -1231,7 +1271,7 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
   a.k1 = q.Dp;
   a.labels = labels; a.ignore = ignore_index; a.classes = (int)V;
   a.inv_tau = 1.f / temperature;
-  a.amax = q.P == 2 ? (const float*)(wk + q.amax) : nullptr;
+  a.amax = q.P == 2 ? (const float*)(copies + q.amax) : nullptr;
   a.part = (float2*)(wk + q.part); a.zlab = (float*)(wk + q.zlab); a.done = (unsigned*)(wk + q.done);
   if (few) {
     if (dtype == CRESTE_DT_F32) ce_few_kernel<CRESTE_DT_F32><<<q.tiles, 256, 0, s>>>(a, D);
@@ -1239,7 +1279,7 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
     else ce_few_kernel<CRESTE_DT_F16><<<q.tiles, 256, 0, s>>>(a, D);
     CRESTE_CHECK_LAUNCH("linear_ce few rows");
   } else {
-    const int rg = q.stream ? ce_stream<CE_LOSS>(q, a, q.sl, s) : ce_gemm<CE_LOSS>(q, a, 1, s);
+    const int rg = q.stream ? ce_stream(q, &a, nullptr, nullptr, s) : ce_gemm<CE_LOSS>(q, a, 1, s);
     if (rg) return rg;
   }
   const int nb = cdiv(N, 64);
@@ -1252,22 +1292,25 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
 
 extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* rows, int64_t N, int64_t V,
                                          int D, int dtype, float temperature, int mean, const float* stat, const float* g_loss,
-                                         void* gx, void* gw, void* work, int64_t work_bytes, void* stream) {
+                                         const void* packs, void* gx, void* gw, void* work, int64_t work_bytes, void* stream) {
   const int bad = ce_check(x, ldx, w, ldw, rows, N, V, D, dtype, temperature);
   if (bad) return bad;
   const CePlan q = ce_plan(N, V, D, dtype, !ce_direct(x, ldx, D, dtype), !ce_direct(w, ldw, D, dtype), true);
   CRESTE_REQUIRE(stat && g_loss && (gx || gw) && work && work_bytes >= q.total, "linear_ce_backward: inputs / workspace (%lld of %lld bytes)",
                  (long long)work_bytes, (long long)q.total);
-  CRESTE_REQUIRE((((uintptr_t)gx | (uintptr_t)gw | (uintptr_t)work) & 15) == 0, "linear_ce_backward: gx, gw and work on 16-byte boundaries");
+  CRESTE_REQUIRE((((uintptr_t)gx | (uintptr_t)gw | (uintptr_t)work | (uintptr_t)packs) & 15) == 0,
+                 "linear_ce_backward: gx, gw, packs and work on 16-byte boundaries");
   hipStream_t s = (hipStream_t)stream;
   char* wk = (char*)work;
   CeOperand X, W;
-  const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, dtype, wk, &X, &W, s);
+  const bool kept = packs && !ce_takes_few(x, ldx, w, ldw, N, D, dtype);
+  char* const copies = kept ? (char*)packs : wk;
+  const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, kept, copies, &X, &W, s);
   if (rc) return rc;
   CeArgs c{};                                       // what every product shares
   c.classes = (int)V;
   c.inv_tau = 1.f / temperature;
-  c.amax = q.P == 2 ? (const float*)(wk + q.amax) : nullptr;
+  c.amax = q.P == 2 ? (const float*)(copies + q.amax) : nullptr;
   c.stat = stat; c.gl = g_loss; c.mean = mean;
   c.gscale = exp2f(ce_gscale_log2(q));
   c.row_l2 = rows; c.row_lab = (const int*)(rows + q.n64); c.row_rest = rows + 2 * q.n64; c.row_g = rows + 3 * q.n64;
@@ -1288,19 +1331,13 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
   dw.which = 0; dw.psplit = q.vc * q.ldq;
   if (q.dwp) dw.partial = (float*)(wk + q.dwp);
   if (q.stream) {
-    if (gx) {
-      dx.a = W.p; dx.lda = W.ld; dx.pa = W.piece; dx.ra = V; dx.m = (int)V;
-      dx.b = X.p; dx.ldb = X.ld; dx.pb = X.piece;
-      const int rg = ce_stream<CE_DX>(q, dx, q.sx, s);
-      if (rg) return rg;
-    }
-    if (gw) {
-      dw.a = X.p; dw.lda = X.ld; dw.pa = X.piece; dw.ra = N; dw.m = (int)N;
-      dw.b = W.p; dw.ldb = W.ld; dw.pb = W.piece; dw.n = (int)V;
-      dw.out = gw;
-      const int rg = ce_stream<CE_DW>(q, dw, q.sw, s);
-      if (rg) return rg;
-    }
+    dx.a = W.p; dx.lda = W.ld; dx.pa = W.piece; dx.ra = V; dx.m = (int)V;
+    dx.b = X.p; dx.ldb = X.ld; dx.pb = X.piece;
+    dw.a = X.p; dw.lda = X.ld; dw.pa = X.piece; dw.ra = N; dw.m = (int)N;
+    dw.b = W.p; dw.ldb = W.ld; dw.pb = W.piece; dw.n = (int)V;
+    dw.out = gw;
+    const int rg = ce_stream(q, nullptr, gx ? &dx : nullptr, gw ? &dw : nullptr, s);
+    if (rg) return rg;
   } else {
     for (int piece = 0; piece < q.pieces; ++piece) {
       const int64_t v0 = piece * q.vc, nv = V - v0 < q.vc ? V - v0 : q.vc;

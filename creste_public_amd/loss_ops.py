@@ -170,7 +170,7 @@ class LinearCEFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, labels, ignore_index, temperature, reduction):
-        loss, nll, saved = ops.linear_ce(x, weight, labels, ignore_index, temperature, reduction)
+        loss, nll, saved = ops.linear_ce(x, weight, labels, ignore_index, temperature, reduction, keep=True)
         ctx.save_for_backward(x, weight, saved)
         ctx.args = (temperature, reduction)
         ctx.mark_non_differentiable(nll)

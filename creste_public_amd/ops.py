@@ -1644,32 +1644,40 @@ def _linear_ce_args(x, w, temperature, reduction):
 
 
 def _ce_saved(N: int) -> int:
-    return 4 + 4 * (-(-N // 64) * 64)          # {sum, count, -, -}, [4][N rounded up to 64]
+    return 4 + 4 * (-(-N // 64) * 64)          # {sum, count, -, -}, [4][N rounded up to 64]: a multiple of 16 bytes
 
 
 def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def linear_ce(x, w, labels, ignore_index: int = -100, temperature: float = 1.0, reduction: str = "mean"):
+# Operands the kernels cannot read in place (fp32, odd widths or strides) are copied.  Up to this many bytes the forward's copies are kept
+# for the backward: small steps are bound by launches (19584 x 4096 x 128 fp32, 12 MB of copies, with both gradients in one launch: 380 -> 361 us)
+CE_KEEP_COPIES = 64 << 20
+
+
+def linear_ce(x, w, labels, ignore_index: int = -100, temperature: float = 1.0, reduction: str = "mean", keep: bool = False):
     """forward of loss_ops.linear_cross_entropy for x [N,D] -> (loss [], nll [N], saved), fp32; `saved` is what linear_ce_bwd needs of it
-    (sum and count, then four words per row)"""
+    (sum and count, four words per row; with keep=True also the copies of the operands, if any and small)"""
     code, x_, w_ = _linear_ce_args(x, w, temperature, reduction)
     N, D = x_.shape
     V, dev = w_.shape[0], x_.device
     labels = _plain(labels, torch.int64, (N,), dev, "linear_cross_entropy: labels")
     loss, nll = torch.empty((), dtype=torch.float32, device=dev), torch.empty(N, dtype=torch.float32, device=dev)
-    saved = torch.empty(_ce_saved(N), dtype=torch.float32, device=dev)
     if N == 0:
-        return loss.zero_(), nll, saved.zero_()
+        return loss.zero_(), nll, torch.zeros(_ce_saved(0), dtype=torch.float32, device=dev)
     lib = _lib.load()
+    packs = lib.creste_linear_ce_packs_bytes(x_.data_ptr(), _row_stride(x_), w_.data_ptr(), _row_stride(w_), N, V, D, code) if keep else 0
+    packs = packs if packs <= CE_KEEP_COPIES else 0
+    saved = torch.empty(_ce_saved(N) + packs // 4, dtype=torch.float32, device=dev)
     with _on(dev) as on:
         nb = lib.creste_linear_ce_workspace_bytes(N, V, D, code, 0)
         work = torch.empty(nb, dtype=torch.uint8, device=dev)
         _lib.check(lib.creste_linear_ce_forward(x_.data_ptr(), _row_stride(x_), w_.data_ptr(), _row_stride(w_), labels.data_ptr(), N, V, D,
                                                 code, _int64(ignore_index, "linear_cross_entropy: ignore_index"), float(temperature),
                                                 int(reduction == "mean"), loss.data_ptr(), nll.data_ptr(), saved.data_ptr() + 16,
-                                                saved.data_ptr(), work.data_ptr(), nb, on.stream), "linear_ce_forward")
+                                                saved.data_ptr(), saved.data_ptr() + 4 * _ce_saved(N) if packs else None,
+                                                work.data_ptr(), nb, on.stream), "linear_ce_forward")
     return loss, nll, saved
 
 
@@ -1677,7 +1685,9 @@ def linear_ce_bwd(x, w, saved, g_loss, temperature: float = 1.0, reduction: str 
                   need_w: bool = True):
     """gradient of linear_ce for the cotangent g_loss (one fp32 element) -> (gx, gw); None for what is not needed"""
     code, x_, w_ = _linear_ce_args(x, w, temperature, reduction)
-    saved = _plain(saved, torch.float32, (_ce_saved(x_.shape[0]),), x_.device, "linear_cross_entropy: saved")
+    if not isinstance(saved, torch.Tensor) or saved.dim() != 1 or saved.numel() < _ce_saved(x_.shape[0]):
+        raise HipLibraryError("linear_cross_entropy: saved: expected what linear_ce returned for these features")
+    saved = _plain(saved, torch.float32, saved.shape, x_.device, "linear_cross_entropy: saved")
     g_loss = _plain(g_loss.reshape(1), torch.float32, (1,), x_.device, "linear_cross_entropy: cotangent")
     return _linear_ce_bwd(x_, w_, saved, g_loss, temperature, reduction, need_x, need_w, code)
 
@@ -1694,9 +1704,14 @@ def _linear_ce_bwd(x, w, saved, g_loss, temperature, reduction, need_x, need_w, 
     with _on(x.device) as on:
         nb = lib.creste_linear_ce_workspace_bytes(N, V, D, code, 1)
         work = torch.empty(nb, dtype=torch.uint8, device=x.device)
+        # the forward's copies serve where the same operands need them: a tensor that saved_tensors_hooks bring back may be laid out anew
+        copies = 4 * (saved.numel() - _ce_saved(N))
+        copies = copies and copies == lib.creste_linear_ce_packs_bytes(x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), N, V, D,
+                                                                       code)
         _lib.check(lib.creste_linear_ce_backward(x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), saved.data_ptr() + 16, N, V,
                                                  D, code, float(temperature), int(reduction == "mean"), saved.data_ptr(),
-                                                 g_loss.data_ptr(), gx.data_ptr() if need_x else None,
+                                                 g_loss.data_ptr(), saved.data_ptr() + 4 * _ce_saved(N) if copies else None,
+                                                 gx.data_ptr() if need_x else None,
                                                  gw.data_ptr() if need_w else None, work.data_ptr(), nb, on.stream),
                    "linear_ce_backward")
     return gx, gw

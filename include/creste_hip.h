@@ -705,14 +705,17 @@ int creste_irl_visitation_mix_f32(const float* exp_svf_raw, const uint8_t* fov, 
  *   forward : loss [1] (mean over the counted rows, 0 if there are none, or sum), nll [N] (0 where ignored), and for the backward
  *             rows [4][N rounded up to 64] 4-byte words (log-sum-exps, labels) and stat [2] = {sum nll, count}.
  *   backward: gx [N][D], gw [V][D] (contiguous, 16-byte aligned, the features' type; either may be NULL) for the cotangent g_loss [1].
+ * packs: operands that the kernels cannot read in place (fp32, odd strides or widths) are copied, packs_bytes of them (0: none), into
+ *          `work`; given a buffer (16-byte aligned) in both calls the forward's copies serve the backward.  NULL: copied in each.
  * work (16-byte aligned): workspace_bytes(..., train = 0) for the forward, train = 1 for the backward; -1 = sizes out of range. */
 int64_t creste_linear_ce_workspace_bytes(int64_t N, int64_t V, int D, int dtype, int train);
+int64_t creste_linear_ce_packs_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int D, int dtype);
 int creste_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* labels, int64_t N, int64_t V,
                              int D, int dtype, int64_t ignore_index, float temperature, int mean, float* loss, float* nll,
-                             float* rows, float* stat, void* work, int64_t work_bytes, void* stream);
+                             float* rows, float* stat, void* packs, void* work, int64_t work_bytes, void* stream);
 int creste_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* rows, int64_t N, int64_t V, int D,
-                              int dtype, float temperature, int mean, const float* stat, const float* g_loss, void* gx, void* gw,
-                              void* work, int64_t work_bytes, void* stream);
+                              int dtype, float temperature, int mean, const float* stat, const float* g_loss, const void* packs,
+                              void* gx, void* gw, void* work, int64_t work_bytes, void* stream);
 
 /* Dropout (csrc/dropout.hip): y_i = keep_i ? x_i / (1 - p) : 0 (+ residual_i), 0 <= p <= 1, n elements.  keep_i = word_i >=
  * round(p 2^32), word_i = word i mod 4 of Philox4x32-10 with counter (i div 4, offset) and key seed, 64 bits each.  The backward is

@@ -56,7 +56,7 @@ def test_entry_points_report_bad_arguments():
         assert rc == -1 and text in lib.creste_last_error(), lib.creste_last_error()
 
     def fwd(x=p, N=4, V=8, D=16, dt=0, tau=1.0, ldx=16, ldw=16, work=p, nb=1 << 40):
-        return lib.creste_linear_ce_forward(x, ldx, p, ldw, p, N, V, D, dt, -100, tau, 1, p, p, p, p, work, nb, None)
+        return lib.creste_linear_ce_forward(x, ldx, p, ldw, p, N, V, D, dt, -100, tau, 1, p, p, p, p, None, work, nb, None)
     err(fwd(x=None), b"null pointer")
     err(fwd(dt=3), b"dtype")
     err(fwd(N=0), b"N 0")
@@ -69,10 +69,10 @@ def test_entry_points_report_bad_arguments():
     err(fwd(tau=float("inf")), b"temperature")
     err(fwd(nb=1000), b"workspace")
     err(fwd(work=None), b"workspace")
-    err(lib.creste_linear_ce_backward(p, 16, p, 16, p, 4, 8, 16, 0, 1.0, 1, p, p, None, None, p, 1 << 40, None), b"inputs")
+    err(lib.creste_linear_ce_backward(p, 16, p, 16, p, 4, 8, 16, 0, 1.0, 1, p, p, None, None, None, p, 1 << 40, None), b"inputs")
     odd = C.c_void_p(4104)
     err(fwd(work=odd), b"16-byte")
-    err(lib.creste_linear_ce_backward(p, 16, p, 16, p, 4, 8, 16, 0, 1.0, 1, p, p, odd, None, p, 1 << 40, None), b"16-byte")
+    err(lib.creste_linear_ce_backward(p, 16, p, 16, p, 4, 8, 16, 0, 1.0, 1, p, p, None, odd, None, p, 1 << 40, None), b"16-byte")
     for bad in ((0, 8, 16, 0), (4, 0, 16, 0), (4, 8, 0, 0), (4, 8, 16, 5), (1 << 31, 8, 16, 0)):
         assert lib.creste_linear_ce_workspace_bytes(*bad, 1) == -1
 
@@ -92,6 +92,21 @@ def test_entry_points_report_bad_arguments():
     err(lib.creste_gated_recurrence_backward(p, 12, 4, p, 12, 4, p, 12, 4, None, None, None, 2, 3, 4, 0, p, p, None, p, 1 << 40, None),
         b"null pointer")
     assert lib.creste_gated_recurrence_workspace_bytes(0, 3, 4) == -1
+
+
+def test_which_operands_are_copied():
+    """bf16 rows of 64, 128, 256 or more multiples of 64 elements on 16-byte boundaries are read in place, the rest is copied once"""
+    f = _lib.load().creste_linear_ce_packs_bytes
+    at = C.c_void_p(4096)
+    assert f(at, 128, at, 128, 100, 50, 128, 1) == 0 and f(at, 320, at, 320, 100, 50, 320, 2) == 0
+    assert f(at, 136, at, 4096, 100, 50, 128, 1) == 0                              # wider rows
+    one = f(at, 100, at, 128, 100, 50, 100, 1)
+    assert one >= (100 + 50) * 128 * 2                                             # padded to 128
+    assert f(C.c_void_p(4098), 128, at, 128, 100, 50, 128, 1) >= 100 * 128 * 2
+    assert f(at, 129, at, 128, 100, 50, 128, 1) >= 100 * 128 * 2
+    assert f(at, 128, at, 128, 100, 50, 128, 0) >= (100 + 50) * 128 * 4             # fp32: two pieces
+    assert f(at, 128, at, 128, 30, 50, 128, 0) == 0                                # few rows: read in place by the forward
+    assert f(at, 128, at, 128, 0, 50, 128, 0) == -1
 
 
 @pytest.mark.parametrize("N,V,D,dt", [(1, 1, 1, 0), (19584, 4096, 128, 0), (4096, 131072, 1024, 1), (1 << 20, 1 << 20, 64, 1),

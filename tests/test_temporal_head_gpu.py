@@ -1,5 +1,7 @@
 """GPU: the operators of the temporal classification head (csrc/linear_ce.hip, dropout.hip, recurrence.hip) against their 64-bit
 definitions, elementwise within derived bounds (temporal_head_oracle.py)."""
+import contextlib
+
 import pytest
 import torch
 
@@ -394,6 +396,34 @@ def test_linear_ce_strides(dt):
         got = _ce_check(xv, wv, labels)
         assert all(torch.equal(a, b) for a, b in zip(ref, got))
     _ce_check(x[:1].expand(90, 128), w, labels)
+
+
+@pytest.mark.parametrize("dt", ALL, ids=IDS)
+def test_linear_ce_kept_copies(dt):
+    """the copies of the operands kept by the forward or made anew by the backward (large operands, tensors laid out anew): the same bits"""
+    x, w, labels = _ce_inputs(90, 300, 100, dt)
+    one = torch.ones((), device="cuda")
+    a, b = ops.linear_ce(x, w, labels, temperature=0.1, keep=True), ops.linear_ce(x, w, labels, temperature=0.1)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and a[2].numel() > b[2].numel()
+    ga, gb = (ops.linear_ce_bwd(x, w, t[2], one, temperature=0.1) for t in (a, b))
+    assert all(torch.equal(u, v) for u, v in zip(ga, gb))
+    for bad in (a[2][:100], b[2].half()):
+        with pytest.raises(E):
+            ops.linear_ce_bwd(x, w, bad, one, temperature=0.1)
+
+
+def test_linear_ce_saved_tensors_come_back_laid_out_anew():
+    """16-bit features of 64: the view off its 16 bytes is copied by the forward, and read in place after its way over the host"""
+    buf = torch.randn(90 * 64 + 1, device="cuda", dtype=F16)
+    w, labels = torch.randn(90, 64, device="cuda", dtype=F16), torch.randint(0, 90, (90,), device="cuda")
+    grads = []
+    for hooks in (False, True):
+        x = buf[1:].view(90, 64).detach().requires_grad_(True)
+        wl = w.clone().requires_grad_(True)
+        with torch.autograd.graph.save_on_cpu() if hooks else contextlib.nullcontext():
+            loss, _ = loss_ops.linear_cross_entropy(x, wl, labels, temperature=4.0)
+        grads.append(torch.autograd.grad(loss, (x, wl)))
+    assert all(torch.equal(u, v) for u, v in zip(*grads))
 
 
 def test_linear_ce_one_sided_gradients():
