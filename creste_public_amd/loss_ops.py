@@ -174,6 +174,7 @@ class LinearCEFn(torch.autograd.Function):
         ctx.save_for_backward(x, weight, saved)
         ctx.args = (temperature, reduction)
         ctx.mark_non_differentiable(nll)
+        ctx.set_materialize_grads(False)       # no zeros for nll; the loss's own cotangent is always there
         return loss, nll
 
     @staticmethod
