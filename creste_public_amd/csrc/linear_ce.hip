@@ -833,8 +833,19 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeArgs p, int D) {
 }
 
 // ---------------------------------------------------------------------------------------------------- small kernels
-// both operands at once: blocks below `split` take the first, the others the second
-struct CeSide { const void* x; int64_t rows, ld; short* out; int64_t piece; };
+// both operands at once: blocks below `split` take the first, the others the second.  Rows of x that do not count are taken as zeros,
+// whatever they hold (0 * NaN would reach dw, a large value fp32's scale): named by their labels, behind the forward by the infinite
+// log-sum-exp it left
+struct CeSide {
+  const void* x;
+  int64_t rows, ld;
+  short* out;
+  int64_t piece;
+  const int64_t* labels;
+  int64_t ignore;
+  const float* counts;
+  __device__ __forceinline__ bool off(int64_t r) const { return labels ? labels[r] == ignore : counts && counts[r] == INFINITY; }
+};
 
 // Each 16 lanes take whole rows, 4 columns a lane and step (no division by the row length).
 // amax: per block max |x| of its operand -> bmax[block]
@@ -847,6 +858,7 @@ __global__ __launch_bounds__(256) void ce_amax_kernel(CeSide u, CeSide v, int co
   float m = 0.f;
   for (int64_t r = (int64_t)blk * 16 + (threadIdx.x >> 4); r < s.rows; r += (int64_t)nb * 16) {
     const float* x = (const float*)s.x + r * s.ld;
+    if (s.off(r)) continue;
     for (int c = c0; c < cols; c += 64)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -882,11 +894,12 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int co
   const int c0 = (threadIdx.x & 15) * 4;
   for (int64_t r = (int64_t)blk * 16 + (threadIdx.x >> 4); r < s.rows; r += (int64_t)nb * 16) {
     const T* x = (const T*)s.x + r * s.ld;
+    const int there = s.off(r) ? 0 : cols;
     for (int c = c0; c < cp; c += 64) {
       ces4 hi, lo;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const T v = c + e < cols ? x[c + e] : (T)0;
+        const T v = c + e < there ? x[c + e] : (T)0;
         if constexpr (sizeof(T) == 4) {
           const float a = v * scale;
           const short h = ce_cvt<CRESTE_DT_F16>(a);       // (a scalar: bit casts of vector elements are miscompiled)
@@ -1012,7 +1025,8 @@ namespace {
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 // Where everything sits in the caller's workspace.  The operands are used in place when a row is a multiple of 64 elements on
-// 16-byte boundaries, else copied once (padded; fp32 always: into its two pieces).
+// 16-byte boundaries, else copied once (padded; fp32 always: into its two pieces).  The gradients always have x from a copy, without what
+// ignored rows hold (a training step of 8192 x 65536 x 256 bf16: 1215 -> 1219 us).
 struct CePlan {
   int P, dt16, es, Dp, ldq, own;   // own: items a streaming workgroup holds
   bool packx, packw, stream;
@@ -1077,7 +1091,7 @@ CePlan ce_plan(int64_t N, int64_t V, int D, int dtype, bool packx, bool packw, b
   q.amax = take(64 + 2 * kCeMaxima * 4);           // the two maxima, the blocks' in front of them
   q.xp = packx ? take(N * q.Dp * 2 * q.P) : 0;
   q.wp = packw ? take(V * q.Dp * 2 * q.P) : 0;
-  q.packs = packx || packw ? o + 16 * packx + 32 * packw : 0;        // the size tells which (all else is in whole 1024 bytes)
+  q.packs = o + 32 * packw;                        // the size tells whether w is among them (all else is in whole 1024 bytes)
   q.tiles = (int)((V + kCeTile - 1) / kCeTile);
   if (!train) {
     q.own = ce_own(q, CE_LOSS);
@@ -1187,16 +1201,18 @@ int ce_grid(int64_t items) { return (int)(items < 1 ? 1 : items > 2048 ? 2048 : 
 
 struct CeOperand { const char* p; int64_t ld, piece; };
 
-// the operands as the kernels read them, from `work` (the maxima and the copies at the offsets of the plan); copied there unless `ready`
+// the operands as the kernels read them, from `work` (the maxima and the copies at the offsets of the plan); copied there unless `ready`.
+// labels, ignore, counts: see CeSide
 int ce_operands(const CePlan& q, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int D, bool ready,
-                char* work, CeOperand* X, CeOperand* W, hipStream_t s) {
+                const int64_t* labels, int64_t ignore, const float* counts, char* work, CeOperand* X, CeOperand* W, hipStream_t s) {
   float *amax = (float*)(work + q.amax), *bmax = amax + 16;
   *X = {(const char*)x, ldx * 2, 0};
   *W = {(const char*)w, ldw * 2, 0};
   if (q.packx) *X = {work + q.xp, (int64_t)q.Dp * 2, N * q.Dp * 2};
   if (q.packw) *W = {work + q.wp, (int64_t)q.Dp * 2, V * q.Dp * 2};
   if (ready) return CRESTE_OK;
-  const CeSide sx{x, N, ldx, (short*)(work + q.xp), N * q.Dp}, sw{w, V, ldw, (short*)(work + q.wp), V * q.Dp};
+  const CeSide sx{x, N, ldx, (short*)(work + q.xp), N * q.Dp, labels, ignore, counts},
+      sw{w, V, ldw, (short*)(work + q.wp), V * q.Dp, nullptr, 0, nullptr};
   auto blocks = [](int64_t rows, int most) { const int64_t b = (rows + 15) / 16; return (int)(b > most ? most : b); };
   const int px = q.packx ? blocks(N, 2048) : 0, pw = q.packw ? blocks(V, 2048) : 0;
   if (q.P == 2) {                                  // (both are copied)
@@ -1218,7 +1234,8 @@ int ce_check(const void* x, int64_t ldx, const void* w, int64_t ldw, const void*
                  (long long)N, (long long)V, D);
   CRESTE_REQUIRE((ldx >= D || (ldx == 0 || N == 1)) && ldx >= 0 && (ldw >= D || V == 1 || ldw == 0) && ldw >= 0,
                  "linear_ce: row strides %lld %lld", (long long)ldx, (long long)ldw);
-  CRESTE_REQUIRE(tau > 0.f && tau < INFINITY, "linear_ce: temperature must be positive and finite");
+  CRESTE_REQUIRE(tau > 0.f && tau < INFINITY && 1.f / tau < INFINITY,
+                 "linear_ce: temperature must be positive and finite, its inverse too");
   return CRESTE_OK;
 }
 
@@ -1242,7 +1259,7 @@ extern "C" int64_t creste_linear_ce_packs_bytes(const void* x, int64_t ldx, cons
                                                 int dtype) {
   if (creste_linear_ce_workspace_bytes(N, V, D, dtype, 0) < 0) return -1;
   if (ce_takes_few(x, ldx, w, ldw, N, D, dtype)) return 0;
-  return ce_plan(N, V, D, dtype, !ce_direct(x, ldx, D, dtype), !ce_direct(w, ldw, D, dtype), false).packs;
+  return ce_plan(N, V, D, dtype, true, !ce_direct(w, ldw, D, dtype), false).packs;
 }
 
 extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* labels, int64_t N,
@@ -1252,7 +1269,9 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
   const int bad = ce_check(x, ldx, w, ldw, labels, N, V, D, dtype, temperature);
   if (bad) return bad;
   const bool few = ce_takes_few(x, ldx, w, ldw, N, D, dtype);
-  const CePlan q = ce_plan(N, V, D, dtype, !few && !ce_direct(x, ldx, D, dtype), !few && !ce_direct(w, ldw, D, dtype), false);
+  // (a row of x only reaches its own softmax, so x need not be copied for what ignored rows hold -- unless the backward is to have it)
+  const CePlan q = ce_plan(N, V, D, dtype, !few && (packs || !ce_direct(x, ldx, D, dtype)), !few && !ce_direct(w, ldw, D, dtype),
+                           false);
   CRESTE_REQUIRE(loss && nll && rows && stat && work && work_bytes >= q.total, "linear_ce_forward: outputs / workspace (%lld of %lld bytes)",
                  (long long)work_bytes, (long long)q.total);
   CRESTE_REQUIRE((((uintptr_t)work | (uintptr_t)packs) & 15) == 0, "linear_ce_forward: work and packs on 16-byte boundaries");
@@ -1261,7 +1280,7 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
   CeOperand X{(const char*)x, ldx * q.es, 0}, W{(const char*)w, ldw * q.es, 0};
   char* const copies = packs ? (char*)packs : wk;
   if (!few) {
-    const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, false, copies, &X, &W, s);
+    const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, false, labels, ignore_index, nullptr, copies, &X, &W, s);
     if (rc) return rc;
   }
   CeArgs a{};
@@ -1295,7 +1314,7 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
                                          const void* packs, void* gx, void* gw, void* work, int64_t work_bytes, void* stream) {
   const int bad = ce_check(x, ldx, w, ldw, rows, N, V, D, dtype, temperature);
   if (bad) return bad;
-  const CePlan q = ce_plan(N, V, D, dtype, !ce_direct(x, ldx, D, dtype), !ce_direct(w, ldw, D, dtype), true);
+  const CePlan q = ce_plan(N, V, D, dtype, true, !ce_direct(w, ldw, D, dtype), true);
   CRESTE_REQUIRE(stat && g_loss && (gx || gw) && work && work_bytes >= q.total, "linear_ce_backward: inputs / workspace (%lld of %lld bytes)",
                  (long long)work_bytes, (long long)q.total);
   CRESTE_REQUIRE((((uintptr_t)gx | (uintptr_t)gw | (uintptr_t)work | (uintptr_t)packs) & 15) == 0,
@@ -1305,7 +1324,7 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
   CeOperand X, W;
   const bool kept = packs && !ce_takes_few(x, ldx, w, ldw, N, D, dtype);
   char* const copies = kept ? (char*)packs : wk;
-  const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, kept, copies, &X, &W, s);
+  const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, kept, nullptr, 0, q.P == 2 ? rows + 2 * q.n64 : rows, copies, &X, &W, s);
   if (rc) return rc;
   CeArgs c{};                                       // what every product shares
   c.classes = (int)V;

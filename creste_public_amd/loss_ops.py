@@ -191,8 +191,8 @@ def linear_cross_entropy(x, weight, labels, ignore_index: int = -100, temperatur
     labels [...] int64, over any number of classes and without ever holding the N x V logits:
         z = x weight^T / temperature;  nll = logsumexp(z) - z[label], 0 where label == ignore_index
     -> (loss, nll): loss = mean of nll over the rows that count (0 when none does) or their sum, a differentiable fp32 scalar;
-    nll [...] fp32, not differentiable.  Features are expected to be finite, those of ignored rows too.  A label that names neither
-    a class nor ignore_index makes the loss and its gradients NaN.  fp32 features are multiplied with 22 significand bits.
+    nll [...] fp32, not differentiable.  The features of ignored rows may be anything (infinite, NaN: padding); their gradient is 0.  A label
+    that names neither a class nor ignore_index makes the loss and its gradients NaN.  fp32 features are multiplied with 22 significand bits.
     Differentiable once; not recorded inside a stream capture (train_ops.recorded)."""
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise HipLibraryError("linear_cross_entropy: x [...,D] expected")

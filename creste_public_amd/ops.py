@@ -1644,21 +1644,22 @@ def _linear_ce_args(x, w, temperature, reduction):
 
 
 def _ce_saved(N: int) -> int:
-    return 4 + 4 * (-(-N // 64) * 64)          # {sum, count, -, -}, [4][N rounded up to 64]: a multiple of 16 bytes
+    return 64 + 4 * (-(-N // 64) * 64)         # {sum, count, -}, [4][N rounded up to 64]: whole 256 bytes, copies behind lie on cache lines
 
 
 def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-# Operands the kernels cannot read in place (fp32, odd widths or strides) are copied.  Up to this many bytes the forward's copies are kept
-# for the backward: small steps are bound by launches (19584 x 4096 x 128 fp32, 12 MB of copies, with both gradients in one launch: 380 -> 361 us)
+# The gradients read a copy of x (ignored rows as zeros), and one of w where it cannot be read in place (fp32, odd widths or strides).  Up
+# to this many bytes the forward's copies are kept for the backward: small steps are bound by launches (19584 x 4096 x 128 fp32, 12 MB of
+# copies, with both gradients in one launch: 380 -> 361 us), large ones by memory
 CE_KEEP_COPIES = 64 << 20
 
 
 def linear_ce(x, w, labels, ignore_index: int = -100, temperature: float = 1.0, reduction: str = "mean", keep: bool = False):
     """forward of loss_ops.linear_cross_entropy for x [N,D] -> (loss [], nll [N], saved), fp32; `saved` is what linear_ce_bwd needs of it
-    (sum and count, four words per row; with keep=True also the copies of the operands, if any and small)"""
+    (sum and count, four words per row; with keep=True also the copies of the operands that the backward reads, if they are small)"""
     code, x_, w_ = _linear_ce_args(x, w, temperature, reduction)
     N, D = x_.shape
     V, dev = w_.shape[0], x_.device
@@ -1675,7 +1676,7 @@ def linear_ce(x, w, labels, ignore_index: int = -100, temperature: float = 1.0, 
         work = torch.empty(nb, dtype=torch.uint8, device=dev)
         _lib.check(lib.creste_linear_ce_forward(x_.data_ptr(), _row_stride(x_), w_.data_ptr(), _row_stride(w_), labels.data_ptr(), N, V, D,
                                                 code, _int64(ignore_index, "linear_cross_entropy: ignore_index"), float(temperature),
-                                                int(reduction == "mean"), loss.data_ptr(), nll.data_ptr(), saved.data_ptr() + 16,
+                                                int(reduction == "mean"), loss.data_ptr(), nll.data_ptr(), saved.data_ptr() + 256,
                                                 saved.data_ptr(), saved.data_ptr() + 4 * _ce_saved(N) if packs else None,
                                                 work.data_ptr(), nb, on.stream), "linear_ce_forward")
     return loss, nll, saved
@@ -1708,7 +1709,7 @@ def _linear_ce_bwd(x, w, saved, g_loss, temperature, reduction, need_x, need_w, 
         copies = 4 * (saved.numel() - _ce_saved(N))
         copies = copies and copies == lib.creste_linear_ce_packs_bytes(x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), N, V, D,
                                                                        code)
-        _lib.check(lib.creste_linear_ce_backward(x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), saved.data_ptr() + 16, N, V,
+        _lib.check(lib.creste_linear_ce_backward(x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), saved.data_ptr() + 256, N, V,
                                                  D, code, float(temperature), int(reduction == "mean"), saved.data_ptr(),
                                                  g_loss.data_ptr(), saved.data_ptr() + 4 * _ce_saved(N) if copies else None,
                                                  gx.data_ptr() if need_x else None,

@@ -701,12 +701,13 @@ int creste_irl_visitation_mix_f32(const float* exp_svf_raw, const uint8_t* fov, 
  *
  * Softmax cross entropy over V classes straight from the features (csrc/linear_ce.hip): z = x w^T / temperature, x [N][ldx],
  * w [V][ldw] (strides in elements, D of them used), labels [N] int64; a row whose label is ignore_index does not count, one whose
- * label names no class makes loss and gradients NaN.  No N x V buffer.
+ * label names no class makes loss and gradients NaN.  No N x V buffer.  An ignored row may hold anything; its gx is 0.
  *   forward : loss [1] (mean over the counted rows, 0 if there are none, or sum), nll [N] (0 where ignored), and for the backward
  *             rows [4][N rounded up to 64] 4-byte words (log-sum-exps, labels) and stat [2] = {sum nll, count}.
  *   backward: gx [N][D], gw [V][D] (contiguous, 16-byte aligned, the features' type; either may be NULL) for the cotangent g_loss [1].
- * packs: operands that the kernels cannot read in place (fp32, odd strides or widths) are copied, packs_bytes of them (0: none), into
- *          `work`; given a buffer (16-byte aligned) in both calls the forward's copies serve the backward.  NULL: copied in each.
+ * packs: the copies of the operands that the backward reads (x, and w where the kernels cannot read it in place: fp32, odd strides or
+ *          widths), packs_bytes (0: the forward makes none).  Given a buffer (16-byte aligned) in both calls the forward's serve the
+ *          backward; NULL: each makes its own in `work`.
  * work (16-byte aligned): workspace_bytes(..., train = 0) for the forward, train = 1 for the backward; -1 = sizes out of range. */
 int64_t creste_linear_ce_workspace_bytes(int64_t N, int64_t V, int D, int dtype, int train);
 int64_t creste_linear_ce_packs_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int D, int dtype);

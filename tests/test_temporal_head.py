@@ -67,6 +67,7 @@ def test_entry_points_report_bad_arguments():
     err(fwd(tau=0.0), b"temperature")
     err(fwd(tau=float("nan")), b"temperature")
     err(fwd(tau=float("inf")), b"temperature")
+    err(fwd(tau=1e-40), b"temperature")
     err(fwd(nb=1000), b"workspace")
     err(fwd(work=None), b"workspace")
     err(lib.creste_linear_ce_backward(p, 16, p, 16, p, 4, 8, 16, 0, 1.0, 1, p, p, None, None, None, p, 1 << 40, None), b"inputs")
@@ -95,16 +96,16 @@ def test_entry_points_report_bad_arguments():
 
 
 def test_which_operands_are_copied():
-    """bf16 rows of 64, 128, 256 or more multiples of 64 elements on 16-byte boundaries are read in place, the rest is copied once"""
+    """the backward reads a copy of x; of w only where it is not 16-bit rows of 64, 128, 256 or more multiples of 64 elements on 16 bytes"""
     f = _lib.load().creste_linear_ce_packs_bytes
     at = C.c_void_p(4096)
-    assert f(at, 128, at, 128, 100, 50, 128, 1) == 0 and f(at, 320, at, 320, 100, 50, 320, 2) == 0
-    assert f(at, 136, at, 4096, 100, 50, 128, 1) == 0                              # wider rows
-    one = f(at, 100, at, 128, 100, 50, 100, 1)
-    assert one >= (100 + 50) * 128 * 2                                             # padded to 128
-    assert f(C.c_void_p(4098), 128, at, 128, 100, 50, 128, 1) >= 100 * 128 * 2
-    assert f(at, 129, at, 128, 100, 50, 128, 1) >= 100 * 128 * 2
-    assert f(at, 128, at, 128, 100, 50, 128, 0) >= (100 + 50) * 128 * 4             # fp32: two pieces
+    alone = f(at, 128, at, 128, 100, 50, 128, 1)
+    assert 100 * 128 * 2 <= alone < 100 * 128 * 2 + 8192
+    assert f(at, 136, at, 4096, 100, 50, 128, 1) == alone                          # wider rows
+    assert f(C.c_void_p(4098), 128, at, 128, 100, 50, 128, 1) == alone
+    for both in (f(at, 100, at, 128, 100, 50, 100, 1), f(at, 128, C.c_void_p(4098), 128, 100, 50, 128, 1),
+                 f(at, 128, at, 129, 100, 50, 128, 1), f(at, 128, at, 128, 100, 50, 128, 0) - 150 * 128 * 2):
+        assert alone + 50 * 128 * 2 <= both < alone + 50 * 128 * 2 + 8192          # padded to 128; fp32: two pieces
     assert f(at, 128, at, 128, 30, 50, 128, 0) == 0                                # few rows: read in place by the forward
     assert f(at, 128, at, 128, 0, 50, 128, 0) == -1
 

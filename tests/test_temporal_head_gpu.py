@@ -356,6 +356,28 @@ def test_linear_ce_nothing_counts(dt):
     assert gx.shape == (0, 64) and not gw.any()
 
 
+@pytest.mark.parametrize("N,V,D", [(5, 300, 64), (70, 300, 64), (70, 300, 37), (130, 2000, 128), (90, 300, 320)])
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("dt", ALL, ids=IDS)
+def test_linear_ce_ignored_rows_may_hold_anything(dt, N, V, D, keep):
+    """padding: infinities, NaN and huge values in rows that do not count, the last one among them -- the same bits as with zeros there"""
+    x, w, labels = _ce_inputs(N, V, D, dt)
+    labels[::3] = -100
+    labels[-1] = -100
+    off = labels == -100
+    one, got = torch.ones((), device="cuda"), []
+    for bad in (False, True):
+        xb = torch.where(off[:, None], torch.zeros_like(x), x)
+        if bad:
+            junk = torch.tensor([float("nan"), float("inf"), float("-inf"), torch.finfo(dt).max], device="cuda", dtype=dt)
+            xb = torch.where(off[:, None], junk[torch.arange(N, device="cuda") % 4][:, None].expand(N, D), x).contiguous()
+        loss, nll, saved = ops.linear_ce(xb, w, labels, temperature=0.1, keep=keep)
+        got.append((loss, nll, *ops.linear_ce_bwd(xb, w, saved, one, temperature=0.1)))
+    assert all(bool(t.isfinite().all()) for t in got[1])
+    assert all(torch.equal(u, v) for u, v in zip(*got))
+    assert not got[1][2][off].any()
+
+
 def test_linear_ce_label_without_a_class_is_loud():
     x, w, labels = _ce_inputs(70, 300, 64, F32, ignore=0)
     for bad in (300, -1, 1 << 40, -(1 << 40)):
@@ -404,7 +426,7 @@ def test_linear_ce_kept_copies(dt):
     x, w, labels = _ce_inputs(90, 300, 100, dt)
     one = torch.ones((), device="cuda")
     a, b = ops.linear_ce(x, w, labels, temperature=0.1, keep=True), ops.linear_ce(x, w, labels, temperature=0.1)
-    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and a[2].numel() > b[2].numel()
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and a[2].numel() > b[2].numel()        # (x [90,100]: padded)
     ga, gb = (ops.linear_ce_bwd(x, w, t[2], one, temperature=0.1) for t in (a, b))
     assert all(torch.equal(u, v) for u, v in zip(ga, gb))
     for bad in (a[2][:100], b[2].half()):
@@ -413,16 +435,16 @@ def test_linear_ce_kept_copies(dt):
 
 
 def test_linear_ce_saved_tensors_come_back_laid_out_anew():
-    """16-bit features of 64: the view off its 16 bytes is copied by the forward, and read in place after its way over the host"""
+    """16-bit features of 64: the weight off its 16 bytes is copied by the forward, and read in place after its way over the host"""
     buf = torch.randn(90 * 64 + 1, device="cuda", dtype=F16)
-    w, labels = torch.randn(90, 64, device="cuda", dtype=F16), torch.randint(0, 90, (90,), device="cuda")
+    x, labels = torch.randn(90, 64, device="cuda", dtype=F16), torch.randint(0, 90, (90,), device="cuda")
     grads = []
     for hooks in (False, True):
-        x = buf[1:].view(90, 64).detach().requires_grad_(True)
-        wl = w.clone().requires_grad_(True)
+        wl = buf[1:].view(90, 64).detach().requires_grad_(True)
+        xl = x.clone().requires_grad_(True)
         with torch.autograd.graph.save_on_cpu() if hooks else contextlib.nullcontext():
-            loss, _ = loss_ops.linear_cross_entropy(x, wl, labels, temperature=4.0)
-        grads.append(torch.autograd.grad(loss, (x, wl)))
+            loss, _ = loss_ops.linear_cross_entropy(xl, wl, labels, temperature=4.0)
+        grads.append(torch.autograd.grad(loss, (xl, wl)))
     assert all(torch.equal(u, v) for u, v in zip(*grads))
 
 
