@@ -1046,9 +1046,12 @@ float ce_gscale_log2(const CePlan& q) { return q.dt16 == CRESTE_DT_F16 ? kCeF16L
 int ce_own(const CePlan& q, int mode) { return 256 * ce_nt(mode, q.P, q.Dp); }
 
 constexpr int kCeMaxima = 512;                     // blocks that look for an operand's largest magnitude
-// A piece of G: 128 MiB, which the memory-side cache still holds when DX and DW read it, but not under 16384 classes (shorter
-// contractions and a partial sum of dx per piece cost more than the cache gives), and never over 512 MiB
-constexpr int64_t kCePieceSmall = 128ll << 20, kCePieceClasses = 16384, kCePieceBytes = 512ll << 20;
+// A piece of G takes 64 to 512 MiB: ce_pieces() weighs what the rounds of workgroups, the launches and dx's partial sums cost against
+// the memory-side cache, which still holds 128 MiB when DX and DW read them.  Whole steps in us, always 128 MiB (16384 classes at least) /
+// always 512 MiB / chosen: 4096 x 131072 x 1024 bf16 4805 / 4880 / 4790, 8192 x 50000 x 512 fp16 2476 / 2370 / 2366, 1000 x 100000 x 768
+// bf16 930 / 877 / 874, 4096 x 65536 x 256 fp32 2195 / 2072 / 2070, 3000 x 30000 x 640 bf16 799 / 711 / 707
+constexpr int64_t kCeCached = 128ll << 20;
+constexpr int kCePieceMiB[] = {512, 384, 256, 192, 128, 64};
 
 // Up to 256 feature columns (fp32's two pieces: 128) the streaming kernels hold the own side in registers; beyond, G in memory
 bool ce_streams(int D, int dtype) { return D <= (dtype == CRESTE_DT_F32 ? 128 : 256); }
@@ -1068,7 +1071,7 @@ bool ce_few(const void* x, int64_t ld, int D, int dtype) {
 
 // splits of the contraction k, of those that fill one to eight rounds of workgroups: least rounds times the length of one (`start`: what its
 // beginning and end cost, in units of k)
-int ce_splits(int64_t tiles, int64_t k, int start) {
+int ce_splits(int64_t tiles, int64_t k, int start, int64_t* least = nullptr) {
   int best = 1;
   int64_t cost = (tiles + 255) / 256 * (k + start);
   for (int r = 1; r <= 8; ++r) {
@@ -1079,7 +1082,31 @@ int ce_splits(int64_t tiles, int64_t k, int start) {
     const int64_t c = (tiles * s + 255) / 256 * (up((k + s - 1) / s, 64) + start);
     if (c < cost) { cost = c; best = (int)s; }
   }
+  if (least) *least = cost;
   return best;
+}
+
+// classes per piece of G, and the splits of its DX and DW.  Costs in the time a workgroup takes for one step of the contraction (33 ns)
+void ce_pieces(CePlan& q, int64_t N, int64_t V, int D) {
+  const int64_t vall = up(V, kCeTile), col = q.n64 * 2 * q.P, mt = (D + kCeTile - 1) / kCeTile, nt = (N + kCeTile - 1) / kCeTile;
+  const int work = q.P == 2 ? 3 : 1;                           // products a step
+  double best = INFINITY;
+  for (const int mib : kCePieceMiB) {
+    int64_t vc = ((int64_t)mib << 20) / col / kCeTile * kCeTile;
+    vc = vc < kCeTile ? kCeTile : vc > vall ? vall : vc;
+    int64_t pieces = (vall + vc - 1) / vc;
+    vc = up((vall + pieces - 1) / pieces, kCeTile);            // pieces of one size
+    pieces = (vall + vc - 1) / vc;
+    if (vc == q.vc) continue;
+    int64_t cx, cw;
+    const int sx = ce_splits(mt * nt, vc, 256, &cx), sw = ce_splits(mt * (vc / kCeTile), q.n64, 256, &cw);
+    double cost = (double)((vc / kCeTile * nt + 255) / 256 * (q.Dp + 256) + cx + cw) * work + 450.;        // and three launches
+    if (pieces > 1) cost += 8e-6 * sx * N * q.ldq * 6.;        // dx's partial sums, read and written: 6 steps a MB
+    if (vc * col > kCeCached) cost += 1e-6 * vc * col * 9.;    // what the cache would have saved: 9 steps a MB of G
+    if (cost * pieces >= best) continue;
+    best = cost * pieces;
+    q.vc = vc; q.pieces = (int)pieces; q.sx = sx; q.sw = sw;
+  }
 }
 
 CePlan ce_plan(int64_t N, int64_t V, int D, int dtype, bool packx, bool packw, bool train) {
@@ -1117,20 +1144,9 @@ CePlan ce_plan(int64_t N, int64_t V, int D, int dtype, bool packx, bool packw, b
     q.sx = ce_splits((N + q.own - 1) / q.own, V, 320);
     q.sw = ce_splits((V + q.own - 1) / q.own, N, 320);
   } else {
-    const int64_t vall = up(V, kCeTile);
-    const int64_t col = q.n64 * 2 * q.P;                         // bytes of a class's column of G
-    int64_t vc = kCePieceSmall / col > kCePieceClasses ? kCePieceSmall / col : kCePieceClasses;
-    if (vc * col > kCePieceBytes) vc = kCePieceBytes / col;
-    vc = vc / kCeTile * kCeTile;
-    vc = vc < kCeTile ? kCeTile : vc > vall ? vall : vc;
-    q.pieces = (int)((vall + vc - 1) / vc);
-    q.vc = up((vall + q.pieces - 1) / q.pieces, kCeTile);        // pieces of one size
-    q.pieces = (int)((vall + q.vc - 1) / q.vc);
+    ce_pieces(q, N, V, D);
     q.ldg = q.vc * 2 + 256;          // (rows a power of two apart would meet in the same memory channels)
     q.g = take(q.n64 * q.ldg * q.P);
-    const int64_t mt = (D + kCeTile - 1) / kCeTile;
-    q.sx = ce_splits(mt * ((N + kCeTile - 1) / kCeTile), q.vc, 256);
-    q.sw = ce_splits(mt * (q.vc / kCeTile), q.n64, 256);
   }
   if (q.sx > 1 || q.pieces > 1) q.dxp = take((int64_t)q.sx * N * q.ldq * 4);
   if (q.sw > 1) q.dwp = take((int64_t)q.sw * q.vc * q.ldq * 4);

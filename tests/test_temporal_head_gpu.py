@@ -467,9 +467,11 @@ def test_linear_ce_is_deterministic():
             assert all(torch.equal(u, v) for u, v in zip(a, (loss, nll) + torch.autograd.grad(loss, (xa, wa))))
 
 
-def test_linear_ce_pieces(dt=BF16):
-    """more G than one piece holds: dx is added up over pieces, dw written piece by piece.  64-bit results on the GPU"""
-    N, V, D = 6000, 70000, 64
+@pytest.mark.parametrize("D", [64, 264])
+def test_linear_ce_pieces(D, dt=BF16):
+    """more G than one piece holds: streamed past, or (D > 256) dx added up over pieces and dw written piece by piece.  64-bit results on
+    the GPU"""
+    N, V = 6000, 70000
     x, w, labels = _ce_inputs(N, V, D, dt)
     lib = _lib.load()
     assert 2 * N * V > 512 << 20 and lib.creste_linear_ce_workspace_bytes(N, V, D, _lib.DT_BF16, 1) < 2 * N * V
