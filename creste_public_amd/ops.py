@@ -1482,14 +1482,14 @@ def _features(t, name: str, ndim=None, like=None) -> int:
 def _plain(t, dtype, shape, device, name: str) -> torch.Tensor:
     """a contiguous tensor of this type, shape and device -- or an error (values are copied if only the strides differ)"""
     if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device:
-        return t.contiguous()
+        return t if t.is_contiguous() else t.detach().contiguous()
     got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
     raise HipLibraryError(f"{name}: expected {dtype} {tuple(shape)} on {device}, got {got}")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """last dimension contiguous, no negative or overlapping-write concerns (the tensor is only read); copied otherwise"""
-    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.detach().contiguous()
 
 
 def _int64(v, name: str) -> int:
@@ -1536,8 +1536,8 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Te
         if residual.shape != x.shape:
             raise HipLibraryError(f"dropout: residual {tuple(residual.shape)} beside x {tuple(x.shape)}")
         _features(residual, "dropout: residual", like=x)
-        r_ = residual.detach().contiguous()
-    return _dropout(x.detach().contiguous(), r_, float(p), _int64(seed, "dropout: seed"), _int64(offset, "dropout: offset"), state, code)
+        r_ = residual if residual.is_contiguous() else residual.detach().contiguous()
+    return _dropout(x if x.is_contiguous() else x.detach().contiguous(), r_, float(p), _int64(seed, "dropout: seed"), _int64(offset, "dropout: offset"), state, code)
 
 
 def _dropout(x, residual, p, seed, offset, state, code):
@@ -1558,10 +1558,10 @@ def _recurrence_args(gate, x, h0, lengths):
         raise HipLibraryError(f"gated_recurrence: gate {tuple(gate.shape)} beside x {tuple(x.shape)}")
     B, T, Cc = gate.shape
     if h0 is not None:
-        h0 = _plain(h0.detach() if isinstance(h0, torch.Tensor) else h0, torch.float32, (B, Cc), gate.device, "gated_recurrence: h0")
+        h0 = _plain(h0, torch.float32, (B, Cc), gate.device, "gated_recurrence: h0")
     if lengths is not None:
         lengths = _plain(lengths, torch.int64, (B,), gate.device, "gated_recurrence: lengths")
-    return code, _rows(gate.detach()), _rows(x.detach()), h0, lengths
+    return code, _rows(gate), _rows(x), h0, lengths
 
 
 def gated_recurrence(gate: torch.Tensor, x: torch.Tensor, h0: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
@@ -1577,7 +1577,7 @@ def gated_recurrence(gate: torch.Tensor, x: torch.Tensor, h0: torch.Tensor | Non
     h = torch.empty((B, T, Cc), dtype=g_.dtype, device=dev)
     lib = _lib.load()
     if h.numel() == 0:
-        last = h0.clone() if h0 is not None else torch.zeros((B, Cc), dtype=torch.float32, device=dev)
+        last = h0.detach().clone() if h0 is not None else torch.zeros((B, Cc), dtype=torch.float32, device=dev)
         return (h, last, torch.empty(0, dtype=torch.float32, device=dev)) if save else (h, last)
     with _on(dev) as on:
         last = torch.empty((B, Cc), dtype=torch.float32, device=dev)
@@ -1640,7 +1640,7 @@ def _linear_ce_args(x, w, temperature, reduction):
         raise HipLibraryError(f"linear_cross_entropy: reduction {reduction!r} (mean or sum)")
     if not 0.0 < float(temperature) < float("inf"):
         raise HipLibraryError(f"linear_cross_entropy: temperature {temperature}")
-    return code, _rows(x.detach()), _rows(w.detach())
+    return code, _rows(x), _rows(w)
 
 
 def _ce_saved(N: int) -> int:
