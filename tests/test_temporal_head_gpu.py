@@ -718,7 +718,8 @@ def test_autograd_is_refused_inside_a_capture():
 
 
 @pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
-def test_head_in_two_captured_graphs(dt):
+@pytest.mark.parametrize("keep", [False, True])
+def test_head_in_two_captured_graphs(keep, dt):
     """forward and backward entry points captured; two graphs with workspaces of their own, replayed in turn with eager work between,
     new inputs and a new draw each time"""
     B, T, Cc, V = 3, 200, 64, 600
@@ -730,7 +731,7 @@ def test_head_in_two_captured_graphs(dt):
     def step(rng):
         h, last, st = ops.gated_recurrence(gate, x, h0, save=True)
         y = ops.dropout(h, 0.2, rng)
-        loss, nll, saved = ops.linear_ce(y.reshape(-1, Cc), w, labels, temperature=0.5)
+        loss, nll, saved = ops.linear_ce(y.reshape(-1, Cc), w, labels, temperature=0.5, keep=keep)
         gy, gw = ops.linear_ce_bwd(y.reshape(-1, Cc), w, saved, one, temperature=0.5)
         gg, gx, gh0 = ops.gated_recurrence_bwd(gate, x, None, st, ops.dropout(gy, 0.2, rng).reshape(B, T, Cc), last)
         return loss, nll, gw, gg, gx, gh0
