@@ -16,10 +16,13 @@
 // maximum's own term is left out of `rest` exactly (a comparison and two selections per logit: 4 % of a training step at 65536 classes,
 // where rows are rarely that sure), so that a confident row (rest << 1) keeps its loss to a few 2^-24 instead of 2^-24 / rest; for fp32
 // features the label's entry of G is expm1(-nll), so its gradient does too.
-// Precision.  16-bit features enter as they are, fp32 features as two fp16 pieces under one power-of-two scale per tensor
-// (22 significand bits; three products hi*hi + hi*lo + lo*hi, error <= 2^-21 of |x||w|).  Accumulation, the softmax statistics and
+// Precision.  16-bit features enter as they are, fp32 features as two fp16 pieces under one power-of-two scale per tensor: an element
+// is off by 2^-22 of itself or 2^-39 of the tensor's largest, whichever is more, and the three products hi*hi + hi*lo + lo*hi leave out
+// 2^-22 of |x||w|.  Where some row's largest magnitude lies more than 17 binades below the tensor's (so that the 2^-39 would reach its 22
+// bits), or anything is infinite or NaN, the operands stay fp32 and go through the fp32 matrix instruction (NATIVE; decided on the
+// device, call by call: ce_pack_kernel).  Accumulation, the softmax statistics and
 // the sums over splits are fp32.  G is rounded once to the operand type (bf16: 2^-8; fp16: 2^-11 relative, scaled by 2^14 so that
-// probabilities down to 2^-28 keep it; fp32 features: two fp16 pieces, 2^-22): the matrix cores take 16-bit operands.
+// probabilities down to 2^-28 keep it; fp32 features: two fp16 pieces, 2^-22 or 2^-39 of 1, NATIVE: none): the matrix cores take 16-bit operands.
 #include "common.h"
 
 namespace creste {
@@ -51,10 +54,10 @@ struct CeArgs {
   // LOSS / GRAD
   const int64_t* labels;
   int64_t ignore;
-  int class0;                       // first class of the piece
+  int class0;                       // GRAD, DX: first class of the piece
   int classes;                      // all classes
   float inv_tau;
-  const float* amax;                // [2] max|x|, max|w| (two-piece operands) or null
+  const float* amax;                // fp32: max|x|, max|w| (0 and 0 where `native`), native; else null
   float2* part;                     // LOSS: [class tile][n] (maximum, rest)
   float* zlab;                      // LOSS: [n] label logit, as maxima in the units of the products
   unsigned* done;                   // LOSS: the joining kernel's counter, cleared here
@@ -87,6 +90,13 @@ __device__ __forceinline__ float ce_operand_inv(const float* amax, int which) {
   return inv;
 }
 
+// fp32 features whose magnitudes two fp16 pieces do not hold: the copies are plain fp32 (ce_pack_kernel decides)
+template <int P>
+__device__ __forceinline__ bool ce_native(const CeArgs& p) {
+  if constexpr (P == 2) return p.amax[2] != 0.f;
+  return false;
+}
+
 // dloss / (tau * count) and the powers of two of the stored operands
 __device__ __forceinline__ float ce_out_scale(const CeArgs& p) {
   float s = p.gl[0] * p.inv_tau;
@@ -107,6 +117,13 @@ __device__ __forceinline__ cef16 ce_mfma(ces8 a, ces8 b, cef16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(ceb8, a), __builtin_bit_cast(ceb8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ceh8, a), __builtin_bit_cast(ceh8, b), c, 0, 0, 0);
+}
+
+// the same tile of fp32 operands, 4 floats a lane in alternate 16-byte pieces of the contraction: 8 elements of it
+__device__ __forceinline__ cef16 ce_mfma_native(cef4 a, cef4 b, cef16 c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+  return c;
 }
 
 template <int DT>
@@ -241,8 +258,8 @@ struct CeShape {
 
 // DT: 16-bit operand type (fp16 for two-piece fp32), P: pieces.  Bound: matrix rate, and for DX / DW reading G.  4096 x 131072 x 1024 bf16:
 // LOSS 1050 us (1050 TF/s), and for each of eight pieces of 16384 classes GRAD 160, DX 155-175, DW 140-150 us (780-980 TF/s)
-template <int MODE, int DT, int P, typename S>
-__global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
+template <int MODE, int DT, int P, typename S, bool NATIVE>
+__device__ __forceinline__ void ce_gemm_body(const CeArgs& p) {
   constexpr bool AKM = MODE == CE_DX || MODE == CE_DW, BKM = MODE == CE_DW;
   constexpr int BM = S::BM, BN = S::BN, BK = S::BK / P, NS = S::NS, NW = S::NW, WTM = BM / S::WM, WTN = BN / S::WN;
   constexpr int MT = WTM / 32, NT = WTN / 32;
@@ -271,6 +288,31 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
+  if constexpr (NATIVE) {
+    // 8 elements of the contraction a step, half a wave 4 of them: one 16-byte load where it runs along memory, four rows where across
+    auto load = [&](const char* base, int64_t ld, int64_t rows, int cols, bool across, int x, int k) __attribute__((always_inline)) {
+      cef4 v;
+      if (!across) return *reinterpret_cast<const cef4*>(base + (x < rows ? x : rows - 1) * 2 * ld + (k + 4 * lh) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t r = k + 4 * lh + e;
+        v[e] = *reinterpret_cast<const float*>(base + (r < rows ? r : rows - 1) * 2 * ld + (x < cols ? x : cols - 1) * 4);
+      }
+      return v;
+    };
+    const char* const first = p.a + (MODE == CE_GRAD || MODE == CE_DX ? p.class0 * p.lda : 0);      // (the piece's: rows are twice as long)
+    for (int k = kb; k < ke; k += 8) {
+      cef4 a[MT], b[NT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) a[i] = load(first, p.lda, p.ra, p.ca / 2, AKM, m0 + wm * WTM + i * 32 + li, k);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) b[j] = load(p.b, p.ldb, p.rb, p.cb / 2, BKM, n0 + wn * WTN + j * 32 + li, k);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = ce_mfma_native(a[i], b[j], acc[i][j]);
+    }
+  }
   auto dma = [&](int k, int s) __attribute__((always_inline)) {
     char* st = smem + s * STAGE;
 #pragma unroll
@@ -279,7 +321,7 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
       ce_dma<BN, BK, BKM, NW>(st + P * LA::BYTES + q * LB::BYTES, p.b + q * p.pb, p.ldb, p.rb, p.cb, n0, n0, k, wave, lane);
     }
   };
-  const int n = ke > kb ? (ke - kb) / BK : 0;
+  const int n = !NATIVE && ke > kb ? (ke - kb) / BK : 0;
 #pragma unroll
   for (int s = 0; s < NS - 1; ++s)
     if (s < n) dma(kb + s * BK, s);
@@ -392,6 +434,7 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
           for (int q = 0; q < 4; ++q) {
             const int cl = i * 32 + 8 * q + 4 * lh;
             ces4 hi, lo;
+            cef4 whole;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float z = acc[i][j][4 * q + e];
@@ -399,13 +442,19 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
               v = __builtin_amdgcn_exp2f(P == 2 ? v - rest : v);
               if (any) v = cl + e == yr ? (P == 2 ? gl : v - p.gscale) : v;
               if (mw + WTM > p.m) v = mw + cl + e < p.m ? v : 0.f;
+              whole[e] = v;
               const short h = ce_cvt<DT>(v);
               hi[e] = h;
               if constexpr (P == 2) lo[e] = ce_cvt<DT>(v - (float)__builtin_bit_cast(_Float16, h));
             }
+            if constexpr (NATIVE) {
+              if (row < p.n64) *reinterpret_cast<cef4*>(p.g + row * 2 * p.ldg + (mw + cl) * 4ll) = whole;
+              continue;
+            }
             *reinterpret_cast<ces4*>(ce_stage<RB>(st, li, cl * 2)) = hi;
             if constexpr (P == 2) *reinterpret_cast<ces4*>(ce_stage<RB>(st + 32 * RB, li, cl * 2)) = lo;
           }
+        if constexpr (NATIVE) continue;
         __builtin_amdgcn_wave_barrier();                // (a wave's LDS operations stay in order)
 #pragma unroll
         for (int q = 0; q < P; ++q)
@@ -422,6 +471,15 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
   } else {
     static_assert(NW * 32 * 512 <= NS * STAGE, "");
     ce_store<DT, MT, NT>(p, acc, smem + wave * (32 * 512), n0 + wn * WTN, m0 + wm * WTM, split, lane);
+  }
+}
+
+template <int MODE, int DT, int P, typename S>
+__global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
+  if (ce_native<P>(p)) {
+    if constexpr (P == 2) ce_gemm_body<MODE, DT, P, S, true>(p);
+  } else {
+    ce_gemm_body<MODE, DT, P, S, false>(p);
   }
 }
 
@@ -515,7 +573,7 @@ __device__ __forceinline__ void ce_interleave() {
 }
 
 // a = the streamed side (p.m items), b = the own side (p.n items), NT x 32 own items per wave
-template <int MODE, int DT, int P, int DP, int NT>
+template <int MODE, int DT, int P, int DP, int NT, bool NATIVE>
 __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int blocks) {
   using L = CeStream<DP, kCeStage, P>;
   constexpr int NS = 3, KS = DP / 16, kDma = P * L::INSTR / 8 + (MODE == CE_DW);
@@ -530,9 +588,15 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
   const int n = ke > kb ? (ke - kb + kCeStage - 1) / kCeStage : 0;
 
   ces8 x[P][NT][KS];
+  cef4 xn[NT][DP / 8];                       // native: 4 floats of every 8
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int64_t o = own0 + j * 32 + li, row = o < p.n ? o : p.n - 1;
+    if constexpr (NATIVE) {
+#pragma unroll
+      for (int kk = 0; kk < DP / 8; ++kk) xn[j][kk] = *reinterpret_cast<const cef4*>(p.b + row * 2 * p.ldb + kk * 32 + lh * 16);
+      continue;
+    }
 #pragma unroll
     for (int q = 0; q < P; ++q)
 #pragma unroll
@@ -576,15 +640,19 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
     if constexpr (MODE == CE_DW) L::dma_info(smem + s * L::BYTES, p, kb + c * kCeStage, wave, lane);
   };
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (the counted waits below count stages only)
+  if constexpr (!NATIVE) {
 #pragma unroll
-  for (int s = 0; s < NS - 1; ++s)
-    if (s < n) fill(s, s);
+    for (int s = 0; s < NS - 1; ++s)
+      if (s < n) fill(s, s);
+  }
   const unsigned rbase = L::row_base(lane), abase = L::across_base(lane);
   int cur = 0, nxt = NS - 1;
   for (int c = 0; c < n; ++c) {
-    if (c + NS - 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * kDma) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (c + NS - 1 < n) fill(c + NS - 1, nxt);
+    if constexpr (!NATIVE) {
+      if (c + NS - 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * kDma) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (c + NS - 1 < n) fill(c + NS - 1, nxt);
+    }
     const char* st = smem + cur * L::BYTES;             // (the rows' values behind the features)
 #pragma unroll 1
     for (int sub = 0; sub < kCeStage / 32; ++sub) {
@@ -595,6 +663,15 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[j][r] = 0.f;
+      if constexpr (NATIVE) {
+        const int64_t other = o0 + li < p.ra ? o0 + li : p.ra - 1;
+#pragma unroll
+        for (int kk = 0; kk < DP / 8; ++kk) {
+          const cef4 a = *reinterpret_cast<const cef4*>(p.a + other * 2 * p.lda + kk * 32 + lh * 16);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) z[j] = ce_mfma_native(a, xn[j][kk], z[j]);
+        }
+      } else {
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
         ces8 a[P];
@@ -610,6 +687,7 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
         }
       }
       ce_interleave<KS * P, NT * (P == 2 ? 3 : 1) * KS>();
+      }
       __builtin_amdgcn_sched_barrier(0);                // (the phases' operands do not fit the registers side by side)
       const bool edge = o0 + 32 > p.m;                  // others behind the last one
       ces8 g[P][NT][2];
@@ -654,7 +732,16 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
           for (int q = 0; q < 4; ++q) {
             cef4 rl, rr, rg;
             cei4 rb;
-            if constexpr (MODE == CE_DW) {              // of the others, which are rows here (padded to whole stages)
+            if constexpr (MODE == CE_DW && NATIVE) {    // of the others, which are rows here (padded to whole stages)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int64_t o = o0 + 8 * q + 4 * lh + e;
+                rl[e] = p.row_l2[o];
+                rb[e] = p.row_lab[o];
+                rr[e] = p.row_rest[o];
+                rg[e] = p.row_g[o];
+              }
+            } else if constexpr (MODE == CE_DW) {
               rl = *reinterpret_cast<const cef4*>(st + L::INFO + (sub * 32 + 8 * q + 4 * lh) * 4);
               rb = *reinterpret_cast<const cei4*>(st + L::INFO + 256 + (sub * 32 + 8 * q + 4 * lh) * 4);
               if constexpr (P == 2) {
@@ -677,6 +764,16 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
 #pragma unroll
               for (int r = 0; r < 16; ++r) v[r] = (r & 3) + 8 * (r >> 2) + 4 * lh == rel ? (P == 2 ? gl[j] : v[r] - p.gscale) : v[r];
           }
+          if constexpr (NATIVE) {                       // register r holds the others 8 (r / 4) + r % 4 of either half
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int64_t o = o0 + (r & 3) + 8 * (r >> 2) + 4 * lh;
+              const float* at = reinterpret_cast<const float*>(p.a + (o < p.ra ? o : p.ra - 1) * 2 * p.lda) + li;
+#pragma unroll
+              for (int d = 0; d < AT; ++d) acc[d][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[d * 32], v[r], acc[d][j], 0, 0, 0);
+            }
+            continue;
+          }
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const short h = ce_cvt<DT>(v[r]);
@@ -685,7 +782,7 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
           }
         }
       }
-      if constexpr (MODE != CE_LOSS) {
+      if constexpr (MODE != CE_LOSS && !NATIVE) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int d = 0; d < AT; ++d)
@@ -729,16 +826,25 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
 // own items per wave / 32: two where the registers hold them (for LOSS their features alone)
 constexpr int ce_nt(int mode, int P, int DP) { return P == 1 && (mode == CE_LOSS || DP == 64) ? 2 : 1; }
 
+template <int MODE, int DT, int P, int DP>
+__device__ __forceinline__ void ce_stream_either(const CeArgs& p, int block, int blocks) {
+  if (ce_native<P>(p)) {
+    if constexpr (P == 2) ce_stream_body<MODE, DT, P, DP, ce_nt(MODE, P, DP), true>(p, block, blocks);
+  } else {
+    ce_stream_body<MODE, DT, P, DP, ce_nt(MODE, P, DP), false>(p, block, blocks);
+  }
+}
+
 template <int DT, int P, int DP>
 __global__ __launch_bounds__(512, 2) void ce_loss_kernel(CeArgs p) {
-  ce_stream_body<CE_LOSS, DT, P, DP, ce_nt(CE_LOSS, P, DP)>(p, blockIdx.x, gridDim.x);
+  ce_stream_either<CE_LOSS, DT, P, DP>(p, blockIdx.x, gridDim.x);
 }
 
 // both gradients in one launch, the first nx workgroups dx: small problems leave CUs to each other
 template <int DT, int P, int DP>
 __global__ __launch_bounds__(512, 2) void ce_grad_kernel(CeArgs dx, CeArgs dw, int nx) {
-  if ((int)blockIdx.x < nx) ce_stream_body<CE_DX, DT, P, DP, ce_nt(CE_DX, P, DP)>(dx, blockIdx.x, nx);
-  else ce_stream_body<CE_DW, DT, P, DP, ce_nt(CE_DW, P, DP)>(dw, blockIdx.x - nx, gridDim.x - nx);
+  if ((int)blockIdx.x < nx) ce_stream_either<CE_DX, DT, P, DP>(dx, blockIdx.x, nx);
+  else ce_stream_either<CE_DW, DT, P, DP>(dw, blockIdx.x - nx, gridDim.x - nx);
 }
 
 // ------------------------------------------------------------------------------------------------------- few rows
@@ -855,49 +961,91 @@ struct CeSide {
   __device__ __forceinline__ bool off(int64_t r) const { return labels ? labels[r] == ignore : counts && counts[r] == INFINITY; }
 };
 
-// Each 16 lanes take whole rows, 4 columns a lane and step (no division by the row length).
-// amax: per block max |x| of its operand -> bmax[block]
-__global__ __launch_bounds__(256) void ce_amax_kernel(CeSide u, CeSide v, int cols, int split, float* __restrict__ bmax) {
-  __shared__ float sh[4];
+// What the blocks of ce_amax_kernel leave of an operand: max |x|, and the smallest exponent of a row's largest magnitude (rows of zeros
+// aside; 255: none)
+struct CeMax { unsigned bits; int low; };
+
+__device__ __forceinline__ CeMax ce_max_join(CeMax a, CeMax b) { return CeMax{max(a.bits, b.bits), min(a.low, b.low)}; }
+
+// over the 256 threads of a block
+__device__ __forceinline__ CeMax ce_max_block(CeMax m, CeMax (&sh)[4]) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = ce_max_join(m, CeMax{(unsigned)__shfl_xor((int)m.bits, o, 64), __shfl_xor(m.low, o, 64)});
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+  __syncthreads();
+  return ce_max_join(ce_max_join(sh[0], sh[1]), ce_max_join(sh[2], sh[3]));
+}
+
+// Each 16 lanes take whole rows, 4 columns a lane and step (no division by the row length).  Magnitudes as bit patterns: they order
+// alike, and a NaN counts as the largest
+__global__ __launch_bounds__(256) void ce_amax_kernel(CeSide u, CeSide v, int cols, int split, unsigned* __restrict__ bmax,
+                                                      uint8_t* __restrict__ blow) {
+  __shared__ CeMax sh[4];
   const bool second = (int)blockIdx.x >= split;
   const CeSide s = second ? v : u;
   const int blk = second ? blockIdx.x - split : blockIdx.x, nb = second ? gridDim.x - split : split;
   const int c0 = (threadIdx.x & 15) * 4;
-  float m = 0.f;
+  CeMax m{0, 255};
   for (int64_t r = (int64_t)blk * 16 + (threadIdx.x >> 4); r < s.rows; r += (int64_t)nb * 16) {
-    const float* x = (const float*)s.x + r * s.ld;
+    const unsigned* x = (const unsigned*)s.x + r * s.ld;
     if (s.off(r)) continue;
+    unsigned row = 0;
     for (int c = c0; c < cols; c += 64)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (c + e < cols) m = fmaxf(m, fabsf(x[c + e]));
+        if (c + e < cols) row = max(row, x[c + e] & 0x7fffffffu);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) row = max(row, (unsigned)__shfl_xor((int)row, o, 64));      // (the 16 lanes of a row are here together)
+    m = ce_max_join(m, CeMax{row, row ? (int)(row >> 23) : 255});
   }
-  m = wave_max(m);
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) bmax[blockIdx.x] = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+  m = ce_max_block(m, sh);
+  if (threadIdx.x == 0) {
+    bmax[blockIdx.x] = m.bits;
+    blow[blockIdx.x] = (uint8_t)m.low;
+  }
+}
+
+// Do two fp16 pieces under one power of two hold an operand's rows to 22 bits of each row's largest magnitude?  That magnitude may lie 17
+// binades below the tensor's (its low piece's steps are 2^-24 where the tensor's largest is 2^14 .. 2^15), nothing may be infinite or
+// NaN, and the tensor's largest not so small that no power of two brings it there
+__device__ __forceinline__ bool ce_even(CeMax m) {
+  const int e = m.bits >> 23;
+  return m.bits == 0 || (e >= 15 && e < 255 && e - m.low <= 17);
 }
 
 // 16-bit copy of the features with rows of cp (a multiple of 64) elements, zero behind the last column.  fp32: two pieces under
-// the power of two of the operand's max |x| (from the na[0] + na[1] block maxima; left in amax[0 / 1])
+// the power of two of the operand's max |x| (from the na0 + na1 blocks' maxima; left in amax[0 / 1]).  Where that does not hold either
+// operand's rows (ce_even), or the logits' unit leaves fp32's range, the copies are fp32 and amax[2] says so: the kernels then multiply
+// with the fp32 matrix instruction.  Pieces / one row 10^9 times the others, us a step: 19584 x 4096 x 128 376 / 1194, 4096 x 65536 x 256
+// 2062 / 6610
 template <typename T>
-__global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int cols, int cp, int split, const float* __restrict__ bmax,
-                                                      int na0, int na1, float* __restrict__ amax) {
+__global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int cols, int cp, int split, const unsigned* __restrict__ bmax,
+                                                      const uint8_t* __restrict__ blow, int na0, int na1, float inv_tau,
+                                                      float* __restrict__ amax) {
   const bool second = (int)blockIdx.x >= split;
   const CeSide s = second ? v : u;
   const int blk = second ? blockIdx.x - split : blockIdx.x, nb = second ? gridDim.x - split : split;
   float scale = 1.f;
+  bool native = false;
   if constexpr (sizeof(T) == 4) {
-    __shared__ float sh[4];
-    float m = 0.f;
-    for (int i = threadIdx.x; i < (second ? na1 : na0); i += 256) m = fmaxf(m, bmax[(second ? na0 : 0) + i]);
-    m = wave_max(m);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-    if (blk == 0 && threadIdx.x == 0) amax[second] = m;
-    float inv;
-    scale = f16_operand_scale(m, &inv);
+    __shared__ CeMax sh[4];
+    CeMax m[2] = {{0, 255}, {0, 255}};
+    for (int i = threadIdx.x; i < na0; i += 256) m[0] = ce_max_join(m[0], CeMax{bmax[i], blow[i]});
+    for (int i = threadIdx.x; i < na1; i += 256) m[1] = ce_max_join(m[1], CeMax{bmax[na0 + i], blow[na0 + i]});
+    float inv[2], sc[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      m[i] = ce_max_block(m[i], sh);
+      sc[i] = f16_operand_scale(__uint_as_float(m[i].bits), &inv[i]);
+    }
+    const float unit = inv[0] * inv[1], c2 = unit * inv_tau * kCeLog2e;
+    native = !ce_even(m[0]) || !ce_even(m[1]) || !(unit >= 0x1p-126f && c2 >= 0x1p-125f && c2 < INFINITY);
+    scale = sc[second];
+    if (blk == 0 && threadIdx.x == 0) {
+      amax[second] = native ? 0.f : __uint_as_float(m[second].bits);
+      if (!second) amax[2] = native ? 1.f : 0.f;
+    }
   }
   const int c0 = (threadIdx.x & 15) * 4;
   for (int64_t r = (int64_t)blk * 16 + (threadIdx.x >> 4); r < s.rows; r += (int64_t)nb * 16) {
@@ -905,10 +1053,12 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int co
     const int there = s.off(r) ? 0 : cols;
     for (int c = c0; c < cp; c += 64) {
       ces4 hi, lo;
+      cef4 whole;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const T v = c + e < there ? x[c + e] : (T)0;
         if constexpr (sizeof(T) == 4) {
+          whole[e] = v;
           const float a = v * scale;
           const short h = ce_cvt<CRESTE_DT_F16>(a);       // (a scalar: bit casts of vector elements are miscompiled)
           hi[e] = h;
@@ -917,6 +1067,11 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int co
           hi[e] = (short)v;
         }
       }
+      if constexpr (sizeof(T) == 4)
+        if (native) {
+          *reinterpret_cast<cef4*>((float*)s.out + r * cp + c) = whole;
+          continue;
+        }
       *reinterpret_cast<ces4*>(s.out + r * cp + c) = hi;
       if constexpr (sizeof(T) == 4) *reinterpret_cast<ces4*>(s.out + s.piece + r * cp + c) = lo;
     }
@@ -1123,7 +1278,7 @@ CePlan ce_plan(int64_t N, int64_t V, int D, int dtype, bool packx, bool packw, b
   q.packw = packw;
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 1024); return at; };
-  q.amax = take(64 + 2 * kCeMaxima * 4);           // the two maxima, the blocks' in front of them
+  q.amax = take(64 + 2 * kCeMaxima * 5);           // the two maxima and `native`; the blocks' maxima, and their lowest exponents
   q.xp = packx ? take(N * q.Dp * 2 * q.P) : 0;
   q.wp = packw ? take(V * q.Dp * 2 * q.P) : 0;
   q.packs = o + 32 * packw;                        // the size tells whether w is among them (all else is in whole 1024 bytes)
@@ -1227,9 +1382,11 @@ struct CeOperand { const char* p; int64_t ld, piece; };
 
 // the operands as the kernels read them, from `work` (the maxima and the copies at the offsets of the plan); copied there unless `ready`.
 // labels, ignore, counts: see CeSide
-int ce_operands(const CePlan& q, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int D, bool ready,
-                const int64_t* labels, int64_t ignore, const float* counts, char* work, CeOperand* X, CeOperand* W, hipStream_t s) {
-  float *amax = (float*)(work + q.amax), *bmax = amax + 16;
+int ce_operands(const CePlan& q, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int D, float inv_tau,
+                bool ready, const int64_t* labels, int64_t ignore, const float* counts, char* work, CeOperand* X, CeOperand* W, hipStream_t s) {
+  float* amax = (float*)(work + q.amax);
+  unsigned* bmax = (unsigned*)amax + 16;
+  uint8_t* blow = (uint8_t*)(bmax + 2 * kCeMaxima);
   *X = {(const char*)x, ldx * 2, 0};
   *W = {(const char*)w, ldw * 2, 0};
   if (q.packx) *X = {work + q.xp, (int64_t)q.Dp * 2, N * q.Dp * 2};
@@ -1241,10 +1398,10 @@ int ce_operands(const CePlan& q, const void* x, int64_t ldx, const void* w, int6
   const int px = q.packx ? blocks(N, 2048) : 0, pw = q.packw ? blocks(V, 2048) : 0;
   if (q.P == 2) {                                  // (both are copied)
     const int ax = blocks(N, kCeMaxima), aw = blocks(V, kCeMaxima);
-    ce_amax_kernel<<<ax + aw, 256, 0, s>>>(sx, sw, D, ax, bmax);
-    ce_pack_kernel<float><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, bmax, ax, aw, amax);
+    ce_amax_kernel<<<ax + aw, 256, 0, s>>>(sx, sw, D, ax, bmax, blow);
+    ce_pack_kernel<float><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, bmax, blow, ax, aw, inv_tau, amax);
   } else if (px + pw) {
-    ce_pack_kernel<short><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, nullptr, 0, 0, nullptr);
+    ce_pack_kernel<short><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, nullptr, nullptr, 0, 0, 0.f, nullptr);
   }
   CRESTE_CHECK_LAUNCH("linear_ce pack");
   return CRESTE_OK;
@@ -1304,7 +1461,7 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
   CeOperand X{(const char*)x, ldx * q.es, 0}, W{(const char*)w, ldw * q.es, 0};
   char* const copies = packs ? (char*)packs : wk;
   if (!few) {
-    const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, false, labels, ignore_index, nullptr, copies, &X, &W, s);
+    const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, 1.f / temperature, false, labels, ignore_index, nullptr, copies, &X, &W, s);
     if (rc) return rc;
   }
   CeArgs a{};
@@ -1348,7 +1505,7 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
   CeOperand X, W;
   const bool kept = packs && !ce_takes_few(x, ldx, w, ldw, N, D, dtype);
   char* const copies = kept ? (char*)packs : wk;
-  const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, kept, nullptr, 0, q.P == 2 ? rows + 2 * q.n64 : rows, copies, &X, &W, s);
+  const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, 1.f / temperature, kept, nullptr, 0, q.P == 2 ? rows + 2 * q.n64 : rows, copies, &X, &W, s);
   if (rc) return rc;
   CeArgs c{};                                       // what every product shares
   c.classes = (int)V;
@@ -1395,7 +1552,7 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
       if (gx) {
         dx.a = a.a; dx.lda = W.ld; dx.pa = W.piece; dx.ra = nv; dx.ca = q.Dp * 2;
         dx.b = a.g; dx.ldb = a.ldg; dx.pb = a.pg; dx.rb = q.n64;
-        dx.m = D;
+        dx.m = D; dx.class0 = (int)v0;
         dx.k1 = (int)up(nv, 64);
         dx.ksplit = q.sx > 1 ? (int)up(cdiv(q.vc, q.sx), 64) : 0;
         dx.accumulate = piece > 0;

@@ -1,0 +1,166 @@
+"""GPU: the operators of the temporal classification head where magnitudes, layouts and sizes are uneven, against 64-bit
+definitions."""
+import pytest
+import torch
+
+from creste_public_amd import _lib, loss_ops, ops, train_ops  # noqa: F401
+from tests import temporal_head_oracle as O
+from tests.temporal_head_oracle import within
+
+pytestmark = pytest.mark.gpu
+E = _lib.HipLibraryError
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# --------------------------------------------------------------------------------------- cross entropy, fp32 rows of uneven magnitude
+def _rowwise(x, w, labels, tau):
+    """64-bit results (reduction: sum) and bounds that hold row by row.  A factor x_ik is off by 2^-22 of its row's largest magnitude X_i,
+    w_jk by 2^-22 of W_j, a product of both remainders is left out (2^-22), and the fp32 sum of D terms is off by D 2^-24 of the magnitudes
+    it adds: e_ij = (2^-21 + (D + 8) 2^-24) sum |x||w| + 2^-22 (X_i sum |w_j| + W_j sum |x_i|), over tau.  The logits' errors move a
+    log-sum-exp to logsumexp(z + e) at most, and a probability to exp(z + e - (lse - e_lse)).  G is off by 2^-21 of its magnitude and
+    2^-39, sums over n by n 2^-24."""
+    x, w = x.double(), w.double()
+    N, D = x.shape
+    V = w.shape[0]
+    u = O.U32
+    z = x @ w.t() / tau
+    xm, wm = x.abs().amax(1, keepdim=True), w.abs().amax(1, keepdim=True)
+    e = ((2.0 ** -21 + (D + 8) * u) * (x.abs() @ w.abs().t()) + 2.0 ** -22 * (xm * w.abs().sum(1)[None] + wm.t() * x.abs().sum(1, keepdim=True))) / tau
+    lse = torch.logsumexp(z, 1)
+    on = labels != -100
+    col = labels.clamp(min=0)[:, None]
+    e_lse = torch.maximum(torch.logsumexp(z + e, 1) - lse, lse - torch.logsumexp(z - e, 1)) + (600 + 4 * lse.abs()) * u
+    nll = torch.where(on, lse - z.gather(1, col)[:, 0], torch.zeros_like(lse))
+    e_nll = e_lse + e.gather(1, col)[:, 0] + 8 * u * z.abs().gather(1, col)[:, 0]
+    p = torch.exp(z - lse[:, None])
+    hot = torch.zeros_like(z).scatter_(1, col, 1.0)
+    live = on[:, None].double()
+    G = (p - hot) * live
+    # (a probability is 1 at most; the argument's own roundings: 4 u of its magnitude)
+    up = torch.exp((z + e - (lse - e_lse)[:, None] + 4 * u * (z.abs() + lse.abs()[:, None])).clamp(max=0.0))
+    dn = torch.exp(z - e - (lse + e_lse)[:, None] - 4 * u * (z.abs() + lse.abs()[:, None]))
+    e_G = live * (torch.maximum(up - p, p - dn) + 2.0 ** -21 * (p + hot) + 2.0 ** -39)
+    mag = live * (p + hot)
+    gx, gw = G @ w / tau, G.t() @ x / tau
+    wq, xq = w.abs() + 2.0 ** -22 * wm, x.abs() + 2.0 ** -22 * xm
+    e_gx = (e_G @ wq + mag @ (2.0 ** -22 * wm.expand_as(w)) + (V + 64) * u * (mag @ w.abs())) / tau + 2 * u * gx.abs()
+    e_gw = (e_G.t() @ xq + mag.t() @ (2.0 ** -22 * xm.expand_as(x)) + (N + 64) * u * (mag.t() @ x.abs())) / tau + 2 * u * gw.abs()
+    return {k: v.cpu() for k, v in dict(nll=nll, e_nll=e_nll, gx=gx, e_gx=1.01 * e_gx, gw=gw, e_gw=1.01 * e_gw).items()}
+
+
+def _unit(n, d, seed):
+    t = torch.randn(n, d, generator=gen(seed))
+    return t / t.norm(dim=1, keepdim=True)
+
+
+def _uneven(N, V, D, seed=0):
+    """features scattered about their prototypes, some rows not counted"""
+    w, labels = _unit(V, D, seed), torch.randint(0, V, (N,), generator=gen(seed + 1))
+    x = w[labels] + torch.randn(N, D, generator=gen(seed + 2)) * (1.5 / D ** 0.5)
+    x = x / x.norm(dim=1, keepdim=True)
+    labels[3::7] = -100
+    return x.cuda(), w.cuda(), labels.cuda()
+
+
+def _uneven_check(x, w, labels, tau=0.1):
+    x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss, nll = loss_ops.linear_cross_entropy(x, w, labels, temperature=tau, reduction="sum")
+    gx, gw = torch.autograd.grad(loss, (x, w))
+    r = _rowwise(x.detach().cpu(), w.detach().cpu(), labels.cpu(), tau) if nll.numel() * w.shape[0] < 1 << 24 else \
+        _rowwise(x.detach(), w.detach(), labels, tau)
+    within(nll, r["nll"], r["e_nll"], "nll")
+    within(gx, r["gx"], r["e_gx"], "dx")
+    within(gw, r["gw"], r["e_gw"], "dw")
+
+
+SIZES = [(16, 1000, 128), (64, 1000, 128), (300, 257, 40), (90, 700, 300), (513, 300, 65)]
+
+
+@pytest.mark.parametrize("N,V,D", SIZES)
+@pytest.mark.parametrize("big", [1e4, 1e7, 1e9, 1e12])
+def test_linear_ce_f32_one_large_row(N, V, D, big):
+    x, w, labels = _uneven(N, V, D)
+    x[5] *= big
+    _uneven_check(x, w, labels)
+
+
+@pytest.mark.parametrize("N,V,D", SIZES)
+@pytest.mark.parametrize("big", [1e4, 1e7, 1e9, 1e12])
+def test_linear_ce_f32_one_large_class(N, V, D, big):
+    x, w, labels = _uneven(N, V, D)
+    w[V // 2] *= big
+    _uneven_check(x, w, labels)
+
+
+@pytest.mark.parametrize("N,V,D", SIZES)
+def test_linear_ce_f32_rows_over_many_magnitudes(N, V, D):
+    x, w, labels = _uneven(N, V, D)
+    _uneven_check(x * 10.0 ** torch.linspace(-8, 0, N, device="cuda")[:, None], w, labels)
+    _uneven_check(x, w * 10.0 ** torch.linspace(0, -8, V, device="cuda")[:, None], labels)
+    x[1], w[2] = 0.0, 0.0                                             # rows of zeros beside ordinary ones
+    _uneven_check(x, w, labels)
+
+
+@pytest.mark.parametrize("N,V,D", SIZES)
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_linear_ce_f32_one_row_that_is_not_finite(N, V, D, bad):
+    """its own loss is NaN, every other row's is right"""
+    x, w, labels = _uneven(N, V, D)
+    r = _rowwise(x.cpu(), w.cpu(), labels.cpu(), 0.1)
+    x[5, D // 2] = bad
+    loss, nll = loss_ops.linear_cross_entropy(x, w, labels, temperature=0.1)
+    assert not torch.isfinite(loss) and not torch.isfinite(nll[5])
+    keep = torch.arange(N) != 5
+    within(nll.cpu()[keep], r["nll"][keep], r["e_nll"][keep], "nll")
+
+
+@pytest.mark.parametrize("N,V,D", [(16, 33, 24), (70, 33, 24), (70, 65, 128), (70, 5, 300), (70, 300, 257)])
+@pytest.mark.parametrize("sx,sw", [(1e-20, 1e-20), (1e-30, 1e-15), (1e18, 1e-38), (1e-38, 1e18)])
+def test_linear_ce_f32_both_operands_tiny(N, V, D, sx, sw):
+    """products that vanish beside 1: the loss of every row is log V; and magnitudes at the two ends of the type's range"""
+    x, w, labels = _uneven(N, V, D)
+    _uneven_check(x * sx, w * sw, labels)
+
+
+@pytest.mark.parametrize("big", [1.0, 1e9])
+def test_linear_ce_f32_uneven_rows_in_pieces_of_the_classes(big):
+    """more G than one piece holds (2048 x 80000 x 4 bytes > 512 MiB); 64-bit results on the GPU"""
+    x, w, labels = _uneven(2048, 80000, 136)
+    x[5] *= big
+    w[70000] *= big
+    _uneven_check(x, w, labels)
+
+
+@pytest.mark.parametrize("D", [100, 300])
+def test_linear_ce_f32_even_and_uneven_rows_in_one_graph(D):
+    """which way the products are formed is decided on the device, call by call: a captured step replayed with either kind of features;
+    the forward's copies kept for the backward or made anew give the same bits"""
+    N, V = 200, 500
+    x, w, labels = _uneven(N, V, D)
+    one, far = torch.ones((), device="cuda"), torch.ones(N, 1, device="cuda")
+    far[7] = 1e10
+    kinds = [x * far, x.clone(), x * far.flip(0)]
+
+    def step(keep):
+        loss, nll, saved = ops.linear_ce(x, w, labels, temperature=0.1, keep=keep)
+        return (loss, nll, *ops.linear_ce_bwd(x, w, saved, one, temperature=0.1))
+    want = []
+    for k in kinds:
+        x.copy_(k)
+        want.append([t.clone() for t in step(True)])
+        assert all(torch.equal(a, b) for a, b in zip(want[-1], step(False)))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(True)
+    for rep in range(2):
+        for k, ref in zip(kinds, want):
+            x.copy_(k)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(ref, out))
+            step(True)
