@@ -164,3 +164,32 @@ def test_linear_ce_f32_even_and_uneven_rows_in_one_graph(D):
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(ref, out))
             step(True)
+
+
+# ------------------------------------------------------------------------------ cross entropy, 16 bit: rows surer than 2^-24
+def _margin_bounds(x, w, labels, tau):
+    """64-bit nll and how far it may be off: 16-bit products are exact, a fp32 sum of D terms is off by (D + 8) 2^-24 of their magnitudes,
+    a difference of two logits by both and four roundings, and nll = log(1 + sum over the other classes of exp(-margin)) is as sure,
+    relatively, as the margins (and 64 roundings)"""
+    x, w = x.double(), w.double()
+    col = labels[:, None]
+    z = x @ w.t() / tau
+    e = (x.shape[1] + 8) * O.U32 * (x.abs() @ w.abs().t()) / tau
+    d = z - z.gather(1, col)
+    e = e + e.gather(1, col) + 4 * O.U32 * (z.abs() + z.abs().gather(1, col))
+    other = torch.ones_like(z).scatter_(1, col, 0.0)
+    nll, up = torch.log1p((torch.exp(d) * other).sum(1)), torch.log1p((torch.exp(d + e) * other).sum(1))
+    return nll, (up - nll) + 64 * O.U32 * nll
+
+
+@pytest.mark.parametrize("dt", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("N,V,D", [(24, 1500, 64), (300, 1025, 64), (300, 5000, 256), (70, 70000, 128), (300, 1025, 320), (70, 9000, 512)])
+def test_linear_ce_16_bit_confident_rows(N, V, D, dt):
+    """logits of 10 to 500, the label's far in front: the loss is never negative and keeps its digits"""
+    w = _unit(V, D, V).to(dt).cuda()
+    labels = torch.randint(0, V, (N,), generator=gen(N)).cuda()
+    x = (w[labels].float() * torch.logspace(-0.7, 1.0, N, device="cuda")[:, None]).to(dt)
+    loss, nll = loss_ops.linear_cross_entropy(x, w, labels, temperature=0.02, reduction="sum")
+    want, bound = _margin_bounds(x.cpu(), w.cpu(), labels.cpu(), 0.02)
+    assert float(nll.min()) >= 0.0 and float(want.min()) < 2.0 ** -30
+    within(nll, want, bound, "nll")
