@@ -1085,28 +1085,31 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int co
   }
 }
 
-// per row: join the class tiles' (maximum, rest); 64 rows x 16 slices of the tiles per block.  Leaves nll, what the gradient kernels ask
-// of a row (padded to whole tiles: rows that do not count get an infinite log-sum-exp, hence G = 0, a label that names no class a
-// NaN), and, from the last block to finish, the loss: sums of the blocks' sums in their order, so the result does not depend on which
-// that was.  Maxima and label logits come in the units of the products.  two: fp32 features, the log-sum-exp in two parts
-__global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ part, int tiles, int n, const float* __restrict__ zlab,
-                                                       const int64_t* __restrict__ labels, int64_t ignore, int classes, int two,
-                                                       const float* __restrict__ amax, float inv_tau, float log2_scale,
-                                                       float* __restrict__ nll, float* __restrict__ rows, uint64_t* __restrict__ bsum,
-                                                       unsigned* __restrict__ done, int mean, float* __restrict__ loss,
-                                                       float* __restrict__ stat) {
+// per row: join the class tiles' (maximum, rest); 64 rows x 16 slices of the tiles per block and turn (blocks of rows).  Leaves nll, what
+// the gradient kernels ask of a row (padded to whole tiles: rows that do not count get an infinite log-sum-exp, hence G = 0, a label that
+// names no class a NaN), and, from the last block to finish, the loss: sums of the blocks' sums in their order, so the result does not
+// depend on which that was.  Maxima and label logits come in the units of the products.  two: fp32 features, the log-sum-exp in two parts
+__global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ part, int tiles, int n, int blocks,
+                                                       const float* __restrict__ zlab, const int64_t* __restrict__ labels, int64_t ignore,
+                                                       int classes, int two, const float* __restrict__ amax, float inv_tau,
+                                                       float log2_scale, float* __restrict__ nll, float* __restrict__ rows,
+                                                       uint64_t* __restrict__ bsum, unsigned* __restrict__ done, int mean,
+                                                       float* __restrict__ loss, float* __restrict__ stat) {
   __shared__ float2 sh[16][64];
   __shared__ bool last;
   const int li = threadIdx.x & 63, sl = threadIdx.x >> 6;
-  const int row = blockIdx.x * 64 + li, n64 = gridDim.x * 64;
+  const int64_t n64 = blocks * 64ll;
   const float c2 = ce_operand_inv(amax, 0) * ce_operand_inv(amax, 1) * inv_tau * kCeLog2e;      // (as the loss kernels')
-  float2 st = make_float2(-3.0e38f, -1.f);
-  if (row < n)
+  for (int blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
+    const int64_t row = blk * 64ll + li;
+    float2 st = make_float2(-3.0e38f, -1.f);
+    if (row < n)
 #pragma unroll 4
-    for (int t = sl; t < tiles; t += 16) st = ce_merge(st, part[(int64_t)t * n + row], c2);
-  sh[sl][li] = st;
-  __syncthreads();
-  if (sl == 0) {
+      for (int t = sl; t < tiles; t += 16) st = ce_merge(st, part[(int64_t)t * n + row], c2);
+    if (blk != (int)blockIdx.x) __syncthreads();        // (everybody has left the turn before)
+    sh[sl][li] = st;
+    __syncthreads();
+    if (sl != 0) continue;
     for (int s = 1; s < 16; ++s) st = ce_merge(st, sh[s][li], c2);
     float l = 0.f, c = 0.f;
     const int64_t y = row < n ? labels[row] : ignore;
@@ -1127,18 +1130,18 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
       l += __shfl_xor(l, o, 64);
       c += __shfl_xor(c, o, 64);
     }
-    if (li == 0) {                                      // one word, written through; the count when it has arrived
-      __hip_atomic_store(bsum + blockIdx.x, (uint64_t)__float_as_uint(c) << 32 | __float_as_uint(l), __ATOMIC_RELAXED,
-                         __HIP_MEMORY_SCOPE_AGENT);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      last = atomicAdd(done, 1u) == gridDim.x - 1;
-    }
+    if (li == 0)                                        // one word, written through; counted when it has arrived
+      __hip_atomic_store(bsum + blk, (uint64_t)__float_as_uint(c) << 32 | __float_as_uint(l), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (threadIdx.x == 0) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    last = atomicAdd(done, 1u) == gridDim.x - 1;
   }
   __syncthreads();
   if (!last) return;
   __shared__ double sl_[1024], sc_[1024];
   double l = 0., c = 0.;
-  for (int i = threadIdx.x; i < (int)gridDim.x; i += 1024) {
+  for (int i = threadIdx.x; i < blocks; i += 1024) {
     const uint64_t v = __hip_atomic_load(bsum + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     l += __uint_as_float((unsigned)v);
     c += __uint_as_float((unsigned)(v >> 32));
@@ -1209,6 +1212,7 @@ struct CePlan {
 float ce_gscale_log2(const CePlan& q) { return q.dt16 == CRESTE_DT_F16 ? kCeF16Log2 : 0.f; }
 int ce_own(const CePlan& q, int mode) { return 256 * ce_nt(mode, q.P, q.Dp); }
 
+constexpr int kCeJoinBlocks = 1 << 20;             // (a launch holds less than 2^32 threads: of 1024 a block)
 constexpr int kCeMaxima = 512;                     // blocks that look for an operand's largest magnitude
 // A piece of G takes 64 to 512 MiB: ce_pieces() weighs what the rounds of workgroups, the launches and dx's partial sums cost against
 // the memory-side cache, which still holds 128 MiB when DX and DW read them.  Whole steps in us, always 128 MiB (16384 classes at least) /
@@ -1324,12 +1328,12 @@ template <int MODE, int DT, int P, typename S>
 int ce_launch(CeArgs a, int splits, hipStream_t s) {
   constexpr int bytes = S::NS * (S::BM + S::BN) * S::BK * 2;
   static std::atomic<uint64_t> mask{0};
-  CRESTE_HIP(ensure_dyn_smem((const void*)ce_gemm_kernel<MODE, DT, P, S>, bytes, mask));
   static_assert(S::BM == kCeTile, "");
   if (MODE != CE_GRAD) a.mt = cdiv(a.m, S::BM);          // (GRAD: given, the zeros behind the last class too)
   a.nt = cdiv(a.n, S::BN);
   const int64_t blocks = (int64_t)a.mt * a.nt * splits;
-  CRESTE_REQUIRE(blocks < (1ll << 31), "linear_ce: too many tiles");
+  CRESTE_REQUIRE(blocks * S::NW * 64 < (1ll << 32), "linear_ce: too many tiles for a launch");
+  CRESTE_HIP(ensure_dyn_smem((const void*)ce_gemm_kernel<MODE, DT, P, S>, bytes, mask));
   ce_gemm_kernel<MODE, DT, P, S><<<(int)blocks, S::NW * 64, bytes, s>>>(a);
   CRESTE_CHECK_LAUNCH("linear_ce gemm");
   return CRESTE_OK;
@@ -1357,7 +1361,7 @@ int ce_stream_launch(const CePlan& q, CeArgs* loss, CeArgs* dx, CeArgs* dw, hipS
   static std::atomic<uint64_t> mask_loss{0}, mask_grad{0};
   const int64_t nl = loss ? ce_stream_blocks(*loss, q.own, q.sl) : 0, nx = dx ? ce_stream_blocks(*dx, q.own, q.sx) : 0,
                 nw = dw ? ce_stream_blocks(*dw, q.own, q.sw) : 0;
-  CRESTE_REQUIRE(nl + nx + nw < (1ll << 31), "linear_ce: too many tiles");
+  CRESTE_REQUIRE((nl + nx + nw) * 512 < (1ll << 32), "linear_ce: too many tiles for a launch");
   if (loss) {
     CRESTE_HIP(ensure_dyn_smem((const void*)ce_loss_kernel<DT, P, DP>, stages, mask_loss));
     ce_loss_kernel<DT, P, DP><<<(int)nl, 512, stages, s>>>(*loss);
@@ -1462,6 +1466,8 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
                            false);
   CRESTE_REQUIRE(loss && nll && rows && stat && work && work_bytes >= q.total, "linear_ce_forward: outputs / workspace (%lld of %lld bytes)",
                  (long long)work_bytes, (long long)q.total);
+  CRESTE_REQUIRE(q.stream || few || (int64_t)q.tiles * ((N + 255) / 256) * 512 < (1ll << 32),
+                 "linear_ce_forward: too many tiles for a launch (2^23 of 256 x 256) at N %lld V %lld", (long long)N, (long long)V);
   CRESTE_REQUIRE((((uintptr_t)work | (uintptr_t)packs) & 15) == 0, "linear_ce_forward: work and packs on 16-byte boundaries");
   hipStream_t s = (hipStream_t)stream;
   char* wk = (char*)work;
@@ -1489,10 +1495,10 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
     const int rg = q.stream ? ce_stream(q, &a, nullptr, nullptr, s) : ce_gemm<CE_LOSS>(q, a, 1, s);
     if (rg) return rg;
   }
-  const int nb = cdiv(N, 64);
-  ce_join_kernel<<<nb, 1024, 0, s>>>(a.part, q.stream && !few ? q.sl : q.tiles, (int)N, a.zlab, labels, ignore_index, (int)V, q.P == 2,
-                                     few ? nullptr : a.amax, a.inv_tau, ce_gscale_log2(q), nll, rows, (uint64_t*)(wk + q.bsum), a.done,
-                                     mean, loss, stat);
+  const int nb = (int)((N + 63) / 64);
+  ce_join_kernel<<<nb < kCeJoinBlocks ? nb : kCeJoinBlocks, 1024, 0, s>>>(
+      a.part, q.stream && !few ? q.sl : q.tiles, (int)N, nb, a.zlab, labels, ignore_index, (int)V, q.P == 2, few ? nullptr : a.amax, a.inv_tau,
+      ce_gscale_log2(q), nll, rows, (uint64_t*)(wk + q.bsum), a.done, mean, loss, stat);
   CRESTE_CHECK_LAUNCH("linear_ce join");
   return CRESTE_OK;
 }

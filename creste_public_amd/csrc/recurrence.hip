@@ -398,7 +398,7 @@ int rec_launch(RecArgs& p, bool bwd, char* work, hipStream_t s) {
   int64_t nw = (p.T + LR - 1) / LR;
   nw = nw > kRecWaves ? kRecWaves : nw;
   const int64_t chunks = (p.T + nw * LR - 1) / (nw * LR);
-  CRESTE_REQUIRE(groups * chunks < (1ll << 31), "gated_recurrence: too many columns and chunks of steps");
+  CRESTE_REQUIRE(groups * chunks * 64 < (1ll << 32), "gated_recurrence: too many columns and chunks of steps for a launch (2^26 workgroups)");
   p.chunks = (int)chunks;
   p.groups = (int)groups;
   if (chunks > 1) {

@@ -193,3 +193,25 @@ def test_linear_ce_16_bit_confident_rows(N, V, D, dt):
     want, bound = _margin_bounds(x.cpu(), w.cpu(), labels.cpu(), 0.02)
     assert float(nll.min()) >= 0.0 and float(want.min()) < 2.0 ** -30
     within(nll, want, bound, "nll")
+
+
+# ------------------------------------------------------------------------------------------------------------ very many rows
+def test_linear_ce_more_than_2_29_rows():
+    """four words a row for the backward pass 2^31 words; rows at both ends and around 2^29, all others ignored"""
+    N, V, D = (1 << 29) + 1000, 5, 8
+    w = _unit(V, D, 1).to(BF16).cuda()
+    at = torch.tensor([0, 1, 65, (1 << 28) + 7, (1 << 29) - 1, 1 << 29, (1 << 29) + 63, N - 1], device="cuda")
+    lab = torch.full((N,), -100, device="cuda")
+    lab[at] = torch.arange(8, device="cuda") % V
+    x = torch.zeros(N, D, dtype=BF16, device="cuda")
+    x[at] = torch.randn(8, D, generator=gen(2)).to(BF16).cuda()
+    loss, nll, saved = ops.linear_ce(x, w, lab, reduction="sum")
+    r = O.linear_ce(x[at], w, lab[at], -100, 1.0, False)
+    within(nll[at], r["nll"], r["e_nll"], "nll")
+    assert int(torch.count_nonzero(nll)) == 8 and abs(float(loss) - float(r["loss"])) <= float(r["e_loss"])
+    del lab
+    gx, gw = ops.linear_ce_bwd(x, w, saved, torch.ones((), device="cuda"), reduction="sum")
+    within(gx[at], r["gx"], r["e_gx"], "dx")
+    within(gw, r["gw"], r["e_gw"], "dw")
+    gx[at] = 0
+    assert not gx[:1 << 20].any() and not gx[-(1 << 20):].any() and not gx[(1 << 29) - 4096:(1 << 29) + 1000].any()
