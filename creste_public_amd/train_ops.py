@@ -22,6 +22,7 @@ import ctypes as C
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
@@ -611,7 +612,10 @@ def reward_forward_train(net, x: torch.Tensor) -> torch.Tensor:
 def recorded(*tensors) -> bool:
     """does autograd record an operation on these (else the Function around it is only overhead).  Not inside a stream capture: a
     captured backward whose leaves also belong to a live eager graph ties the capture to the eager stream and ends the process, and
-    whether such a graph lives cannot be seen from here.  A captured step calls the two halves in `ops` itself."""
+    whether such a graph lives cannot be seen from here.  A captured step calls the two halves in `ops` itself.
+    Raises for a tensor with a forward-mode tangent, as a Function does: the operators have no forward-mode derivative."""
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode derivatives of dropout, gated_recurrence and linear_cross_entropy are not implemented")
     if not torch.is_grad_enabled() or not any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
         return False
     if any(isinstance(t, torch.Tensor) and t.is_cuda for t in tensors) and torch.cuda.is_current_stream_capturing():

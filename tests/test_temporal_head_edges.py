@@ -1,7 +1,11 @@
 """CPU: sizes that the operators of the temporal classification head refuse before anything is launched, and what their host side decides."""
 import ctypes as C
 
-from creste_public_amd import _lib
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from creste_public_amd import _lib, loss_ops, train_ops
 
 P = C.c_void_p(4096)                       # never dereferenced
 
@@ -21,3 +25,25 @@ def test_launches_of_more_threads_than_the_device_takes_are_refused():
     N = V = 1 << 20
     rc = lib.creste_linear_ce_forward(P, 512, P, 512, P, N, V, 512, 1, -100, 1.0, 1, P, P, P, P, None, P, 1 << 62, None)
     _refused(rc, b"too many tiles")
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("call", [
+    lambda d, p: train_ops.dropout(d, 0.5, 1), lambda d, p: train_ops.dropout(p, 0.5, 1, residual=d),
+    lambda d, p: train_ops.gated_recurrence(d, p), lambda d, p: train_ops.gated_recurrence(p, d),
+    lambda d, p: train_ops.gated_recurrence(p, p, d[:, 0]),
+    lambda d, p: loss_ops.linear_cross_entropy(d, p[0], torch.zeros(2, 3, dtype=torch.long)),
+    lambda d, p: loss_ops.linear_cross_entropy(p, d[0], torch.zeros(2, 3, dtype=torch.long))])
+def test_forward_mode_derivatives_are_refused(call, grad):
+    """a tangent that were dropped would read as a derivative of 0; also where nothing is recorded for a backward"""
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        d = forward_ad.make_dual(torch.randn(2, 3, 4), torch.ones(2, 3, 4))
+        with pytest.raises(NotImplementedError):
+            call(d, torch.randn(2, 3, 4))
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(lambda t: call(t, torch.randn(2, 3, 4)), (torch.randn(2, 3, 4),), (torch.ones(2, 3, 4),))
+
+
+def test_a_level_without_tangents_is_no_obstacle():
+    with forward_ad.dual_level():
+        assert train_ops.recorded(torch.randn(3)) is False and train_ops.recorded(torch.randn(3, requires_grad=True), None) is True
