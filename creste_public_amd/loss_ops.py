@@ -190,6 +190,7 @@ def linear_cross_entropy(x, weight, labels, ignore_index: int = -100, temperatur
     """Cross entropy of the linear classifier `weight` [V,D] on features x [...,D] (fp32 / bf16 / fp16, one type for both) against
     labels [...] int64, over any number of classes and without ever holding the N x V logits:
         z = x weight^T / temperature;  nll = logsumexp(z) - z[label], 0 where label == ignore_index
+    (temperature is a number, without a gradient: a learned one divides x before the call)
     -> (loss, nll): loss = mean of nll over the rows that count (0 when none does) or their sum, a differentiable fp32 scalar;
     nll [...] fp32, not differentiable.  The features of ignored rows may be anything (infinite, NaN: padding); their gradient is 0.  A label
     that names neither a class nor ignore_index makes the loss and its gradients NaN.  fp32 features are multiplied with 22 significand bits

@@ -1500,6 +1500,13 @@ def _int64(v, name: str) -> int:
     return v - (1 << 64) if v >= (1 << 63) else v
 
 
+def _number(v, name: str) -> float:
+    """a plain number: a tensor would be read back to the host, and no gradient would reach it"""
+    if isinstance(v, torch.Tensor):
+        raise HipLibraryError(f"{name}: a number expected, got a tensor (there is no gradient for it)")
+    return float(v)
+
+
 class _on:
     """make `device` the current one for a call; `.stream` = its current stream"""
     __slots__ = ("dev", "prev", "stream")
@@ -1525,8 +1532,9 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Te
     Philox4x32-10 per element, compared with round(p 2^32).  Calls that shall draw independently take different offsets (or seeds).
     `seed`: an int, or a CUDA int64 tensor (seed, offset) read when the kernel runs, so that a captured call can draw anew
     on each replay (its second element is added to `offset`)."""
+    p = _number(p, "dropout: p")
     code = _features(x, "dropout: x")
-    if not 0.0 <= float(p) <= 1.0:
+    if not 0.0 <= p <= 1.0:
         raise HipLibraryError(f"dropout: p = {p} outside [0, 1]")
     state = None
     if isinstance(seed, torch.Tensor):
@@ -1537,7 +1545,7 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Te
             raise HipLibraryError(f"dropout: residual {tuple(residual.shape)} beside x {tuple(x.shape)}")
         _features(residual, "dropout: residual", like=x)
         r_ = residual if residual.is_contiguous() else residual.detach().contiguous()
-    return _dropout(x if x.is_contiguous() else x.detach().contiguous(), r_, float(p), _int64(seed, "dropout: seed"), _int64(offset, "dropout: offset"), state, code)
+    return _dropout(x if x.is_contiguous() else x.detach().contiguous(), r_, p, _int64(seed, "dropout: seed"), _int64(offset, "dropout: offset"), state, code)
 
 
 def _dropout(x, residual, p, seed, offset, state, code):
@@ -1632,13 +1640,14 @@ def _recurrence_bwd(gate, x, lengths, starts, gh, gh_last, code):
 
 
 def _linear_ce_args(x, w, temperature, reduction):
+    temperature = _number(temperature, "linear_cross_entropy: temperature")
     code = _features(x, "linear_cross_entropy: x", 2)
     _features(w, "linear_cross_entropy: weight", 2, like=x)
     if w.shape[1] != x.shape[1] or w.shape[0] < 1 or w.shape[1] < 1:
         raise HipLibraryError(f"linear_cross_entropy: x {tuple(x.shape)} beside weight {tuple(w.shape)}")
     if reduction not in ("mean", "sum"):
         raise HipLibraryError(f"linear_cross_entropy: reduction {reduction!r} (mean or sum)")
-    if not 0.0 < float(temperature) < float("inf"):
+    if not 0.0 < temperature < float("inf"):
         raise HipLibraryError(f"linear_cross_entropy: temperature {temperature}")
     return code, _rows(x), _rows(w)
 

@@ -5,7 +5,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from creste_public_amd import _lib, loss_ops, train_ops
+from creste_public_amd import _lib, loss_ops, ops, train_ops
 
 P = C.c_void_p(4096)                       # never dereferenced
 
@@ -47,3 +47,13 @@ def test_forward_mode_derivatives_are_refused(call, grad):
 def test_a_level_without_tangents_is_no_obstacle():
     with forward_ad.dual_level():
         assert train_ops.recorded(torch.randn(3)) is False and train_ops.recorded(torch.randn(3, requires_grad=True), None) is True
+
+
+def test_tensors_in_the_place_of_numbers_are_refused():
+    """they would be read back to the host, and their gradient would be None without a word"""
+    x, w, lab = torch.randn(3, 4), torch.randn(5, 4), torch.zeros(3, dtype=torch.long)
+    for t in (torch.tensor(0.1), torch.tensor(0.1, requires_grad=True), torch.nn.Parameter(torch.ones(()))):
+        for call in (lambda: loss_ops.linear_cross_entropy(x, w, lab, temperature=t), lambda: ops.linear_ce(x, w, lab, -100, t),
+                     lambda: ops.linear_ce_bwd(x, w, x, x, temperature=t), lambda: train_ops.dropout(x, t, 1), lambda: ops.dropout(x, t, 1)):
+            with pytest.raises(_lib.HipLibraryError, match="a number expected"):
+                call()
