@@ -1212,6 +1212,7 @@ struct CePlan {
 float ce_gscale_log2(const CePlan& q) { return q.dt16 == CRESTE_DT_F16 ? kCeF16Log2 : 0.f; }
 int ce_own(const CePlan& q, int mode) { return 256 * ce_nt(mode, q.P, q.Dp); }
 
+constexpr int kCeFewRows = 32;
 constexpr int kCeJoinBlocks = 1 << 20;             // (a launch holds less than 2^32 threads: of 1024 a block)
 constexpr int kCeMaxima = 512;                     // blocks that look for an operand's largest magnitude
 // A piece of G takes 64 to 512 MiB: ce_pieces() weighs what the rounds of workgroups, the launches and dx's partial sums cost against
@@ -1228,8 +1229,6 @@ int ce_padded(int D, int dtype) { return ce_streams(D, dtype) ? (D <= 64 ? 64 : 
 bool ce_direct(const void* x, int64_t ld, int D, int dtype) {
   return dtype != CRESTE_DT_F32 && D == ce_padded(D, dtype) && ld % 8 == 0 && ld < (1 << 24) && ((uintptr_t)x & 15) == 0;
 }
-
-constexpr int kCeFewRows = 32;
 
 // rows that the few-rows kernel can read in place: whole 32-byte steps on 16-byte boundaries
 bool ce_few(const void* x, int64_t ld, int D, int dtype) {
@@ -1297,7 +1296,8 @@ CePlan ce_plan(int64_t N, int64_t V, int D, int dtype, bool packx, bool packw, b
   if (!train) {
     q.own = ce_own(q, CE_LOSS);
     q.sl = q.stream ? ce_splits((N + q.own - 1) / q.own, V, 320) : 0;
-    q.part = take((int64_t)(q.sl > q.tiles ? q.sl : q.tiles) * N * 8);
+    const bool tiles = !q.stream || N <= kCeFewRows;            // (few rows: which kernel depends on alignment too)
+    q.part = take((int64_t)(tiles && q.tiles > q.sl ? q.tiles : q.sl) * N * 8);
     q.zlab = take(N * 4);
     q.bsum = take((N + 63) / 64 * 8);
     q.done = take(4);

@@ -57,3 +57,15 @@ def test_tensors_in_the_place_of_numbers_are_refused():
                      lambda: ops.linear_ce_bwd(x, w, x, x, temperature=t), lambda: train_ops.dropout(x, t, 1), lambda: ops.dropout(x, t, 1)):
             with pytest.raises(_lib.HipLibraryError, match="a number expected"):
                 call()
+
+
+@pytest.mark.parametrize("N,V,D,dt", [(156672, 131072, 256, 1), (1 << 20, 1 << 20, 64, 1), (19584, 4096, 128, 0), (100000, 50000, 200, 2),
+                                      (33, 1 << 20, 64, 1), (1, 7, 3, 0), (32, 1 << 20, 128, 0)])
+def test_streamed_forward_keeps_one_statistic_per_split(N, V, D, dt):
+    """up to 256 feature columns (fp32: 128) the forward leaves one (maximum, rest) per row and split, and no more splits than fill eight
+    rounds of 256 workgroups of 512 rows; few rows: one per 256 classes"""
+    es, most = (4, 128) if dt == 0 else (2, 256)
+    assert D <= most
+    packs = (N + V) * (64 if D <= 64 else 128 if D <= 128 else 256) * es
+    stats = 8 * (2048 * 512 + N) if N > 32 else 8 * N * max(-(-V // 256), 256)
+    assert 0 < _lib.load().creste_linear_ce_workspace_bytes(N, V, D, dt, 0) <= packs + stats + 5 * N + 16384
