@@ -1426,8 +1426,8 @@ int ce_check(const void* x, int64_t ldx, const void* w, int64_t ldw, const void*
                  (long long)N, (long long)V, D);
   CRESTE_REQUIRE((ldx >= D || (ldx == 0 || N == 1)) && ldx >= 0 && (ldw >= D || V == 1 || ldw == 0) && ldw >= 0,
                  "linear_ce: row strides %lld %lld", (long long)ldx, (long long)ldw);
-  CRESTE_REQUIRE(tau > 0.f && tau < INFINITY && 1.f / tau < INFINITY,
-                 "linear_ce: temperature must be positive and finite, its inverse too");
+  CRESTE_REQUIRE(tau > 0.f && tau < INFINITY && 1.f / tau * kCeLog2e < INFINITY,
+                 "linear_ce: temperature must be positive and finite, its inverse (in units of log 2) too");
   return CRESTE_OK;
 }
 

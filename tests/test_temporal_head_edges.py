@@ -69,3 +69,13 @@ def test_streamed_forward_keeps_one_statistic_per_split(N, V, D, dt):
     packs = (N + V) * (64 if D <= 64 else 128 if D <= 128 else 256) * es
     stats = 8 * (2048 * 512 + N) if N > 32 else 8 * N * max(-(-V // 256), 256)
     assert 0 < _lib.load().creste_linear_ce_workspace_bytes(N, V, D, dt, 0) <= packs + stats + 5 * N + 16384
+
+
+def test_temperatures_whose_scale_overflows_are_refused():
+    """logits are taken in units of log2(e) / temperature: 1 / temperature may be finite where that is not"""
+    lib = _lib.load()
+    for tau in (1 / 3.0e38, 1 / 2.4e38):
+        rc = lib.creste_linear_ce_forward(P, 16, P, 16, P, 4, 8, 16, 0, -100, tau, 1, P, P, P, P, None, P, 1000, None)
+        _refused(rc, b"temperature")
+    rc = lib.creste_linear_ce_forward(P, 16, P, 16, P, 4, 8, 16, 0, -100, 1 / 2.3e38, 1, P, P, P, P, None, P, 1000, None)
+    _refused(rc, b"workspace")
