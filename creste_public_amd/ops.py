@@ -1479,17 +1479,27 @@ def _features(t, name: str, ndim=None, like=None) -> int:
     return _DTYPE_CODE[t.dtype]
 
 
+def _values(t: torch.Tensor) -> torch.Tensor:
+    """a tensor whose memory holds its values: a view that records a negation (the .imag of a conjugate) is written out"""
+    return t.detach().resolve_neg() if t.is_neg() else t
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """contiguous values, copied if they are not"""
+    return _values(t) if t.is_contiguous() else t.detach().contiguous()
+
+
 def _plain(t, dtype, shape, device, name: str) -> torch.Tensor:
     """a contiguous tensor of this type, shape and device -- or an error (values are copied if only the strides differ)"""
     if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device:
-        return t if t.is_contiguous() else t.detach().contiguous()
+        return _dense(t)
     got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
     raise HipLibraryError(f"{name}: expected {dtype} {tuple(shape)} on {device}, got {got}")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """last dimension contiguous, no negative or overlapping-write concerns (the tensor is only read); copied otherwise"""
-    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.detach().contiguous()
+    return _values(t) if t.shape[-1] == 1 or t.stride(-1) == 1 else t.detach().contiguous()
 
 
 def _int64(v, name: str) -> int:
@@ -1544,8 +1554,8 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Te
         if residual.shape != x.shape:
             raise HipLibraryError(f"dropout: residual {tuple(residual.shape)} beside x {tuple(x.shape)}")
         _features(residual, "dropout: residual", like=x)
-        r_ = residual if residual.is_contiguous() else residual.detach().contiguous()
-    return _dropout(x if x.is_contiguous() else x.detach().contiguous(), r_, p, _int64(seed, "dropout: seed"), _int64(offset, "dropout: offset"), state, code)
+        r_ = _dense(residual)
+    return _dropout(_dense(x), r_, p, _int64(seed, "dropout: seed"), _int64(offset, "dropout: offset"), state, code)
 
 
 def _dropout(x, residual, p, seed, offset, state, code):

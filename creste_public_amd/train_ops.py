@@ -678,8 +678,8 @@ class GatedRecurrenceFn(torch.autograd.Function):
         gate, x, lengths, starts = ctx.saved_tensors
         if gh is None:
             gh = torch.zeros((), dtype=gate.dtype, device=gate.device).expand(gate.shape)
-        gg, gx, gh0 = ops._recurrence_bwd(ops._rows(gate), ops._rows(x), lengths if lengths is None else lengths.contiguous(), starts,
-                                          ops._rows(gh), gh_last if gh_last is None else gh_last.contiguous(), ops._DTYPE_CODE[gate.dtype])
+        gg, gx, gh0 = ops._recurrence_bwd(ops._rows(gate), ops._rows(x), lengths if lengths is None else ops._dense(lengths), starts,
+                                          ops._rows(gh), gh_last if gh_last is None else ops._dense(gh_last), ops._DTYPE_CODE[gate.dtype])
         want = ctx.needs_input_grad
         return gg if want[0] else None, gx if want[1] else None, gh0 if want[2] else None, None
 

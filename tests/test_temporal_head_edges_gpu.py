@@ -215,3 +215,29 @@ def test_linear_ce_more_than_2_29_rows():
     within(gw, r["gw"], r["e_gw"], "dw")
     gx[at] = 0
     assert not gx[:1 << 20].any() and not gx[-(1 << 20):].any() and not gx[(1 << 29) - 4096:(1 << 29) + 1000].any()
+
+
+# ------------------------------------------------------------------------------------------------------------- layouts
+def test_views_that_record_a_negation():
+    """.imag of a conjugate (also as a cotangent) is a view that keeps the memory and records the sign"""
+    def neg(t):
+        v = torch._neg_view(-t)
+        assert v.is_neg() and v.is_contiguous() and torch.equal(v, t)
+        return v
+    x, res = torch.randn(2, 37, device="cuda").unbind(0)
+    gate, xs, gh = torch.randn(3, 2, 70, 6, device="cuda").unbind(0)
+    h0 = torch.randn(2, 6, device="cuda")
+    f, w, lab = torch.randn(40, 64, device="cuda"), torch.randn(9, 64, device="cuda"), torch.arange(40, device="cuda") % 9
+
+    def all_of(t):
+        y = ops.dropout(t(x), 0.3, 1, residual=t(res))
+        h, last, st = ops.gated_recurrence(t(gate), t(xs), t(h0), save=True)
+        back = ops.gated_recurrence_bwd(t(gate), t(xs), None, st, t(gh), t(last))
+        loss, nll, saved = ops.linear_ce(t(f), t(w), lab)
+        out = [y, h, last, *back, loss, nll, *ops.linear_ce_bwd(t(f), t(w), saved, t(loss))]
+        leaves = [u.clone().requires_grad_(True) for u in (x, gate, xs, h0, f, w)]
+        h, last = train_ops.gated_recurrence(*leaves[1:4])
+        loss, _ = loss_ops.linear_cross_entropy(leaves[4], leaves[5], lab)
+        return out + list(torch.autograd.grad((train_ops.dropout(leaves[0], 0.3, 1), h, last, loss), leaves, (t(x), t(gh), t(h0), t(loss.detach()))))
+    want, got = all_of(lambda t: t), all_of(neg)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
