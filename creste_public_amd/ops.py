@@ -1594,14 +1594,14 @@ def gated_recurrence(gate: torch.Tensor, x: torch.Tensor, h0: torch.Tensor | Non
     dev = g_.device
     h = torch.empty((B, T, Cc), dtype=g_.dtype, device=dev)
     lib = _lib.load()
+    starts = None
+    if save:
+        starts = torch.empty((-(-T // lib.creste_gated_recurrence_chunk_steps()), B, Cc), dtype=torch.float32, device=dev)
     if h.numel() == 0:
         last = h0.detach().clone() if h0 is not None else torch.zeros((B, Cc), dtype=torch.float32, device=dev)
-        return (h, last, torch.empty(0, dtype=torch.float32, device=dev)) if save else (h, last)
+        return (h, last, starts) if save else (h, last)
     with _on(dev) as on:
         last = torch.empty((B, Cc), dtype=torch.float32, device=dev)
-        starts = None
-        if save:
-            starts = torch.empty((-(-T // lib.creste_gated_recurrence_chunk_steps()), B, Cc), dtype=torch.float32, device=dev)
         nb = lib.creste_gated_recurrence_workspace_bytes(B, T, Cc)
         work = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
         _lib.check(lib.creste_gated_recurrence_forward(

@@ -241,3 +241,12 @@ def test_views_that_record_a_negation():
         return out + list(torch.autograd.grad((train_ops.dropout(leaves[0], 0.3, 1), h, last, loss), leaves, (t(x), t(gh), t(h0), t(loss.detach()))))
     want, got = all_of(lambda t: t), all_of(neg)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("shape", [(0, 5, 4), (2, 70, 0), (2, 0, 4)])
+def test_recurrence_halves_of_empty_batches(shape):
+    """what the forward saves of an empty batch is what the backward asks for"""
+    x = torch.zeros(shape, device="cuda")
+    h, last, starts = ops.gated_recurrence(x, x, save=True)
+    gg, gx, gh0 = ops.gated_recurrence_bwd(x, x, None, starts, h, last)
+    assert gg.shape == gx.shape == h.shape == x.shape and gh0.shape == last.shape == (shape[0], shape[2])
