@@ -181,7 +181,7 @@ class LinearCEFn(torch.autograd.Function):
     @once
     def backward(ctx, gl, _):
         x, weight, saved = ctx.saved_tensors
-        gx, gw = ops._linear_ce_bwd(ops._rows(x), ops._rows(weight), saved, ops._values(gl), *ctx.args, ctx.needs_input_grad[0],
+        gx, gw = ops._linear_ce_bwd(ops._rows_apart(x), ops._rows_apart(weight), saved, ops._values(gl), *ctx.args, ctx.needs_input_grad[0],
                                     ctx.needs_input_grad[1], ops._DTYPE_CODE[x.dtype])
         return gx, gw, None, None, None, None
 

@@ -1502,6 +1502,12 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return _values(t) if t.shape[-1] == 1 or t.stride(-1) == 1 else t.detach().contiguous()
 
 
+def _rows_apart(t: torch.Tensor) -> torch.Tensor:
+    """_rows of a matrix; rows that overlap (windows of one signal) are copied"""
+    t = _rows(t)
+    return t.detach().contiguous() if 0 < t.stride(0) < t.shape[1] and t.shape[0] > 1 else t
+
+
 def _int64(v, name: str) -> int:
     """a 64-bit pattern as the signed value ctypes takes"""
     v = int(v)
@@ -1659,7 +1665,7 @@ def _linear_ce_args(x, w, temperature, reduction):
         raise HipLibraryError(f"linear_cross_entropy: reduction {reduction!r} (mean or sum)")
     if not 0.0 < temperature < float("inf"):
         raise HipLibraryError(f"linear_cross_entropy: temperature {temperature}")
-    return code, _rows(x), _rows(w)
+    return code, _rows_apart(x), _rows_apart(w)
 
 
 def _ce_saved(N: int) -> int:

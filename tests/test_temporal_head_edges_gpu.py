@@ -250,3 +250,21 @@ def test_recurrence_halves_of_empty_batches(shape):
     h, last, starts = ops.gated_recurrence(x, x, save=True)
     gg, gx, gh0 = ops.gated_recurrence_bwd(x, x, None, starts, h, last)
     assert gg.shape == gx.shape == h.shape == x.shape and gh0.shape == last.shape == (shape[0], shape[2])
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+def test_linear_ce_overlapping_windows(dt):
+    """features that are windows of one signal, a row a few elements behind the one before"""
+    for D, step in ((64, 8), (37, 3), (320, 64)):
+        sig = torch.randn(3000, generator=gen(D)).to(dt).cuda()
+        x, w = sig.unfold(0, D, step)[:40], sig[:1500].unfold(0, D, 2 * step)[:9]
+        assert 0 < x.stride(0) < D
+        lab = torch.arange(40, device="cuda") % 9
+        want, got = [], []
+        for a, b, out in ((x.contiguous(), w.contiguous(), want), (x, w, got)):
+            loss, nll, saved = ops.linear_ce(a, b, lab)
+            out += [loss, nll, *ops.linear_ce_bwd(a, b, saved, loss)]
+            a, b = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+            loss, nll = loss_ops.linear_cross_entropy(a, b, lab)
+            out += [loss, nll, *torch.autograd.grad(loss, (a, b))]
+        assert all(torch.equal(u, v) for u, v in zip(want, got))
