@@ -15,29 +15,30 @@ from creste_public_amd.config import maxent_irl_cfg
 from tests.test_model_gpu import _irl_step, _rms, _with_eval_backbone, calibrate_bn
 
 pytestmark = pytest.mark.gpu
-# How far from the edge the two may still disagree: normalised inputs reach 10 in magnitude, and the roundings of a sum of 1000 products
-# (5 x 5 x 40) add up like a random walk, sqrt(1000) 2^-24 of that
-EDGE = 1000 ** 0.5 * 2.0 ** -24 * 10
 
 
 class _Relu(torch.nn.Module):
-    """ReLU with given sides"""
+    """ReLU with the sides of `y`, another forward's output.  far: how far the two differ where both are positive, at most; off_by: how far
+    from the edge an input lies whose sides differ; top: the largest output"""
 
-    def __init__(self, on):
+    def __init__(self, y):
         super().__init__()
-        self.on, self.off_by = on, 0.0
+        self.y = y.double()
 
     def forward(self, x):
-        self.off_by = float((x.detach().abs() * ((x > 0) != self.on)).max())
-        return torch.where(self.on, x, torch.zeros_like(x))
+        on, mine = self.y > 0, x.detach() > 0
+        self.far = float(((self.y - x.detach()).abs() * (on & mine)).max())
+        self.off_by = float((x.detach().abs() * (on != mine)).max())
+        self.top = float(x.detach().max())
+        return torch.where(on, x, torch.zeros_like(x))
 
 
 class _Pool(torch.nn.Module):
-    """2 x 2 maximum with a given element of each window"""
+    """2 x 2 maximum with a given element of each window; off_by: how much larger another one is"""
 
     def __init__(self, idx):
         super().__init__()
-        self.idx, self.off_by = idx, 0.0
+        self.idx = idx
 
     def forward(self, x):
         B, Cn, H, W = x.shape
@@ -54,7 +55,7 @@ def _with_sides_of(net, engine):
         sides = []
         for op in getattr(engine, name).ops:
             if isinstance(op, train_ops.ReLUT) or (isinstance(op, train_ops.BNT) and op.relu):
-                sides.append(_Relu(op.y.nchw() > 0))
+                sides.append(_Relu(op.y.nchw()))
             elif isinstance(op, train_ops.PoolT):
                 sides.append(_Pool(op.idx.permute(0, 3, 1, 2).long()))
         new += sides
@@ -120,7 +121,14 @@ def test_reward_gradients_with_the_sides_of_the_forward(step, prec):
     ref_net = copy.deepcopy(step["oracle"].traversability_head.r).cuda().double()
     sided = _with_sides_of(ref_net, net._train_engine)
     ref = _gradients(ref_net, step["lm"], step["out"], "cuda", torch.float64, *step["data"])
-    assert sided and max(s.off_by for s in sided) < EDGE
-    assert set(got) == set(ref)
+    far = 0.0
+    for s in sided:                            # sides differ only as close to the edge as the forwards do elsewhere in the layer
+        if isinstance(s, _Relu):
+            far = s.far
+            assert far <= 1e-4 * s.top         # (fp32 sums of up to 1000 products; some channels scaled up by their BatchNorm)
+            assert s.off_by <= far
+        else:
+            assert s.off_by <= 2 * far
+    assert far and set(got) == set(ref)
     for n in ref:
         assert _rms(got[n] - ref[n]) <= 2e-3 * max(_rms(ref[n]), 1e-8) + 1e-9, n
