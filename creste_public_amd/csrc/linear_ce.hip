@@ -52,7 +52,6 @@ struct CeArgs {
   int k1, ksplit;                   // contraction length; ksplit > 0: split s works [s * ksplit, + ksplit)
   // LOSS / GRAD
   const int64_t* labels;
-  int64_t ignore;
   int class0;                       // GRAD, DX: first class of the piece
   int classes;                      // all classes
   float inv_tau;
@@ -278,7 +277,7 @@ struct CeShape {
 };
 
 // DT: 16-bit operand type (fp16 for two-piece fp32), P: pieces.  Bound: matrix rate, and for DX / DW reading G.  4096 x 131072 x 1024 bf16:
-// LOSS 1050 us (1050 TF/s), and for each of eight pieces of 16384 classes GRAD 160, DX 155-175, DW 140-150 us (780-980 TF/s)
+// LOSS 1050-1140 us (1000 TF/s), and for each of eight pieces of 16384 classes GRAD 160, DX 155-175, DW 140-150 us (780-980 TF/s)
 template <int MODE, int DT, int P, typename S, bool NATIVE>
 __device__ __forceinline__ void ce_gemm_body(const CeArgs& p) {
   constexpr bool AKM = MODE == CE_DX || MODE == CE_DW, BKM = MODE == CE_DW;
@@ -501,9 +500,9 @@ __global__ __launch_bounds__(S::NW * 64, 2) void ce_gemm_kernel(CeArgs p) {
 // streamed tile take them in the order in which the accumulator holds them.  One tile in LDS serves both products (rows for z,
 // transposed for the second), its 16-byte chunks swizzled by the row: a bijection over 16 rows for the row reads, different 64-byte
 // windows for the 4 rows of a transposing read.
-// Bound: matrix rate, then the exponentials beside it.  8192 x 65536 x 256 bf16: loss 260 us (1060 TF/s), both gradients 1060-1155 us
-// (8NVD, 950-1040 TF/s; a large library product: 1216).  19584 x 4096 x 128 fp32: 80 and 253 us (770 and 970 TF/s of fp16 products).
-// Against the tiled product with G in memory: 1845 -> 1200 us and 596 -> 345 us for the whole step.
+// Bound: matrix rate, then the exponentials beside it.  8192 x 65536 x 256 bf16: loss 270-290 us (980 TF/s), both gradients 1060-1170 us
+// (8NVD, 940-1040 TF/s; a large library product: 1216).  19584 x 4096 x 128 fp32: 75 and 257 us (820 and 960 TF/s of fp16 products).
+// Against the tiled product with G in memory: 1845 -> 1236 us and 596 -> 341 us for the whole step.
 template <int DP, int OTS, int P>
 struct CeStream {
   static constexpr int ROWB = DP * 2, CPR = ROWB / 16, PIECE = OTS * ROWB, INFO = P * PIECE, BYTES = INFO + 1024, INSTR = PIECE / 1024;
@@ -1482,7 +1481,7 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
   a.b = X.p; a.ldb = X.ld; a.pb = X.piece; a.rb = N;
   a.m = (int)V; a.n = (int)N;
   a.k1 = q.Dp;
-  a.labels = labels; a.ignore = ignore_index; a.classes = (int)V;
+  a.labels = labels; a.classes = (int)V;
   a.inv_tau = 1.f / temperature;
   a.amax = q.P == 2 ? (const float*)(copies + q.amax) : nullptr;
   a.part = (float2*)(wk + q.part); a.zlab = (float*)(wk + q.zlab); a.done = (unsigned*)(wk + q.done);

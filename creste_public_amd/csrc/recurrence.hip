@@ -48,8 +48,8 @@ __device__ __forceinline__ void rec_put(uint64_t* p, uint64_t v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// f = sigmoid(g), u = 1 - f, both to a few 2^-24 relative (hardware exponential and reciprocal: a full division would cost as much
-// as the rest of a step)
+// f = sigmoid(g), u = 1 - f; the exponential's rounded argument leaves the smaller of the two (2 + 1.5 |g|) 2^-24 off, relatively, the
+// larger a few 2^-24 (hardware exponential and reciprocal: a full division would cost as much as the rest of a step)
 __device__ __forceinline__ void rec_gate(float g, float& f, float& u) {
   const float e = __builtin_amdgcn_exp2f(-1.44269504088896341f * fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
   f = g >= 0.f ? r : s;

@@ -166,7 +166,7 @@ class SmoothL1Fn(torch.autograd.Function):
 
 class LinearCEFn(torch.autograd.Function):
     """softmax cross entropy of x w^T / temperature against class labels, without the logits (csrc/linear_ce.hip); the backward
-    forms them again in pieces of the classes.  -> (loss, nll [N])"""
+    forms them again.  -> (loss, nll [N])"""
 
     @staticmethod
     def forward(ctx, x, weight, labels, ignore_index, temperature, reduction):
@@ -194,7 +194,9 @@ def linear_cross_entropy(x, weight, labels, ignore_index: int = -100, temperatur
     -> (loss, nll): loss = mean of nll over the rows that count (0 when none does) or their sum, a differentiable fp32 scalar;
     nll [...] fp32, not differentiable.  The features of ignored rows may be anything (infinite, NaN: padding); their gradient is 0.  A label
     that names neither a class nor ignore_index makes the loss and its gradients NaN.  fp32 features are multiplied with 22 significand bits
-    of each row's largest magnitude at least (rows more than 2^17 apart, or not finite: in fp32, at a third of the speed).
+    of each row's largest magnitude at least (rows more than 2^17 apart, or not finite: in fp32, at a third of the speed), 16-bit ones as
+    they are.  For the gradients the softmax's is rounded to what the matrix cores take: bf16 2^-8, fp16 2^-11 (2^-39 of a certain row's at
+    least), fp32 2^-22 (2^-39); all sums are fp32, and each output is rounded once more, to the features' type.
     Differentiable once; not recorded inside a stream capture (train_ops.recorded)."""
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise HipLibraryError("linear_cross_entropy: x [...,D] expected")
