@@ -5,6 +5,9 @@
 // one tiled matrix product (ce_gemm_kernel) serves all four products:
 //   LOSS   z = w x^T; its epilogue leaves (max, sum exp) of the tile's 256 classes per row, and the label's logit
 //   GRAD   z again, its epilogue turns the tile into G (16 bit) for a PIECE of the classes; a piece is bounded in bytes
+// Every kernel forms a logit in the same order of additions, so the largest of a row comes out of the gradients' products with the bits
+// it had in the loss and G is taken against it, not against a rounded log-sum-exp: at logits of 10^6 that would be off by tens of percent.
+// (Up to 32 rows fp32 features therefore stay fp32 in both directions, as the few-rows kernel takes them.)
 //   DX     dx += w^T G over the piece, DW  dw = x^T G over the rows
 // Layout.  Every product has the operand whose index lands in the accumulator REGISTERS first (classes for LOSS / GRAD, feature
 // columns for DX / DW) and the other one in the lanes: a lane then owns one row of the softmax (reductions over classes are
@@ -14,7 +17,7 @@
 // stored transposed.  Both layouts are swizzled in 16-byte chunks (on the global address of the DMA, whose LDS side is fixed).
 // A row's softmax is kept as (maximum, rest): sum of exponentials = exp(maximum) (1 + rest).  The maximum's own term never meets the
 // others in one sum (CeTop), so that a confident row (rest << 1) keeps its loss to a few 2^-24 instead of 2^-24 / rest, and no loss is
-// negative; for fp32 features the label's entry of G is expm1(-nll), so its gradient does too.  Against plain sums that is 1.5 % of a
+// negative; the label's entry of G is expm1(-nll), so its gradient does too.  Against plain sums that is 1.5 % of a
 // training step of 8192 x 65536 x 256 bf16 (1217 -> 1236 us), 0.5 % at 4096 x 131072 x 1024.
 // Precision.  16-bit features enter as they are, fp32 features as two fp16 pieces under one power-of-two scale per tensor: an element
 // is off by 2^-22 of itself or 2^-39 of the tensor's largest, whichever is more, and the three products hi*hi + hi*lo + lo*hi leave out
@@ -59,10 +62,9 @@ struct CeArgs {
   float2* part;                     // LOSS: [class tile][n] (maximum, rest)
   float* zlab;                      // LOSS: [n] label logit, as maxima in the units of the products
   unsigned* done;                   // LOSS: the joining kernel's counter, cleared here
-  // GRAD, DX, DW, per row (padded to 64).  16-bit features: row_l2 = log-sum-exp (log2 units) minus log2 of G's scale, infinity where a
-  // row does not count.  fp32: row_l2 = the maximum (log2 units, rounded), row_rest = what is left of the log-sum-exp, with the maximum's
-  // rounding, minus log2 of G's scale, or infinity, and row_g = the label's entry of G
-  const float *row_l2, *row_rest, *row_g;
+  // GRAD, DX, DW, per row (padded to 64): the largest product z, log2 of the sum relative to its term minus log2 of G's scale -- infinity
+  // where a row does not count --, and the label's entry of G
+  const float *row_max, *row_rest, *row_g;
   const int* row_lab;               // label, -1 where none applies
   char* g;                          // GRAD: [n64][ldg] elements, pieces pg bytes apart
   int64_t ldg, pg;
@@ -93,6 +95,13 @@ template <int P>
 __device__ __forceinline__ bool ce_native(const CeArgs& p) {
   if constexpr (P == 2) return p.amax[2] != 0.f;
   return false;
+}
+
+// exp2 argument of a softmax gradient: the logit against its row's largest, exactly (the kernels form both in the same order), then the rest.
+// unit: power of two of the operands' products, kappa = log2(e) / tau
+template <int P>
+__device__ __forceinline__ float ce_exponent(float z, float unit, float mx, float kappa, float rest) {
+  return fmaf(P == 2 ? fmaf(z, unit, -mx) : z - mx, kappa, -rest);
 }
 
 // dloss / (tau * count) and the powers of two of the stored operands
@@ -381,7 +390,7 @@ __device__ __forceinline__ void ce_gemm_body(const CeArgs& p) {
   __syncthreads();                                      // the stages are free
 
   if constexpr (MODE == CE_LOSS || MODE == CE_GRAD) {
-    const float c2 = ce_operand_inv(p.amax, 0) * ce_operand_inv(p.amax, 1) * p.inv_tau * kCeLog2e;
+    const float unit = ce_operand_inv(p.amax, 0) * ce_operand_inv(p.amax, 1), c2 = unit * p.inv_tau * kCeLog2e, kappa = p.inv_tau * kCeLog2e;
     const int mw = m0 + wm * WTM;                       // first class of this wave, within the piece
     if constexpr (MODE == CE_LOSS) {
       float2* sh = reinterpret_cast<float2*>(smem);     // [wm][BN rows]
@@ -433,8 +442,8 @@ __device__ __forceinline__ void ce_gemm_body(const CeArgs& p) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int row = n0 + wn * WTN + j * 32 + li;
-        const float l2 = row < p.n64 ? p.row_l2[row] : INFINITY;
-        const float rest = P == 2 && row < p.n64 ? p.row_rest[row] : 0.f, gl = P == 2 && row < p.n64 ? p.row_g[row] : 0.f;
+        const float mx = row < p.n64 ? p.row_max[row] : 0.f, rest = row < p.n64 ? p.row_rest[row] : INFINITY,
+                    gl = row < p.n64 ? p.row_g[row] : 0.f;
         const int yr = (row < p.n64 ? p.row_lab[row] : -1) - p.class0 - mw;
         const bool any = __any(yr >= 0 && yr < WTM);
 #pragma unroll
@@ -446,10 +455,8 @@ __device__ __forceinline__ void ce_gemm_body(const CeArgs& p) {
             cef4 whole;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float z = acc[i][j][4 * q + e];
-              float v = fmaf(z, c2, -l2);
-              v = __builtin_amdgcn_exp2f(P == 2 ? v - rest : v);
-              if (any) v = cl + e == yr ? (P == 2 ? gl : v - p.gscale) : v;
+              float v = __builtin_amdgcn_exp2f(ce_exponent<P>(acc[i][j][4 * q + e], unit, mx, kappa, rest));
+              if (any) v = cl + e == yr ? gl : v;
               if (mw + WTM > p.m) v = mw + cl + e < p.m ? v : 0.f;
               whole[e] = v;
               const short h = ce_cvt<DT>(v);
@@ -558,8 +565,8 @@ struct CeStream {
   // DW: what a row brings along, behind the features (every wave issues as many loads: some twice)
   static __device__ __forceinline__ void dma_info(char* lds, const CeArgs& p, int64_t o0, int wave, int lane) {
     static_assert(OTS == 64, "one 4-byte load per lane");
-    const int which = P == 2 ? wave & 3 : wave & 1;
-    const char* src = which == 3 ? (const char*)p.row_g : which == 2 ? (const char*)p.row_rest : which ? (const char*)p.row_lab : (const char*)p.row_l2;
+    const int which = wave & 3;
+    const char* src = which == 3 ? (const char*)p.row_g : which == 2 ? (const char*)p.row_rest : which ? (const char*)p.row_lab : (const char*)p.row_max;
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + (o0 + lane) * 4),
                                      (__attribute__((address_space(3))) void*)(lds + INFO + which * 256), 4, 0, 0);
   }
@@ -611,10 +618,10 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) x[q][j][kk] = *reinterpret_cast<const ces8*>(p.b + q * p.pb + row * p.ldb + kk * 32 + lh * 16);
   }
-  const float c2 = ce_operand_inv(p.amax, 0) * ce_operand_inv(p.amax, 1) * p.inv_tau * kCeLog2e;
+  const float unit = ce_operand_inv(p.amax, 0) * ce_operand_inv(p.amax, 1), c2 = unit * p.inv_tau * kCeLog2e, kappa = p.inv_tau * kCeLog2e;
   // LOSS: the maximum mx so far, the sum of exp2((z - near) c2) as two tops; near follows the maximum in steps, when a logit passes `lim`
   // (8 above: such an exponent is off by 2^-22)
-  float l2[NT], rest[NT], gl[NT], mx[NT], zl[NT], near[NT], lim[NT];
+  float rest[NT], gl[NT], mx[NT], zl[NT], near[NT], lim[NT];
   CeTop top[NT][2];
   int lab[NT];                               // LOSS / DX: the row's label; DW: the own class
 #pragma unroll
@@ -624,18 +631,16 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
     lim[j] = -INFINITY;
     near[j] = -3.0e38f;
     top[j][0] = top[j][1] = CeTop{0.f, 0.f};
-    zl[j] = l2[j] = rest[j] = gl[j] = 0.f;
+    zl[j] = rest[j] = gl[j] = 0.f;
     lab[j] = o;
     if constexpr (MODE == CE_LOSS) {
       const int64_t y = o < p.n ? p.labels[o] : -1;
       lab[j] = y >= 0 && y < p.classes ? (int)y : -1;
     }
     if constexpr (MODE == CE_DX) {
-      l2[j] = o < p.n ? p.row_l2[o] : INFINITY;
-      if constexpr (P == 2) {
-        rest[j] = o < p.n ? p.row_rest[o] : 0.f;
-        gl[j] = o < p.n ? p.row_g[o] : 0.f;
-      }
+      mx[j] = o < p.n ? p.row_max[o] : 0.f;
+      rest[j] = o < p.n ? p.row_rest[o] : INFINITY;
+      gl[j] = o < p.n ? p.row_g[o] : 0.f;
       lab[j] = o < p.n ? p.row_lab[o] : -1;
     }
   }
@@ -692,9 +697,9 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
         for (int q = 0; q < P; ++q) a[q] = L::row(smem, stage + q * L::PIECE + rbase, kk);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          if constexpr (P == 2) {
-            z[j] = ce_mfma<DT>(a[1], x[0][j][kk], z[j]);
-            z[j] = ce_mfma<DT>(a[0], x[1][j][kk], z[j]);
+          if constexpr (P == 2) {                       // w's low piece first on either side: the same sums
+            z[j] = MODE == CE_DW ? ce_mfma<DT>(a[0], x[1][j][kk], z[j]) : ce_mfma<DT>(a[1], x[0][j][kk], z[j]);
+            z[j] = MODE == CE_DW ? ce_mfma<DT>(a[1], x[0][j][kk], z[j]) : ce_mfma<DT>(a[0], x[1][j][kk], z[j]);
           }
           z[j] = ce_mfma<DT>(a[0], x[0][j][kk], z[j]);
         }
@@ -706,7 +711,7 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
       ces8 g[P][NT][2];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        if (edge && MODE != CE_DW)                      // (DW: such rows have l2 = infinity)
+        if (edge && MODE != CE_DW)                      // (DW: such rows have rest = infinity)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (o0 + (r & 3) + 8 * (r >> 2) + 4 * lh >= p.m) z[j][r] = -INFINITY;
@@ -733,41 +738,49 @@ __device__ __forceinline__ void ce_stream_body(const CeArgs& p, int block, int b
           mx[j] = ce_max(mx[j], m);
         } else {
           float v[16];
+          // DW: what the others, rows here (padded to whole stages), brought along: 4 of word `which`
+          auto info = [&](int which, int q) __attribute__((always_inline)) {
+            const int at = sub * 32 + 8 * q + 4 * lh;
+            cei4 w4;
+            if constexpr (NATIVE) {
+              const int* src = which == 3 ? (const int*)p.row_g : which == 2 ? (const int*)p.row_rest : which ? p.row_lab : (const int*)p.row_max;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w4[e] = src[kb + c * kCeStage + at + e];
+            } else {
+              w4 = *reinterpret_cast<const cei4*>(st + L::INFO + which * 256 + at * 4);
+            }
+            return w4;
+          };
+          bool hit = false;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            cef4 rl, rr, rg;
-            cei4 rb;
-            if constexpr (MODE == CE_DW && NATIVE) {    // of the others, which are rows here (padded to whole stages)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int64_t o = o0 + 8 * q + 4 * lh + e;
-                rl[e] = p.row_l2[o];
-                rb[e] = p.row_lab[o];
-                rr[e] = p.row_rest[o];
-                rg[e] = p.row_g[o];
-              }
-            } else if constexpr (MODE == CE_DW) {
-              rl = *reinterpret_cast<const cef4*>(st + L::INFO + (sub * 32 + 8 * q + 4 * lh) * 4);
-              rb = *reinterpret_cast<const cei4*>(st + L::INFO + 256 + (sub * 32 + 8 * q + 4 * lh) * 4);
-              if constexpr (P == 2) {
-                rr = *reinterpret_cast<const cef4*>(st + L::INFO + 512 + (sub * 32 + 8 * q + 4 * lh) * 4);
-                rg = *reinterpret_cast<const cef4*>(st + L::INFO + 768 + (sub * 32 + 8 * q + 4 * lh) * 4);
-              }
+            cef4 rm, rr;
+            if constexpr (MODE == CE_DW) {
+              rm = __builtin_bit_cast(cef4, info(0, q));
+              rr = __builtin_bit_cast(cef4, info(2, q));
+              const cei4 rb = info(1, q);
+              hit |= rb[0] == lab[j] || rb[1] == lab[j] || rb[2] == lab[j] || rb[3] == lab[j];
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = 4 * q + e;
-              const float a = MODE == CE_DW ? rl[e] : l2[j];
-              const float u = fmaf(z[j][r], c2, -a);
-              v[r] = __builtin_amdgcn_exp2f(P == 2 ? u - (MODE == CE_DW ? rr[e] : rest[j]) : u);
-              if constexpr (MODE == CE_DW) v[r] = rb[e] == lab[j] ? (P == 2 ? rg[e] : v[r] - p.gscale) : v[r];
-            }
+            for (int e = 0; e < 4; ++e)
+              v[4 * q + e] = __builtin_amdgcn_exp2f(
+                  ce_exponent<P>(z[j][4 * q + e], unit, MODE == CE_DW ? rm[e] : mx[j], kappa, MODE == CE_DW ? rr[e] : rest[j]));
+          }
+          if constexpr (MODE == CE_DW) {
+            if (__any(hit))
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const cei4 rb = info(1, q);
+                const cef4 rg = __builtin_bit_cast(cef4, info(3, q));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * q + e] = rb[e] == lab[j] ? rg[e] : v[4 * q + e];
+              }
           }
           if constexpr (MODE == CE_DX) {
             const int rel = lab[j] - o0;
             if (__any(rel >= 0 && rel < 32))
 #pragma unroll
-              for (int r = 0; r < 16; ++r) v[r] = (r & 3) + 8 * (r >> 2) + 4 * lh == rel ? (P == 2 ? gl[j] : v[r] - p.gscale) : v[r];
+              for (int r = 0; r < 16; ++r) v[r] = (r & 3) + 8 * (r >> 2) + 4 * lh == rel ? gl[j] : v[r];
           }
           if constexpr (NATIVE) {                       // register r holds the others 8 (r / 4) + r % 4 of either half
 #pragma unroll
@@ -955,7 +968,7 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeArgs p, int D) {
 // ---------------------------------------------------------------------------------------------------- small kernels
 // both operands at once: blocks below `split` take the first, the others the second.  Rows of x that do not count are taken as zeros,
 // whatever they hold (0 * NaN would reach dw, a large value fp32's scale): named by their labels, behind the forward by the infinite
-// log-sum-exp it left
+// rest it left
 struct CeSide {
   const void* x;
   int64_t rows, ld;
@@ -1027,7 +1040,7 @@ __device__ __forceinline__ bool ce_even(CeMax m) {
 // 2062 / 6610
 template <typename T>
 __global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int cols, int cp, int split, const unsigned* __restrict__ bmax,
-                                                      const uint8_t* __restrict__ blow, int na0, int na1, float inv_tau,
+                                                      const uint8_t* __restrict__ blow, int na0, int na1, float inv_tau, bool force,
                                                       float* __restrict__ amax) {
   const bool second = (int)blockIdx.x >= split;
   const CeSide s = second ? v : u;
@@ -1046,7 +1059,7 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int co
       sc[i] = f16_operand_scale(__uint_as_float(m[i].bits), &inv[i]);
     }
     const float unit = inv[0] * inv[1], c2 = unit * inv_tau * kCeLog2e;
-    native = !ce_even(m[0]) || !ce_even(m[1]) || !(unit >= 0x1p-126f && c2 >= 0x1p-125f && c2 < INFINITY);
+    native = force || !ce_even(m[0]) || !ce_even(m[1]) || !(unit >= 0x1p-126f && unit < INFINITY && c2 >= 0x1p-125f && c2 < INFINITY);
     scale = sc[second];
     if (blk == 0 && threadIdx.x == 0) {
       amax[second] = native ? 0.f : __uint_as_float(m[second].bits);
@@ -1085,12 +1098,12 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int co
 }
 
 // per row: join the class tiles' (maximum, rest); 64 rows x 16 slices of the tiles per block and turn (blocks of rows).  Leaves nll, what
-// the gradient kernels ask of a row (padded to whole tiles: rows that do not count get an infinite log-sum-exp, hence G = 0, a label that
+// the gradient kernels ask of a row (padded to whole tiles: rows that do not count get an infinite rest, hence G = 0, a label that
 // names no class a NaN), and, from the last block to finish, the loss: sums of the blocks' sums in their order, so the result does not
-// depend on which that was.  Maxima and label logits come in the units of the products.  two: fp32 features, the log-sum-exp in two parts
+// depend on which that was.  Maxima and label logits come in the units of the products
 __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ part, int tiles, int n, int blocks,
                                                        const float* __restrict__ zlab, const int64_t* __restrict__ labels, int64_t ignore,
-                                                       int classes, int two, const float* __restrict__ amax, float inv_tau,
+                                                       int classes, const float* __restrict__ amax, float inv_tau,
                                                        float log2_scale, float* __restrict__ nll, float* __restrict__ rows,
                                                        uint64_t* __restrict__ bsum, unsigned* __restrict__ done, int mean,
                                                        float* __restrict__ loss, float* __restrict__ stat) {
@@ -1098,7 +1111,7 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
   __shared__ bool last;
   const int li = threadIdx.x & 63, sl = threadIdx.x >> 6;
   const int64_t n64 = blocks * 64ll;
-  const float c2 = ce_operand_inv(amax, 0) * ce_operand_inv(amax, 1) * inv_tau * kCeLog2e;      // (as the loss kernels')
+  const float unit = ce_operand_inv(amax, 0) * ce_operand_inv(amax, 1), c2 = unit * inv_tau * kCeLog2e;      // (as the loss kernels')
   for (int blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
     const int64_t row = blk * 64ll + li;
     float2 st = make_float2(-3.0e38f, -1.f);
@@ -1119,11 +1132,10 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
       c = 1.f;
     }
     if (row < n) nll[row] = l;
-    const float m2 = st.x * c2, rest = (lr * kCeLog2e + fmaf(st.x, c2, -m2)) - log2_scale;
-    rows[row] = !on ? (two ? 0.f : INFINITY) : !ok ? __builtin_nanf("") : two ? m2 : m2 + rest;
+    rows[row] = !on ? 0.f : ok ? st.x * unit : __builtin_nanf("");
     reinterpret_cast<int*>(rows)[n64 + row] = on && ok ? (int)y : -1;
-    rows[2 * n64 + row] = !two ? 0.f : on ? rest : INFINITY;
-    rows[3 * n64 + row] = two && on ? expm1f(-l) * exp2f(log2_scale) : 0.f;
+    rows[2 * n64 + row] = on ? lr * kCeLog2e - log2_scale : INFINITY;
+    rows[3 * n64 + row] = on ? expm1f(-l) * exp2f(log2_scale) : 0.f;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       l += __shfl_xor(l, o, 64);
@@ -1409,9 +1421,9 @@ int ce_operands(const CePlan& q, const void* x, int64_t ldx, const void* w, int6
   if (q.P == 2) {                                  // (both are copied)
     const int ax = blocks(N, kCeMaxima), aw = blocks(V, kCeMaxima);
     ce_amax_kernel<<<ax + aw, 256, 0, s>>>(sx, sw, D, ax, bmax, blow);
-    ce_pack_kernel<float><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, bmax, blow, ax, aw, inv_tau, amax);
+    ce_pack_kernel<float><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, bmax, blow, ax, aw, inv_tau, N <= kCeFewRows, amax);
   } else if (px + pw) {
-    ce_pack_kernel<short><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, nullptr, nullptr, 0, 0, 0.f, nullptr);
+    ce_pack_kernel<short><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, nullptr, nullptr, 0, 0, 0.f, false, nullptr);
   }
   CRESTE_CHECK_LAUNCH("linear_ce pack");
   return CRESTE_OK;
@@ -1496,7 +1508,7 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
   }
   const int nb = (int)((N + 63) / 64);
   ce_join_kernel<<<nb < kCeJoinBlocks ? nb : kCeJoinBlocks, 1024, 0, s>>>(
-      a.part, q.stream && !few ? q.sl : q.tiles, (int)N, nb, a.zlab, labels, ignore_index, (int)V, q.P == 2, few ? nullptr : a.amax, a.inv_tau,
+      a.part, q.stream && !few ? q.sl : q.tiles, (int)N, nb, a.zlab, labels, ignore_index, (int)V, few ? nullptr : a.amax, a.inv_tau,
       ce_gscale_log2(q), nll, rows, (uint64_t*)(wk + q.bsum), a.done, mean, loss, stat);
   CRESTE_CHECK_LAUNCH("linear_ce join");
   return CRESTE_OK;
@@ -1517,7 +1529,7 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
   CeOperand X, W;
   const bool kept = packs && !ce_takes_few(x, ldx, w, ldw, N, D, dtype);
   char* const copies = kept ? (char*)packs : wk;
-  const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, 1.f / temperature, kept, nullptr, 0, q.P == 2 ? rows + 2 * q.n64 : rows, copies, &X, &W, s);
+  const int rc = ce_operands(q, x, ldx, w, ldw, N, V, D, 1.f / temperature, kept, nullptr, 0, rows + 2 * q.n64, copies, &X, &W, s);
   if (rc) return rc;
   CeArgs c{};                                       // what every product shares
   c.classes = (int)V;
@@ -1525,7 +1537,7 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
   c.amax = q.P == 2 ? (const float*)(copies + q.amax) : nullptr;
   c.stat = stat; c.gl = g_loss; c.mean = mean;
   c.gscale = exp2f(ce_gscale_log2(q));
-  c.row_l2 = rows; c.row_lab = (const int*)(rows + q.n64); c.row_rest = rows + 2 * q.n64; c.row_g = rows + 3 * q.n64;
+  c.row_max = rows; c.row_lab = (const int*)(rows + q.n64); c.row_rest = rows + 2 * q.n64; c.row_g = rows + 3 * q.n64;
   c.n64 = (int)q.n64;
   c.out_dt = dtype;
   c.ldo = c.m_out = D;

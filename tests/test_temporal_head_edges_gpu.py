@@ -195,6 +195,45 @@ def test_linear_ce_16_bit_confident_rows(N, V, D, dt):
     within(nll, want, bound, "nll")
 
 
+@pytest.mark.parametrize("dt", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("tau", [0.02, 1e-5, 1e-15])
+@pytest.mark.parametrize("N,V,D", [(24, 700, 64), (300, 257, 64), (300, 3000, 128), (300, 3000, 256), (300, 1025, 320)])
+def test_linear_ce_gradients_of_sure_rows(N, V, D, dt, tau):
+    """logits of 10 to 500 at tau 0.02, to 10^16 at the smallest: the softmax gradient of a row is the other classes' probabilities and, at
+    the label, minus their sum; each is as sure, relatively, as the margins e (and its rounding for the matrix cores: u_g, not below
+    2^-39 of 1 for the fp16 pieces), so that a row that is sure beyond doubt gets no gradient"""
+    w = _unit(V, D, V).to(dt).cuda()
+    labels = torch.randint(0, V, (N,), generator=gen(N)).cuda()
+    x = (w[labels].float() * torch.logspace(-0.7, 1.0, N, device="cuda")[:, None]).to(dt)
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss, nll = loss_ops.linear_cross_entropy(a, b, labels, temperature=tau, reduction="sum")
+    gx, gw = torch.autograd.grad(loss, (a, b))
+    xd, wd, lab = x.double().cpu(), w.double().cpu(), labels.cpu()
+    z = xd @ wd.t() / tau
+    prod = 2.0 ** -20 if dt == F32 else 0.0
+    e = (prod + (D + 8) * O.U32) * (xd.abs() @ wd.abs().t()) / tau
+    d, e = z - z.gather(1, lab[:, None]), e + e.gather(1, lab[:, None])
+    hot = torch.zeros_like(z).scatter_(1, lab[:, None], 1.0)
+    e = e + 4 * O.U32 * (z.abs() + z.abs().gather(1, lab[:, None]))
+
+    def others(t):                                                    # probabilities of the other classes for margins t
+        q = torch.exp(t.clamp(max=700)) * (1 - hot)
+        return q / (1 + q.sum(1, keepdim=True))
+    q = others(d)
+    top = (torch.exp((d + e).clamp(max=700)) * (1 - hot)).clamp(max=1.0)          # (a probability is at most its ratio to the label's, and 1)
+    e_q = (top - q).clamp(min=0) + (q - (torch.exp(d - e) * (1 - hot)) / (1 + (torch.exp((d + e).clamp(max=700)) * (1 - hot)).sum(1, keepdim=True))).clamp(min=0)
+    G, mag = q - hot * q.sum(1, keepdim=True), q + hot * q.sum(1, keepdim=True)
+    u_g = {BF16: 2.0 ** -8, F16: 2.0 ** -11, F32: 2.0 ** -20}[dt]
+    floor = 2.0 ** -126 if dt == BF16 else 2.0 ** -39                  # (bf16: a probability below fp32's normal range may be taken as 0)
+    e_G = e_q + hot * e_q.sum(1, keepdim=True).clamp(max=1.0) + (u_g + (max(N, V) + 64) * O.U32) * mag + floor
+    half = O.half_step(dt)
+    tiny = 2.0 ** -24 if dt == F16 else 0.0
+    for got, want, bound, name in ((gx, G @ wd / tau, e_G @ wd.abs() / tau, "dx"), (gw, G.t() @ xd / tau, e_G.t() @ xd.abs() / tau, "dw")):
+        if dt == F16 and float(want.abs().max() + bound.max()) > 6e4:
+            continue                                                  # (beyond the type)
+        within(got, want, 1.01 * bound + half * want.abs() + tiny, name)
+
+
 # ------------------------------------------------------------------------------------------------------------ very many rows
 def test_linear_ce_more_than_2_29_rows():
     """four words a row for the backward pass 2^31 words; rows at both ends and around 2^29, all others ignored"""
