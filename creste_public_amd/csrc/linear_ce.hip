@@ -329,17 +329,33 @@ __device__ __forceinline__ void ce_gemm_body(const CeArgs& p) {
       }
       return v;
     };
+    // (columns of the output that are not there, most of them where there are few rows, stay 0)
+    const int nw = n0 + wn * WTN, cols = nw >= p.n ? 0 : p.n - nw;
     const char* const first = p.a + (MODE == CE_GRAD || MODE == CE_DX ? p.class0 * p.lda : 0);      // (the piece's: rows are twice as long)
-    for (int k = kb; k < ke; k += 8) {
-      cef4 a[MT], b[NT];
+    constexpr int AHEAD = 2;                            // steps in flight (a step's loads take longer than its products)
+    cef4 a[AHEAD][MT], b[AHEAD][NT];
+    auto fetch = [&](int k, int at) __attribute__((always_inline)) {
+      k = k < ke ? k : ke - 8;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) a[i] = load(first, p.lda, p.ra, p.ca / 2, AKM, m0 + wm * WTM + i * 32 + li, k);
+      for (int i = 0; i < MT; ++i) a[at][i] = load(first, p.lda, p.ra, p.ca / 2, AKM, m0 + wm * WTM + i * 32 + li, k);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) b[j] = load(p.b, p.ldb, p.rb, p.cb / 2, BKM, n0 + wn * WTN + j * 32 + li, k);
+      for (int j = 0; j < NT; ++j)
+        if (cols > j * 32) b[at][j] = load(p.b, p.ldb, p.rb, p.cb / 2, BKM, nw + j * 32 + li, k);
+    };
+    if (cols > 0 && kb < ke) {                          // (whole 64 elements, hence whole rounds of AHEAD steps)
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int h = 0; h < AHEAD; ++h) fetch(kb + h * 8, h);
+      for (int k = kb; k < ke; k += AHEAD * 8)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = ce_mfma_native(a[i], b[j], acc[i][j]);
+        for (int h = 0; h < AHEAD; ++h) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            if (cols <= j * 32) break;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i][j] = ce_mfma_native(a[h][i], b[h][j], acc[i][j]);
+          }
+          fetch(k + (h + AHEAD) * 8, h);
+        }
     }
   }
   auto dma = [&](int k, int s) __attribute__((always_inline)) {
@@ -1061,9 +1077,10 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeSide u, CeSide v, int co
     const float unit = inv[0] * inv[1], c2 = unit * inv_tau * kCeLog2e;
     native = force || !ce_even(m[0]) || !ce_even(m[1]) || !(unit >= 0x1p-126f && unit < INFINITY && c2 >= 0x1p-125f && c2 < INFINITY);
     scale = sc[second];
-    if (blk == 0 && threadIdx.x == 0) {
-      amax[second] = native ? 0.f : __uint_as_float(m[second].bits);
-      if (!second) amax[2] = native ? 1.f : 0.f;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      amax[0] = native ? 0.f : __uint_as_float(m[0].bits);
+      amax[1] = native ? 0.f : __uint_as_float(m[1].bits);
+      amax[2] = native ? 1.f : 0.f;
     }
   }
   const int c0 = (threadIdx.x & 15) * 4;
@@ -1209,7 +1226,7 @@ namespace {
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 // Where everything sits in the caller's workspace.  The operands are used in place when a row is a multiple of 64 elements on
-// 16-byte boundaries, else copied once (padded; fp32 always: into its two pieces).  The gradients always have x from a copy, without what
+// 16-byte boundaries, else copied once (padded; fp32 into its two pieces unless x has few rows).  The gradients always have x from a copy, without what
 // ignored rows hold (a training step of 8192 x 65536 x 256 bf16: 1215 -> 1219 us).
 struct CePlan {
   int P, dt16, es, Dp, ldq, own;   // own: items a streaming workgroup holds
@@ -1237,8 +1254,11 @@ constexpr int kCePieceMiB[] = {512, 384, 256, 192, 128, 64};
 bool ce_streams(int D, int dtype) { return D <= (dtype == CRESTE_DT_F32 ? 128 : 256); }
 int ce_padded(int D, int dtype) { return ce_streams(D, dtype) ? (D <= 64 ? 64 : D <= 128 ? 128 : 256) : (int)up(D, 64); }
 
-bool ce_direct(const void* x, int64_t ld, int D, int dtype) {
-  return dtype != CRESTE_DT_F32 && D == ce_padded(D, dtype) && ld % 8 == 0 && ld < (1 << 24) && ((uintptr_t)x & 15) == 0;
+// 16-bit rows of whole padded widths are read in place, and fp32 ones where there are few rows of x (NATIVE then, ce_operands)
+bool ce_direct(const void* x, int64_t ld, int64_t N, int D, int dtype) {
+  const int part = dtype == CRESTE_DT_F32 ? 4 : 8;
+  return (dtype != CRESTE_DT_F32 || N <= kCeFewRows) && D == ce_padded(D, dtype) && ld % part == 0 && ld < (1 << 24) &&
+         ((uintptr_t)x & 15) == 0;
 }
 
 // rows that the few-rows kernel can read in place: whole 32-byte steps on 16-byte boundaries
@@ -1418,10 +1438,11 @@ int ce_operands(const CePlan& q, const void* x, int64_t ldx, const void* w, int6
       sw{w, V, ldw, (short*)(work + q.wp), V * q.Dp, nullptr, 0, nullptr};
   auto blocks = [](int64_t rows, int most) { const int64_t b = (rows + 15) / 16; return (int)(b > most ? most : b); };
   const int px = q.packx ? blocks(N, 2048) : 0, pw = q.packw ? blocks(V, 2048) : 0;
-  if (q.P == 2) {                                  // (both are copied)
-    const int ax = blocks(N, kCeMaxima), aw = blocks(V, kCeMaxima);
-    ce_amax_kernel<<<ax + aw, 256, 0, s>>>(sx, sw, D, ax, bmax, blow);
-    ce_pack_kernel<float><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, bmax, blow, ax, aw, inv_tau, N <= kCeFewRows, amax);
+  if (q.P == 2) {                                  // (x at least is copied where not the few-rows kernel takes both)
+    const bool force = N <= kCeFewRows;            // (as the few-rows kernel multiplies: no magnitudes asked for)
+    const int ax = force ? 0 : blocks(N, kCeMaxima), aw = force ? 0 : blocks(V, kCeMaxima);
+    if (!force) ce_amax_kernel<<<ax + aw, 256, 0, s>>>(sx, sw, D, ax, bmax, blow);
+    ce_pack_kernel<float><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, bmax, blow, ax, aw, inv_tau, force, amax);
   } else if (px + pw) {
     ce_pack_kernel<short><<<px + pw, 256, 0, s>>>(sx, sw, D, q.Dp, px, nullptr, nullptr, 0, 0, 0.f, false, nullptr);
   }
@@ -1462,7 +1483,7 @@ extern "C" int64_t creste_linear_ce_packs_bytes(const void* x, int64_t ldx, cons
                                                 int dtype) {
   if (creste_linear_ce_workspace_bytes(N, V, D, dtype, 0) < 0) return -1;
   if (ce_takes_few(x, ldx, w, ldw, N, D, dtype)) return 0;
-  return ce_plan(N, V, D, dtype, true, !ce_direct(w, ldw, D, dtype), false).packs;
+  return ce_plan(N, V, D, dtype, true, !ce_direct(w, ldw, N, D, dtype), false).packs;
 }
 
 extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* labels, int64_t N,
@@ -1473,7 +1494,7 @@ extern "C" int creste_linear_ce_forward(const void* x, int64_t ldx, const void* 
   if (bad) return bad;
   const bool few = ce_takes_few(x, ldx, w, ldw, N, D, dtype);
   // (a row of x only reaches its own softmax, so x need not be copied for what ignored rows hold -- unless the backward is to have it)
-  const CePlan q = ce_plan(N, V, D, dtype, !few && (packs || !ce_direct(x, ldx, D, dtype)), !few && !ce_direct(w, ldw, D, dtype),
+  const CePlan q = ce_plan(N, V, D, dtype, !few && (packs || !ce_direct(x, ldx, N, D, dtype)), !few && !ce_direct(w, ldw, N, D, dtype),
                            false);
   CRESTE_REQUIRE(loss && nll && rows && stat && work && work_bytes >= q.total, "linear_ce_forward: outputs / workspace (%lld of %lld bytes)",
                  (long long)work_bytes, (long long)q.total);
@@ -1519,7 +1540,7 @@ extern "C" int creste_linear_ce_backward(const void* x, int64_t ldx, const void*
                                          const void* packs, void* gx, void* gw, void* work, int64_t work_bytes, void* stream) {
   const int bad = ce_check(x, ldx, w, ldw, rows, N, V, D, dtype, temperature);
   if (bad) return bad;
-  const CePlan q = ce_plan(N, V, D, dtype, true, !ce_direct(w, ldw, D, dtype), true);
+  const CePlan q = ce_plan(N, V, D, dtype, true, !ce_direct(w, ldw, N, D, dtype), true);
   CRESTE_REQUIRE(stat && g_loss && (gx || gw) && work && work_bytes >= q.total, "linear_ce_backward: inputs / workspace (%lld of %lld bytes)",
                  (long long)work_bytes, (long long)q.total);
   CRESTE_REQUIRE((((uintptr_t)gx | (uintptr_t)gw | (uintptr_t)work | (uintptr_t)packs) & 15) == 0,

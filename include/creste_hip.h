@@ -705,7 +705,7 @@ int creste_irl_visitation_mix_f32(const float* exp_svf_raw, const uint8_t* fov, 
  *   forward : loss [1] (mean over the counted rows, 0 if there are none, or sum), nll [N] (0 where ignored), and for the backward
  *             rows [4][N rounded up to 64] 4-byte words (softmax statistics, labels) and stat [2] = {sum nll, count}.
  *   backward: gx [N][D], gw [V][D] (contiguous, 16-byte aligned, the features' type; either may be NULL) for the cotangent g_loss [1].
- * packs: the copies of the operands that the backward reads (x, and w where the kernels cannot read it in place: fp32, odd strides or
+ * packs: the copies of the operands that the backward reads (x, and w where the kernels cannot read it in place: fp32 beyond 32 rows, odd strides or
  *          widths), packs_bytes (0: the forward makes none).  Given a buffer (16-byte aligned) in both calls the forward's serve the
  *          backward; NULL: each makes its own in `work`.
  * work (16-byte aligned): workspace_bytes(..., train = 0) for the forward, train = 1 for the backward; -1 = sizes out of range. */

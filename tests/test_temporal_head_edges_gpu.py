@@ -234,6 +234,25 @@ def test_linear_ce_gradients_of_sure_rows(N, V, D, dt, tau):
         within(got, want, 1.01 * bound + half * want.abs() + tiny, name)
 
 
+@pytest.mark.parametrize("xo,wo", [(0, 0), (1, 0), (0, 1), (1, 1)])
+@pytest.mark.parametrize("N,V,D", [(32, 500, 64), (7, 500, 128), (20, 300, 320), (32, 300, 40)])
+def test_linear_ce_f32_few_rows_in_place_or_copied(N, V, D, xo, wo):
+    """up to 32 rows stay fp32 in both directions; rows off their 16 bytes are copied; kept copies or new ones: the same bits"""
+    x, w, labels = _uneven(N, V, D)
+
+    def at(t, off):
+        buf = torch.zeros(t.numel() + 4, device="cuda")
+        buf[off:off + t.numel()] = t.reshape(-1)
+        return buf[off:off + t.numel()].view(t.shape)
+    one, got = torch.ones((), device="cuda"), []
+    for keep in (False, True):
+        loss, nll, saved = ops.linear_ce(at(x, xo), at(w, wo), labels, temperature=0.1, keep=keep)
+        got.append((loss, nll, *ops.linear_ce_bwd(at(x, xo), at(w, wo), saved, one, temperature=0.1)))
+    assert all(torch.equal(u, v) for u, v in zip(*got))
+    _uneven_check(at(x, xo), at(w, wo), labels)
+    _uneven_check(at(x * 1e6, xo), at(w, wo), labels)                 # logits of 10^7
+
+
 # ------------------------------------------------------------------------------------------------------------ very many rows
 def test_linear_ce_more_than_2_29_rows():
     """four words a row for the backward pass 2^31 words; rows at both ends and around 2^29, all others ignored"""
