@@ -332,7 +332,9 @@ __device__ __forceinline__ void ce_gemm_body(const CeArgs& p) {
     // (columns of the output that are not there, most of them where there are few rows, stay 0)
     const int nw = n0 + wn * WTN, cols = nw >= p.n ? 0 : p.n - nw;
     const char* const first = p.a + (MODE == CE_GRAD || MODE == CE_DX ? p.class0 * p.lda : 0);      // (the piece's: rows are twice as long)
-    constexpr int AHEAD = 2;                            // steps in flight (a step's loads take longer than its products)
+    // steps in flight (a step's loads take longer than its products): a training step of 16 x 65536 x 512 394 us with one, 353 with two, 363
+    // with four, whose registers also cost a large uneven one (4096 x 65536 x 256: 6565 -> 7384)
+    constexpr int AHEAD = 2;
     cef4 a[AHEAD][MT], b[AHEAD][NT];
     auto fetch = [&](int k, int at) __attribute__((always_inline)) {
       k = k < ke ? k : ke - 8;
@@ -1254,7 +1256,8 @@ constexpr int kCePieceMiB[] = {512, 384, 256, 192, 128, 64};
 bool ce_streams(int D, int dtype) { return D <= (dtype == CRESTE_DT_F32 ? 128 : 256); }
 int ce_padded(int D, int dtype) { return ce_streams(D, dtype) ? (D <= 64 ? 64 : D <= 128 ? 128 : 256) : (int)up(D, 64); }
 
-// 16-bit rows of whole padded widths are read in place, and fp32 ones where there are few rows of x (NATIVE then, ce_operands)
+// 16-bit rows of whole padded widths are read in place, and fp32 ones where there are few rows of x (NATIVE then, ce_operands; a training
+// step of 16 x 65536 x 512: 294 us, 353 with a copy of w)
 bool ce_direct(const void* x, int64_t ld, int64_t N, int D, int dtype) {
   const int part = dtype == CRESTE_DT_F32 ? 4 : 8;
   return (dtype != CRESTE_DT_F32 || N <= kCeFewRows) && D == ce_padded(D, dtype) && ld % part == 0 && ld < (1 << 24) &&
